@@ -66,6 +66,13 @@ enum {
   TCL_VMODE_BILINEAR_THRESHOLD = 2 /* models/cpn.py:288-290: bilinear then (> 0.5)      */
 };
 
+/* element type of the tensors of the frame-attention entry points (tcl_rotate_positions, tcl_block_*, tcl_select_blocks) */
+enum {
+  TCL_DT_F32 = 0,
+  TCL_DT_BF16 = 1,
+  TCL_DT_F16 = 2
+};
+
 int tcl_version(void);
 const char *tcl_last_error(void);
 
@@ -248,6 +255,63 @@ int tcl_crop_flow(const float *flow, float *out, int64_t N, int64_t H, int64_t W
                   int64_t ch, int64_t cw, int64_t py, int64_t px, void *stream);
 /* resize_flow, utils/flow.py:87-90 (legacy nearest).  flow (N,H,W,2) -> out (N,oh,ow,2). */
 int tcl_resize_flow(const float *flow, float *out, int64_t N, int64_t H, int64_t W, int64_t oh, int64_t ow, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Frame attention: tokens of a target frame over the visible tokens of reference frames.  No counterpart in the reference, whose
+ *   all-pairs correlation (A1) is the quadratic form of the same question; these entry points answer it for whole feature maps and
+ *   long frame windows by attending to chosen blocks of reference tokens only.
+ *   Token tensors are (batch, token, head, channel) of `dtype`, addressed by element strides (sb, sn, sh) with dense channels;
+ *   Hq query heads share Hkv key heads in consecutive groups of G = Hq / Hkv.  Sums, statistics and accumulators are fp32 or wider.
+ *   tcl_block_*, tcl_select_blocks: D a multiple of 8 up to 128; token rows must start on 16 bytes.
+ * ------------------------------------------------------------------------------------------- */
+/*   Rotary positions over n_sections axes (1..4).  Section a of `sections` (a HOST array of even channel counts, in all at most D)
+ *   turns its channel pair i by positions[n][a] * base^(-2 i / sections[a]); a pair is channels (i, i + half) of the section, or
+ *   (2 i, 2 i + 1) when `interleaved`; channels behind the last section are copied.  positions: (N, n_sections) fp32 or int32, dense;
+ *   p_sb = elements to the next batch item's positions (0: all share one).  `inverse` negates the angle (the backward pass).
+ *   D even, up to 256.  y may be x. */
+int tcl_rotate_positions(const void *x, int64_t x_sb, int64_t x_sn, int64_t x_sh, const void *positions, int positions_int32, int64_t p_sb,
+                         void *y, int64_t y_sb, int64_t y_sn, int64_t y_sh, int64_t B, int64_t N, int64_t H, int64_t D,
+                         const int32_t *sections, int64_t n_sections, double base, int interleaved, int inverse, int dtype, void *stream);
+
+/*   Mean of the visible keys of every block of `block` (64 or 128) consecutive tokens: k (B,N,H,D), visible (B,N) fp32 (seen where
+ *   > 0.5; nullable: all) -> means fp32 (B,H,nb,D), counts int32 (B,nb), nb = ceil(N / block); a block without a visible key has mean
+ *   0 and count 0. */
+int tcl_block_means(const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh, const float *visible, float *means, int32_t *counts,
+                    int64_t B, int64_t N, int64_t H, int64_t D, int64_t block, int dtype, void *stream);
+
+/*   The blocks each group of queries attends to.  A group is q_block consecutive tokens with the G query heads of one key head; its
+ *   score of block j is <sum of its queries, means[j]> in 64 bits.  blocks int32 (B,Hkv,S,top_k), S = ceil(N / q_block): the top_k
+ *   best blocks with counts > 0 (ties to the lower index; a score of -inf or NaN is not chosen), in ascending order, -1 behind the
+ *   last.  nb up to 16,384. */
+size_t tcl_select_blocks_workspace_bytes(int64_t B, int64_t Hkv, int64_t S, int64_t nb, int64_t D);
+int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const float *means, const int32_t *counts, int32_t *blocks,
+                      int64_t B, int64_t N, int64_t H, int64_t Hkv, int64_t D, int64_t nb, int64_t top_k, int64_t q_block, int dtype,
+                      void *workspace, size_t workspace_bytes, void *stream);
+
+/*   out = softmax(scale q k^T) v over the visible keys of the blocks chosen for the query's group; a query that sees no key gets 0 and
+ *   lse = -inf.  visible as in tcl_block_means; blocks (B,Hkv,S,top_k) int32: an index outside [0, nb) is no block, a repeated one
+ *   counts once, order does not matter.  lse (B,Hq,Nq) fp32, natural logarithm, nullable (the backward pass needs it).
+ *   Limits: top_k <= 2048, nb <= 65,536, q_block * G <= 2^20 (q_block beyond Nq counts as Nq).
+ *   Contents of invisible keys do not matter (NaN and infinities included). */
+size_t tcl_block_attention_fwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block,
+                                               int64_t q_block);
+int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh,
+                            const void *v, int64_t v_sb, int64_t v_sn, int64_t v_sh, const float *visible, const int32_t *blocks,
+                            void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, float *lse,
+                            int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block, int64_t q_block,
+                            double scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+/*   grad_out like out -> g_q, g_k, g_v (each nullable); out and lse are the forward's.  Every row of the gradients is written (zero
+ *   for keys that no group sees), except in an empty attention (B, Nq or Nk of 0), where nothing is.  No atomics on values:
+ *   the same inputs give the same bits. */
+size_t tcl_block_attention_bwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block,
+                                               int64_t q_block);
+int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64_t g_sn, int64_t g_sh, const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
+                            const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+                            const float *visible, const int32_t *blocks, const void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, const float *lse,
+                            void *g_q, int64_t gq_sb, int64_t gq_sn, int64_t gq_sh, void *g_k, int64_t gk_sb, int64_t gk_sn, int64_t gk_sh,
+                            void *g_v, int64_t gv_sb, int64_t gv_sn, int64_t gv_sh,
+                            int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block, int64_t q_block,
+                            double scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

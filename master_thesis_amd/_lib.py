@@ -52,10 +52,20 @@ SIGNATURES = {
     "tcl_flow_add_identity": (_INT, [_P] * 2 + [_I64] * 3 + [_INT, _P]),
     "tcl_crop_flow": (_INT, [_P] * 2 + [_I64] * 7 + [_P]),
     "tcl_resize_flow": (_INT, [_P] * 2 + [_I64] * 5 + [_P]),
+    "tcl_rotate_positions": (_INT, [_P] + [_I64] * 3 + [_P, _INT, _I64, _P] + [_I64] * 7 + [_P, _I64, _c.c_double, _INT, _INT, _INT, _P]),
+    "tcl_block_means": (_INT, [_P] + [_I64] * 3 + [_P] * 3 + [_I64] * 5 + [_INT, _P]),
+    "tcl_select_blocks_workspace_bytes": (_SZ, [_I64] * 5),
+    "tcl_select_blocks": (_INT, [_P] + [_I64] * 3 + [_P] * 3 + [_I64] * 8 + [_INT, _P, _SZ, _P]),
+    "tcl_block_attention_fwd_workspace_bytes": (_SZ, [_I64] * 9),
+    "tcl_block_attention_fwd": (_INT, ([_P] + [_I64] * 3) * 3 + [_P] * 2 + [_P] + [_I64] * 3 + [_P] + [_I64] * 9 + [_c.c_double, _INT, _P, _SZ, _P]),
+    "tcl_block_attention_bwd_workspace_bytes": (_SZ, [_I64] * 9),
+    "tcl_block_attention_bwd": (_INT, ([_P] + [_I64] * 3) * 4 + [_P] * 2 + [_P] + [_I64] * 3 + [_P] + ([_P] + [_I64] * 3) * 3 + [_I64] * 9
+                                + [_c.c_double, _INT, _P, _SZ, _P]),
 }
 
 PREC_F32, PREC_BF16, PREC_BF16X3 = 0, 1, 2
 CTX_DEFAULT, CTX_COMPLETE, CTX_CM_MODULE = 0, 1, 2
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 VMODE_NONE, VMODE_NEAREST, VMODE_BILINEAR_THRESHOLD = 0, 1, 2
 
 _lib = None

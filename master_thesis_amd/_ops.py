@@ -606,3 +606,222 @@ class ResizeFlowFn(torch.autograd.Function):
         idx = (sy[:, None] * w + sx[None, :]).reshape(-1)
         gf.view(b, f, h * w, 2).index_add_(2, idx, g.reshape(b, f, oh * ow, 2))
         return gf, None
+
+
+# ----------------------------------------------------------------------------------------------- frame attention
+# Token tensors (B, N, H, D) in fp32, bf16 or fp16; the kernels read them through (batch, token, head) strides, so views of
+# (B, H, N, D) tensors and slices of a cache need no copy as long as channels are dense and rows start on 16 bytes.
+_DT = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+_plain_fwd = torch.amp.custom_fwd(device_type="cuda")
+
+
+def _tokens_device(what, *tensors):
+    """Device and dtype of token tensors (B,N,H,D), which have to share both."""
+    dev, dtype = tensors[0].device, tensors[0].dtype
+    for t in tensors:
+        if not t.is_cuda:
+            raise TclError("tcl ops run on the GPU only (got a %s tensor); there is no CPU fallback" % t.device)
+        if t.device != dev:
+            raise TclError("tensors on different devices: %s vs %s" % (dev, t.device))
+        if t.dtype not in _DT or t.dtype != dtype:
+            raise TclError("%s takes float32, bfloat16 or float16 tensors of one dtype (got %s and %s)" % (what, dtype, t.dtype))
+        if t.dim() != 4:
+            raise ValueError("%s takes tokens (batch, token, head, channel), got %s" % (what, tuple(t.shape)))
+    return dev
+
+
+def _side(what, t, dev, dtypes, shape):
+    """A plan tensor (mask, block list, summary): on `dev`, of one of `dtypes`, of this shape; made dense."""
+    if t.device != dev:
+        raise TclError("tensors on different devices: %s vs %s" % (dev, t.device))
+    if t.dtype not in dtypes:
+        raise TclError("%s must be %s (got %s)" % (what, " or ".join(str(d) for d in dtypes), t.dtype))
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must be %s, got %s" % (what, tuple(shape), tuple(t.shape)))
+    return t.detach().contiguous()
+
+
+def _visible(visible, dev, b, n):
+    if visible is None:
+        return None
+    v = _side("visible", visible, dev, (torch.float32, torch.bool), (b, n))
+    return v.float() if v.dtype == torch.bool else v
+
+
+def _strides(t):
+    """(batch, token, head) strides; the stride of a dimension of size one is never used."""
+    return tuple(0 if t.shape[i] == 1 else t.stride(i) for i in range(3))
+
+
+def _rows16(t):
+    """t itself if its channels are dense and every row starts on 16 bytes, else a dense copy."""
+    per = 16 // t.element_size()
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in _strides(t)):
+        return t
+    c = t.contiguous()
+    return c.clone() if c.data_ptr() % 16 else c
+
+
+class RotatePositionsFn(torch.autograd.Function):
+    @staticmethod
+    @_plain_fwd
+    def forward(ctx, x, positions, sections, base, interleaved):
+        ctx.meta = (sections, base, interleaved)
+        ctx.save_for_backward(positions)
+        return _rotate(x, positions, sections, base, interleaved, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @_bwd
+    def backward(ctx, g):
+        positions, = ctx.saved_tensors
+        return _rotate(g, positions, *ctx.meta, True), None, None, None, None
+
+
+def _rotate(x, positions, sections, base, interleaved, inverse):
+    b, n, h, d = x.shape
+    x = x if x.stride(3) == 1 or d == 1 else x.contiguous()
+    y = torch.empty_like(x)                   # keeps the order of x's dimensions; dense where x is an expanded view
+    if y.stride(3) != 1:
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    secs = (ctypes.c_int32 * len(sections))(*sections)
+    with _on(x.device):
+        _lib.call("tcl_rotate_positions", _p(x), *_strides(x), _p(positions), int(positions.dtype == torch.int32),
+                  n * len(sections) if positions.dim() == 3 else 0, _p(y), *_strides(y), b, n, h, d, secs, len(sections), base,
+                  int(interleaved), int(inverse), _DT[x.dtype], _stream(x.device))
+    return y
+
+
+def rotate_positions(x, positions, sections, base=10000.0, interleaved=False):
+    dev = _tokens_device("rotate_positions", x)
+    b, n, h, d = x.shape
+    sections = tuple(int(s) for s in sections)
+    if not 1 <= len(sections) <= 4 or any(s < 0 or s % 2 for s in sections) or sum(sections) > d:
+        raise ValueError("sections %s: 1 to 4 even channel counts, in all at most %d" % (sections, d))
+    if h < 1 or d % 2 or not 2 <= d <= 256:
+        raise ValueError("rotate_positions takes heads of an even size up to 256 (got %s)" % (tuple(x.shape),))
+    if not (base > 0 and base != float("inf")):
+        raise ValueError("base must be positive (got %r)" % (base,))
+    if positions.requires_grad:
+        raise TclError("positions are data: no gradient flows to them")
+    shape = (n, len(sections)) if positions.dim() == 2 else (b, n, len(sections))
+    pos = _side("positions", positions, dev, (torch.float32, torch.int32), shape)
+    return RotatePositionsFn.apply(x, pos, sections, float(base), bool(interleaved))
+
+
+def _head_size(what, d):
+    if d % 8 or not 8 <= d <= 128:
+        raise ValueError("%s takes heads of a multiple of 8 channels up to 128 (got %d)" % (what, d))
+
+
+def _block_size(block):
+    if block not in (64, 128):
+        raise ValueError("blocks hold 64 or 128 keys (got %r)" % (block,))
+
+
+def block_means(k, visible=None, block=64):
+    dev = _tokens_device("block_means", k)
+    b, n, h, d = k.shape
+    _head_size("block_means", d)
+    _block_size(block)
+    if h < 1:
+        raise ValueError("block_means needs at least one head")
+    vis = _visible(visible, dev, b, n)
+    nb = -(-n // block)
+    kc = _rows16(k.detach())
+    means = torch.empty((b, h, nb, d), dtype=torch.float32, device=dev)
+    counts = torch.empty((b, nb), dtype=torch.int32, device=dev)
+    with _on(dev):
+        _lib.call("tcl_block_means", _p(kc), *_strides(kc), _p(vis), _p(means), _p(counts), b, n, h, d, block, _DT[k.dtype], _stream(dev))
+    return means, counts
+
+
+def select_blocks(q, means, counts, top_k, q_block=64):
+    dev = _tokens_device("select_blocks", q)
+    b, n, h, d = q.shape
+    _head_size("select_blocks", d)
+    top_k, q_block = int(top_k), int(q_block)
+    if top_k < 1 or q_block < 1:
+        raise ValueError("top_k and q_block start at 1 (got %d, %d)" % (top_k, q_block))
+    if means.dim() != 4 or means.shape[1] < 1 or h < 1 or h % means.shape[1]:
+        raise ValueError("means %s do not fit %d query heads" % (tuple(means.shape), h))
+    hk, nb = means.shape[1], means.shape[2]
+    mc = _side("means", means, dev, (torch.float32,), (b, hk, nb, d))
+    cc = _side("counts", counts, dev, (torch.int32,), (b, nb))
+    s = -(-n // q_block)
+    qc = q.detach() if q.stride(3) == 1 else q.detach().contiguous()
+    blocks = torch.empty((b, hk, s, top_k), dtype=torch.int32, device=dev)
+    ws = _workspace(_lib.lib().tcl_select_blocks_workspace_bytes(b, hk, s, nb, d), dev)
+    with _on(dev):
+        _lib.call("tcl_select_blocks", _p(qc), *_strides(qc), _p(mc), _p(cc), _p(blocks), b, n, h, hk, d, nb, top_k, q_block, _DT[q.dtype],
+                  _p(ws), ws.numel(), _stream(dev))
+    return blocks
+
+
+class BlockAttentionFn(torch.autograd.Function):
+    """-> out (B,Nq,Hq,D), lse (B,Hq,Nq) | None.  Gradients flow to q, k and v through out; blocks and visible are data, lse is a
+    statistic."""
+
+    @staticmethod
+    @_plain_fwd
+    def forward(ctx, q, k, v, blocks, visible, block, q_block, scale, want_lse):
+        dev = q.device
+        b, nq, hq, d = q.shape
+        nk, hk = k.shape[1], k.shape[2]
+        top = blocks.shape[3]
+        qc, kc, vc = _rows16(q), _rows16(k), _rows16(v)
+        out = torch.empty((b, nq, hq, d), dtype=q.dtype, device=dev)
+        lse = torch.empty((b, hq, nq), dtype=torch.float32, device=dev) if want_lse or any(ctx.needs_input_grad[:3]) else None
+        ws = _workspace(_lib.lib().tcl_block_attention_fwd_workspace_bytes(b, nq, nk, hq, hk, d, top, block, q_block), dev)
+        with _on(dev):
+            _lib.call("tcl_block_attention_fwd", _p(qc), *_strides(qc), _p(kc), *_strides(kc), _p(vc), *_strides(vc), _p(visible), _p(blocks),
+                      _p(out), *_strides(out), _p(lse), b, nq, nk, hq, hk, d, top, block, q_block, scale, _DT[q.dtype],
+                      _p(ws), ws.numel(), _stream(dev))
+        ctx.save_for_backward(qc, kc, vc, blocks, visible, out, lse)
+        ctx.meta = (block, q_block, scale)
+        if lse is not None:
+            ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @_bwd
+    def backward(ctx, g_out, _g_lse):
+        q, k, v, blocks, visible, out, lse = ctx.saved_tensors
+        block, q_block, scale = ctx.meta
+        b, nq, hq, d = q.shape
+        nk, hk = k.shape[1], k.shape[2]
+        top, dev = blocks.shape[3], q.device
+        make = torch.empty if nq and nk else torch.zeros
+        g_q, g_k, g_v = (make(t.shape, dtype=t.dtype, device=dev) if need else None for t, need in zip((q, k, v), ctx.needs_input_grad))
+        none = (0, 0, 0)
+        go = _rows16(g_out)
+        ws = _workspace(_lib.lib().tcl_block_attention_bwd_workspace_bytes(b, nq, nk, hq, hk, d, top, block, q_block), dev)
+        with _on(dev):
+            _lib.call("tcl_block_attention_bwd", _p(go), *_strides(go), _p(q), *_strides(q), _p(k), *_strides(k), _p(v), *_strides(v),
+                      _p(visible), _p(blocks), _p(out), *_strides(out), _p(lse),
+                      _p(g_q), *(none if g_q is None else _strides(g_q)), _p(g_k), *(none if g_k is None else _strides(g_k)),
+                      _p(g_v), *(none if g_v is None else _strides(g_v)),
+                      b, nq, nk, hq, hk, d, top, block, q_block, scale, _DT[q.dtype], _p(ws), ws.numel(), _stream(dev))
+        return g_q, g_k, g_v, None, None, None, None, None, None
+
+
+def block_attention(q, k, v, blocks, visible=None, block=64, q_block=64, scale=None, return_lse=False):
+    if torch.is_autocast_enabled("cuda"):      # as torch's own attention: the operands of the products take the region's type
+        q, k, v = (t.to(torch.get_autocast_dtype("cuda")) if t.is_floating_point() and t.is_cuda else t for t in (q, k, v))
+    dev = _tokens_device("block_attention", q, k, v)
+    b, nq, hq, d = q.shape
+    nk, hk = k.shape[1], k.shape[2]
+    _head_size("block_attention", d)
+    _block_size(block)
+    q_block = int(q_block)
+    if q_block < 1:
+        raise ValueError("q_block starts at 1 (got %d)" % q_block)
+    if tuple(k.shape) != (b, nk, hk, d) or v.shape != k.shape or hk < 1 or hq < 1 or hq % hk:
+        raise ValueError("queries %s do not fit keys %s and values %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if blocks.dim() != 4 or blocks.shape[3] < 1:
+        raise ValueError("blocks must be (batch, key head, group, choice), got %s" % (tuple(blocks.shape),))
+    bl = _side("blocks", blocks, dev, (torch.int32,), (b, hk, -(-nq // q_block), blocks.shape[3]))
+    vis = _visible(visible, dev, b, nk)
+    out, lse = BlockAttentionFn.apply(q, k, v, bl, vis, block, q_block, float(d ** -0.5 if scale is None else scale), bool(return_lse))
+    return (out, lse) if return_lse else out

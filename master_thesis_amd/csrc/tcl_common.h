@@ -11,6 +11,7 @@ namespace tcl {
 
 int set_error(int code, const char *fmt, ...);  // records the thread-local message, returns code
 int check_launch(const char *what);             // hipGetLastError -> TCL_ERR_LAUNCH
+bool lds_ready(const void *kernel, size_t lds);  // may `kernel` be launched with `lds` bytes of dynamic LDS?  Raises its limit once per device
 
 inline bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 inline size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }

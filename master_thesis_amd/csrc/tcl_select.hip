@@ -1,0 +1,348 @@
+// Block summaries and block selection of the frame attention: tcl_block_means, tcl_select_blocks.
+//
+// Keys lie in blocks of 64 or 128 consecutive tokens.  A block is summarised by the mean of its visible keys; a group of queries
+// (q_block consecutive tokens with all query heads of one key head) scores block j by <sum of its queries, mean_j> and takes the
+// top_k best blocks that have a visible key.  A choice is a comparison of values that can lie arbitrarily close, so sums, products
+// and comparisons are all carried in 64 bits: a result of fp32 scores would depend on the order of summation.
+#include "tcl_common.h"
+
+namespace tcl {
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, int V> struct SelVec { typedef T type __attribute__((ext_vector_type(V))); };
+
+// ------------------------------------------------------------------------------------------ block means
+struct MeansArgs {
+  const void *k;
+  const float *vis;
+  float *means;
+  int32_t *counts;
+  int64_t sb, sn, sh;
+  int B, N, H, D, block, nb;
+};
+
+// One wave per (item, head, block).  A row takes D / VE lanes (16-byte loads), so 64 / (D / VE) rows are read per step, four steps in
+// flight; every lane sums its channels of its rows in 64 bits, the row groups are joined through LDS.
+// Bound: memory (K once).
+template <typename T>
+__global__ __launch_bounds__(256) void block_means_kernel(MeansArgs a) {
+  constexpr int VE = 16 / sizeof(T);
+  typedef typename SelVec<T, VE>::type vec;
+  __shared__ double part[4][64 * VE];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int64_t items = (int64_t)a.B * a.H * a.nb;
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+  const bool live = id < items;
+  const int64_t w = live ? id : items - 1;
+  // heads innermost: the waves of one workgroup read neighbouring rows of the same tokens
+  const int h = (int)(w % a.H);
+  const int64_t bj = w / a.H;
+  const int j = (int)(bj % a.nb), b = (int)(bj / a.nb);
+  const int n0 = j * a.block;
+  uint64_t seen[2];
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = i * 64 + lane, n = n0 + r;
+    bool ok = r < a.block && n < a.N;
+    if (ok && a.vis) ok = a.vis[(int64_t)b * a.N + n] > 0.5f;
+    seen[i] = __ballot(ok);
+    count += __popcll(seen[i]);
+  }
+  const int lr = a.D / VE, rp = 64 / lr;             // lanes of a row, rows of a step
+  const int rg = lane / lr, ch = (lane - rg * lr) * VE;
+  const bool in = rg < rp;
+  double acc[VE] = {};
+  const T *base = reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sb + (int64_t)h * a.sh + ch;
+  const int last = min(a.block, a.N - n0) - 1;
+  for (int r0 = 0; r0 <= last; r0 += 4 * rp) {
+    vec t[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = min(r0 + u * rp + (in ? rg : 0), last);
+      t[u] = *reinterpret_cast<const vec *>(base + (int64_t)(n0 + r) * a.sn);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + u * rp + rg;
+      const bool use = in && r <= last && ((seen[r >= 64] >> (r & 63)) & 1);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[e] += use ? (double)(float)t[u][e] : 0.0;
+    }
+  }
+  if (in) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) part[wave][rg * a.D + ch + e] = acc[e];
+  }
+  __syncthreads();
+  if (!live) return;
+  const int64_t row = ((int64_t)b * a.H + h) * a.nb + j;
+  for (int c = lane; c < a.D; c += 64) {
+    double sum = 0.0;
+    for (int g = 0; g < rp; ++g) sum += part[wave][g * a.D + c];
+    a.means[row * a.D + c] = (float)(sum / (double)max(count, 1));
+  }
+  if (h == 0 && lane == 0) a.counts[(int64_t)b * a.nb + j] = count;
+}
+
+// ------------------------------------------------------------------------------------------ selection
+struct SelectArgs {
+  const void *q;
+  const float *means;
+  const int32_t *counts;
+  int32_t *blocks;
+  double *pooled;      // (B, Hkv, S, D)
+  uint64_t *keys;      // (B, Hkv, S, nb)
+  int64_t sb, sn, sh;
+  int B, N, H, Hkv, G, D, nb, top, q_block, S;
+};
+
+// sum of the queries of one group, 64 bits.  One wave per (item, key head, group); a lane owns channels lane and lane + 64.
+template <typename T>
+__global__ __launch_bounds__(256) void select_pool_kernel(SelectArgs a) {
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+  if (id >= (int64_t)a.B * a.Hkv * a.S) return;
+  const int s = (int)(id % a.S);
+  const int64_t bh = id / a.S;
+  const int hk = (int)(bh % a.Hkv), b = (int)(bh / a.Hkv);
+  const T *q = reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sb + (int64_t)hk * a.G * a.sh;
+  const int n0 = (int)((int64_t)s * a.q_block), n1 = (int)min((int64_t)a.N, (int64_t)n0 + a.q_block);
+  for (int c = lane; c < a.D; c += 64) {
+    double sum = 0.0;
+    for (int n = n0; n < n1; ++n)
+      for (int g = 0; g < a.G; ++g) sum += (double)(float)q[(int64_t)n * a.sn + (int64_t)g * a.sh + c];
+    a.pooled[id * a.D + c] = sum;
+  }
+}
+
+// Order-preserving map of a score to 64 bits; 0 is reserved for "cannot be chosen" (no visible key, a score of -inf or NaN).
+__device__ __forceinline__ uint64_t score_key(double s, bool can) {
+  s += 0.0;                                                     // -0 and +0 tie
+  const uint64_t u = (uint64_t)__double_as_longlong(s);
+  const uint64_t m = (u >> 63) ? ~u : (u | (1ull << 63));
+  return can && s > -__builtin_inf() ? m : 0ull;
+}
+
+// scores of 16 groups x 16 blocks per wave with v_mfma_f64_16x16x4: lane l holds row (column) l % 16 of both operands and, in a
+// slice of 16 channels, channels 4 (l / 16) .. + 3, one of them per instruction.
+__global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int r = lane % 16, g = lane / 16;
+  const int64_t bh = blockIdx.z;
+  const int s0 = blockIdx.y * 16, j0 = (blockIdx.x * 4 + wave) * 16;
+  if (j0 >= a.nb) return;
+  const int b = (int)(bh / a.Hkv);
+  const int s = min(s0 + r, a.S - 1), j = min(j0 + r, a.nb - 1);
+  const double *qp = a.pooled + (bh * a.S + s) * a.D;
+  const float *mp = a.means + (bh * a.nb + j) * a.D;
+  f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+  for (int c0 = 0; c0 < a.D; c0 += 16) {
+    const int c = c0 + 4 * g;
+    const bool in = c < a.D;                                    // D is a multiple of 8
+    double qv[4];
+    float mv[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      qv[e] = in ? qp[c + e] : 0.0;
+      mv[e] = in ? mp[c + e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(qv[e], (double)mv[e], acc, 0, 0, 0);
+  }
+  // result: column l % 16, rows l / 16 + 4 i
+  const int col = j0 + r;
+  const bool can = col < a.nb && a.counts[(int64_t)b * a.nb + col] > 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = s0 + g + 4 * i;
+    if (row < a.S && col < a.nb) a.keys[(bh * a.S + row) * a.nb + col] = score_key(acc[i], can);
+  }
+}
+
+// The top_k largest keys of one row, ties to the lower index, ascending, -1 behind the last.  One wave per row, R keys per lane.
+// The threshold is found bit by bit from the top (how many keys are >= the candidate?), and the search ends as soon as exactly
+// the wanted number passes.
+template <int R>
+__global__ __launch_bounds__(256) void select_topk_wave_kernel(SelectArgs a) {
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  if (row >= (int64_t)a.B * a.Hkv * a.S) return;
+  uint64_t key[R];
+  int valid = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int j = i * 64 + lane;
+    key[i] = j < a.nb ? a.keys[row * a.nb + j] : 0ull;
+    valid += __popcll(__ballot(key[i] != 0));
+  }
+  const int want = min(a.top, valid);
+  uint64_t t = 1;                                               // everything that can be chosen
+  int have = valid;
+  if (have > want) {
+    t = 0;
+    for (int bit = 63; bit >= 0 && have != want; --bit) {
+      const uint64_t cand = t | (1ull << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= cand));
+      if (n >= want) { t = cand; have = n; }
+    }
+  }
+  int spare = have - want;                                      // keys equal to t that have to stay out: the last ones
+  int equal = 0;
+  if (spare > 0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) equal += __popcll(__ballot(key[i] == t));
+    equal -= spare;                                             // how many of them stay in
+  }
+  int32_t *out = a.blocks + row * a.top;
+  const uint64_t below = (1ull << lane) - 1;
+  int at = 0, eq = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const bool same = spare > 0 && key[i] == t;
+    const uint64_t sm = __ballot(same);
+    const bool in = key[i] >= t && want > 0 && (!same || eq + __popcll(sm & below) < equal);
+    const uint64_t m = __ballot(in);
+    if (in) out[at + __popcll(m & below)] = i * 64 + lane;
+    at += __popcll(m);
+    eq += __popcll(sm);
+  }
+  for (int i = at + lane; i < a.top; i += 64) out[i] = -1;
+}
+
+// The same for long rows: one workgroup per row, the keys in LDS.
+__global__ __launch_bounds__(256) void select_topk_block_kernel(SelectArgs a) {
+  extern __shared__ uint64_t lkey[];
+  __shared__ int lsum[2][4];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int64_t row = blockIdx.x;
+  const int padded = (a.nb + 255) / 256 * 256;
+  int flip = 0;
+  auto total = [&](int n) {                                     // n is wave-uniform
+    if (lane == 0) lsum[flip][wave] = n;
+    __syncthreads();
+    const int t = lsum[flip][0] + lsum[flip][1] + lsum[flip][2] + lsum[flip][3];
+    flip ^= 1;                                                  // the other half: no second barrier needed before the next write
+    return t;
+  };
+  auto count = [&](uint64_t c) {
+    int n = 0;
+    for (int j = threadIdx.x; j < padded; j += 256) n += __popcll(__ballot(lkey[j] >= c));
+    return total(n);
+  };
+  for (int j = threadIdx.x; j < padded; j += 256) lkey[j] = j < a.nb ? a.keys[row * a.nb + j] : 0ull;
+  __syncthreads();
+  const int valid = count(1);
+  const int want = min(a.top, valid);
+  uint64_t t = 1;
+  int have = valid;
+  if (have > want) {
+    t = 0;
+    for (int bit = 63; bit >= 0 && have != want; --bit) {
+      const uint64_t cand = t | (1ull << bit);
+      const int n = count(cand);
+      if (n >= want) { t = cand; have = n; }
+    }
+  }
+  const int spare = have - want;
+  int equal = 0;
+  if (spare > 0) {
+    int n = 0;
+    for (int j = threadIdx.x; j < padded; j += 256) n += __popcll(__ballot(lkey[j] == t));
+    equal = total(n) - spare;
+  }
+  int32_t *out = a.blocks + row * a.top;
+  if (wave != 0) return;
+  const uint64_t below = (1ull << lane) - 1;
+  int at = 0, eq = 0;
+  for (int j = lane; j < padded; j += 64) {
+    const uint64_t key = lkey[j];
+    const bool same = spare > 0 && key == t;
+    const uint64_t sm = __ballot(same);
+    const bool in = key >= t && want > 0 && (!same || eq + __popcll(sm & below) < equal);
+    const uint64_t m = __ballot(in);
+    if (in) out[at + __popcll(m & below)] = j;
+    at += __popcll(m);
+    eq += __popcll(sm);
+  }
+  for (int i = at + lane; i < a.top; i += 64) out[i] = -1;
+}
+
+constexpr int64_t kMaxBlocks = 16384;   // keys of one row in LDS: 128 KB
+constexpr int kWaveKeys = 8;            // up to 512 blocks a wave holds the row in registers
+
+static size_t pooled_bytes(int64_t B, int64_t Hkv, int64_t S, int64_t D) { return round_up((size_t)(B * Hkv * S * D) * sizeof(double), 256); }
+
+template <typename T> static void launch_pool(const SelectArgs &a, unsigned blocks, hipStream_t s) {
+  hipLaunchKernelGGL((select_pool_kernel<T>), dim3(blocks), dim3(256), 0, s, a);
+}
+
+}  // namespace tcl
+
+using namespace tcl;
+
+extern "C" int tcl_block_means(const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh, const float *visible, float *means, int32_t *counts,
+                               int64_t B, int64_t N, int64_t H, int64_t D, int64_t block, int dtype, void *stream) {
+  TCL_REQUIRE(B >= 0 && N >= 0 && H > 0 && B < (1LL << 31) && N < (1LL << 31) && H < (1LL << 31), TCL_ERR_SHAPE, "block_means: bad shape");
+  TCL_REQUIRE(D > 0 && D % 8 == 0 && D <= 128, TCL_ERR_UNSUPPORTED, "block_means: head size %ld (a multiple of 8 up to 128)", (long)D);
+  TCL_REQUIRE(block == 64 || block == 128, TCL_ERR_UNSUPPORTED, "block_means: blocks of 64 or 128 keys (got %ld)", (long)block);
+  TCL_REQUIRE(dtype == TCL_DT_F32 || dtype == TCL_DT_BF16 || dtype == TCL_DT_F16, TCL_ERR_UNSUPPORTED, "block_means: unknown dtype %d", dtype);
+  if (B == 0 || N == 0) return TCL_OK;
+  TCL_REQUIRE(k && means && counts, TCL_ERR_ARG, "block_means: null pointer");
+  const int64_t ve = dtype == TCL_DT_F32 ? 4 : 8;
+  TCL_REQUIRE(aligned(k, 16) && k_sb % ve == 0 && k_sn % ve == 0 && k_sh % ve == 0, TCL_ERR_ARG, "block_means: key rows must start on 16 bytes");
+  MeansArgs a{k, visible, means, counts, k_sb, k_sn, k_sh, (int)B, (int)N, (int)H, (int)D, (int)block, (int)cdiv(N, block)};
+  const int64_t blocks = cdiv(B * H * a.nb, 4);
+  TCL_REQUIRE(blocks < (1LL << 31), TCL_ERR_SHAPE, "block_means: grid of %ld blocks", (long)blocks);
+  const dim3 grid((unsigned)blocks);
+  const hipStream_t s = (hipStream_t)stream;
+  if (dtype == TCL_DT_F32) hipLaunchKernelGGL((block_means_kernel<float>), grid, dim3(256), 0, s, a);
+  else if (dtype == TCL_DT_BF16) hipLaunchKernelGGL((block_means_kernel<__bf16>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((block_means_kernel<_Float16>), grid, dim3(256), 0, s, a);
+  return check_launch("block_means");
+}
+
+extern "C" size_t tcl_select_blocks_workspace_bytes(int64_t B, int64_t Hkv, int64_t S, int64_t nb, int64_t D) {
+  if (B <= 0 || Hkv <= 0 || S <= 0 || nb <= 0 || D <= 0) return 256;
+  return pooled_bytes(B, Hkv, S, D) + round_up((size_t)(B * Hkv * S * nb) * sizeof(uint64_t), 256);
+}
+
+extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const float *means, const int32_t *counts, int32_t *blocks,
+                                 int64_t B, int64_t N, int64_t H, int64_t Hkv, int64_t D, int64_t nb, int64_t top_k, int64_t q_block, int dtype,
+                                 void *workspace, size_t workspace_bytes, void *stream) {
+  TCL_REQUIRE(B >= 0 && N >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && nb >= 0 && top_k > 0 && q_block > 0, TCL_ERR_SHAPE, "select_blocks: bad shape");
+  TCL_REQUIRE(B < (1LL << 31) && N < (1LL << 31) && H < (1LL << 31) && top_k < (1LL << 31) && q_block < (1LL << 31), TCL_ERR_SHAPE, "select_blocks: bad shape");
+  TCL_REQUIRE(D > 0 && D % 8 == 0 && D <= 128, TCL_ERR_UNSUPPORTED, "select_blocks: head size %ld (a multiple of 8 up to 128)", (long)D);
+  TCL_REQUIRE(nb <= kMaxBlocks, TCL_ERR_UNSUPPORTED, "select_blocks: %ld blocks (at most %ld)", (long)nb, (long)kMaxBlocks);
+  TCL_REQUIRE(dtype == TCL_DT_F32 || dtype == TCL_DT_BF16 || dtype == TCL_DT_F16, TCL_ERR_UNSUPPORTED, "select_blocks: unknown dtype %d", dtype);
+  const int64_t S = cdiv(N, q_block), rows = B * Hkv * S;
+  if (rows == 0) return TCL_OK;
+  TCL_REQUIRE(q && blocks && (nb == 0 || (means && counts)), TCL_ERR_ARG, "select_blocks: null pointer");
+  TCL_REQUIRE(rows < (1LL << 31) && B * Hkv < 65536 && cdiv(S, 16) < 65536, TCL_ERR_SHAPE, "select_blocks: %ld groups are too many for one call", (long)rows);
+  const size_t need = tcl_select_blocks_workspace_bytes(B, Hkv, S, nb, D);
+  TCL_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, TCL_ERR_WORKSPACE, "select_blocks: workspace of %zu bytes needed", need);
+  SelectArgs a{q, means, counts, blocks, (double *)workspace, nullptr, q_sb, q_sn, q_sh, (int)B, (int)N, (int)H, (int)Hkv, (int)(H / Hkv), (int)D, (int)nb,
+               (int)top_k, (int)q_block, (int)S};
+  a.keys = (uint64_t *)((char *)workspace + pooled_bytes(B, Hkv, S, D));
+  const hipStream_t s = (hipStream_t)stream;
+  if (nb > 0) {
+    const unsigned pb = (unsigned)cdiv(rows, 4);
+    if (dtype == TCL_DT_F32) launch_pool<float>(a, pb, s);
+    else if (dtype == TCL_DT_BF16) launch_pool<__bf16>(a, pb, s);
+    else launch_pool<_Float16>(a, pb, s);
+    hipLaunchKernelGGL(select_score_kernel, dim3((unsigned)cdiv(nb, 64), (unsigned)cdiv(S, 16), (unsigned)(B * Hkv)), dim3(256), 0, s, a);
+  }
+  const dim3 wg((unsigned)cdiv(rows, 4));
+  if (nb <= 64) hipLaunchKernelGGL((select_topk_wave_kernel<1>), wg, dim3(256), 0, s, a);
+  else if (nb <= 256) hipLaunchKernelGGL((select_topk_wave_kernel<4>), wg, dim3(256), 0, s, a);
+  else if (nb <= 64 * kWaveKeys) hipLaunchKernelGGL((select_topk_wave_kernel<kWaveKeys>), wg, dim3(256), 0, s, a);
+  else {
+    const size_t lds = (size_t)(nb + 255) / 256 * 256 * sizeof(uint64_t);
+    TCL_REQUIRE(lds_ready((const void *)select_topk_block_kernel, lds), TCL_ERR_LAUNCH, "select_blocks: the device refuses %zu bytes of LDS", lds);
+    hipLaunchKernelGGL(select_topk_block_kernel, dim3((unsigned)rows), dim3(256), lds, s, a);
+  }
+  return check_launch("select_blocks");
+}
