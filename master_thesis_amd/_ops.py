@@ -654,9 +654,10 @@ def _strides(t):
 
 
 def _rows16(t):
-    """t itself if its channels are dense and every row starts on 16 bytes, else a dense copy."""
-    per = 16 // t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in _strides(t)):
+    """t itself if its channels are dense, every row starts on 16 bytes and tokens lie less than 2^22 elements apart, else a dense
+    copy."""
+    per, st = 16 // t.element_size(), _strides(t)
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in st) and st[1] < 1 << 22:
         return t
     c = t.contiguous()
     return c.clone() if c.data_ptr() % 16 else c

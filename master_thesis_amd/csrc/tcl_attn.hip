@@ -4,12 +4,17 @@
 //   (0, and lse = -inf, where nothing is visible).
 //
 // All products run on the matrix pipe in one shape, 16 x 16 with 32 k-elements per step (one v_mfma_f32_16x16x32 for 16-bit
-// operands, eight v_mfma_f32_16x16x4_f32 for fp32): lane l holds row (column) l % 16 of an operand and 8 consecutive
-// k-elements of the quarter l / 16; the result has column l % 16 and rows 4 (l / 16) .. + 3.  The order of the k-elements is free
-// as long as both operands share it, and that is what keeps the probabilities in registers: S^T = K Q^T leaves a lane 4 + 4
-// probabilities of ITS query (two 16-key tiles), which are, as they are, the second operand of O^T = V^T P^T once V^T is read
-// in the same key order.  For that V lies in LDS in quads of 4 keys, [key / 4][channel][key % 4].  The backward products use the same
-// two forms (rows as they are for contractions over channels, quads for contractions over tokens).
+// operands, eight v_mfma_f32_16x16x4_f32 for fp32): lane l holds row (column) l % 16 of an operand and 8 k-elements of the quarter
+// l / 16; the result has column l % 16 and rows 4 (l / 16) .. + 3.  The order of the k-elements is free as long as both operands
+// share it, and that is what keeps the probabilities in registers: S^T = K Q^T leaves a lane 4 + 4 probabilities of ITS query (two
+// 16-key tiles), which are, as they are, the second operand of O^T = V^T P^T once V^T is read in the same key order: for 16-bit
+// types with the transposing LDS read, for fp32 element by element.  So every tensor has ONE image in LDS, rows as they lie in
+// memory, for contractions over channels and over tokens alike.
+//
+// Tiles go from memory to LDS without passing registers (16-byte pieces, global_load_lds), one tile ahead of the products: an image
+// is a run of 1 KiB pieces that a wave's 64 lanes fill in lane order, so the order of the 16-byte chunks within a row is turned
+// (an exclusive or with bits of the row) on the SOURCE side, such that both ways of reading hit every bank once.  Rows that are not to be
+// seen are read from 16 zero bytes instead: what lies in a hole never reaches a product.
 //
 // Statistics (running maximum, sum, lse, rowsum(dout o out)) and all accumulators are fp32.  16-bit inputs: the probabilities and the
 // score gradients are rounded to the inputs' type as operands of the second product (half a step of it relative to each
@@ -64,87 +69,89 @@ struct AttnArgs {
   FastDiv by_g, by_rows;
 };
 
-// LDS images of a tile of TK token rows x DP channels
-template <typename T, int DP> struct Lay {
+// LDS image of token rows of DP channels: NCH chunks of 16 bytes per row (a power of two)
+template <typename T, int DP> struct Img {
   static constexpr int VE = 16 / sizeof(T);
-  static constexpr int LD = DP + VE;                                  // rows, + 16 bytes: 16 lanes reading 16 bytes each of 16 rows hit every bank once
-  static constexpr int QD = 4 * (DP + (sizeof(T) == 2 ? 16 : 0));     // quads of 4 tokens (16-bit: + 128 bytes, so that the two quads of a half wave use different banks)
-  static constexpr size_t rows(int tk) { return (size_t)tk * LD * sizeof(T); }
-  static constexpr size_t quads(int tk) { return (size_t)tk / 4 * QD * sizeof(T); }
+  static constexpr int NCH = DP / VE <= 4 ? 4 : DP / VE <= 8 ? 8 : DP / VE <= 16 ? 16 : 32;
+  static constexpr int RB = NCH * 16;
+  // chunk c of row r lies at c ^ swz(r): 16 rows reading one chunk, and 8 rows reading two neighbouring ones, hit different banks
+  __device__ __forceinline__ static int swz(int r) {
+    if (NCH == 4) return ((r >> 2) & 1) << 1 | ((r >> 3) & 1);
+    if (NCH == 8) return ((r >> 1) & 3) << 1 | ((r >> 3) & 1);
+    return (r & 7) << 1 | ((r >> 3) & 1);
+  }
 };
 
-// the 8 k-elements of a lane for a contraction over channels
-template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type row_frag(const T *rows, int row, int ch) {
-  return *reinterpret_cast<const typename Vec8<T>::type *>(rows + row * Lay<T, DP>::LD + ch);
+typedef __attribute__((address_space(3))) void *lds_vptr;
+typedef const __attribute__((address_space(1))) void *glb_cvptr;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+static __device__ __attribute__((aligned(16))) const uint32_t g_zero_chunk[4] = {0, 0, 0, 0};
+
+__device__ __forceinline__ void dma16(const char *src, char *lds) {   // lds: of the wave's first lane
+  __builtin_amdgcn_global_load_lds((glb_cvptr)src, (lds_vptr)lds, 16, 0, 0);
 }
-// ... over the 32 tokens that start at t0: tokens t0 + 4 g .. + 3 and t0 + 16 + 4 g .. + 3 of channel d
-template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type quad_frag(const T *quads, int t0, int g, int d) {
-  typedef typename Vec4<T>::type v4;
-  const T *p = quads + (t0 / 4 + g) * Lay<T, DP>::QD + d * 4;
-  const v4 a = *reinterpret_cast<const v4 *>(p), b = *reinterpret_cast<const v4 *>(p + 4 * Lay<T, DP>::QD);
-  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+// every LDS-DMA of this wave has landed and every LDS read of it has been served; then the workgroup meets
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
-// A tile's global loads, kept in registers until the barrier that frees the LDS tile: 16-byte pieces of rows
-template <typename T, int DP, int TK> struct RowStage {
-  typedef T vec __attribute__((ext_vector_type(Lay<T, DP>::VE)));
-  static constexpr int VE = Lay<T, DP>::VE, PER = DP / VE, NU = TK * PER / 256;
-  static_assert(TK * PER % 256 == 0, "whole pieces per thread");
-  vec r[NU];
-  // at(row) -> pointer to the row's first channel, or null for a row of zeros
-  template <typename F> __device__ __forceinline__ void load(F at, int D) {
+// ROWS rows -> image.  at(row) -> pointer to the row's first channel, or null for a row of zeros; chunks beyond `chunks` are zeros.
+// Called by all 256 threads.
+template <typename T, int DP, int ROWS, typename F> __device__ __forceinline__ void dma_rows(char *img, int chunks, F at) {
+  typedef Img<T, DP> I;
+  constexpr int PIECES = ROWS * I::NCH;
+  const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int id = threadIdx.x + u * 256, row = id / PER, ch = id % PER * VE;
-      const T *p = at(row);
-      const bool in = p != nullptr && ch < D;
-      vec t = {};
-      if (in) t = *reinterpret_cast<const vec *>(p + ch);
-      r[u] = t;
-    }
+  for (int u = 0; u < (PIECES + 255) / 256; ++u) {
+    const int first = u * 256 + (int)(threadIdx.x & ~63u);
+    if (PIECES % 256 && first >= PIECES) break;                  // wave-uniform
+    const int id = u * 256 + threadIdx.x, row = id / I::NCH, ch = (id % I::NCH) ^ I::swz(row);
+    const char *p = at(row);
+    dma16(p != nullptr && ch < chunks ? p + ch * 16 : zero, img + (size_t)__builtin_amdgcn_readfirstlane(first) * 16);
   }
-  __device__ __forceinline__ void store(T *lds) const {
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int id = threadIdx.x + u * 256, row = id / PER, ch = id % PER * VE;
-      *reinterpret_cast<vec *>(lds + row * Lay<T, DP>::LD + ch) = r[u];
-    }
+}
+
+// the 8 k-elements (channels ch .. ch + 7) of a lane for a contraction over channels; row: a multiple of 16 + the lane's column
+template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type row_frag(const char *img, int row, int ch) {
+  typedef Img<T, DP> I;
+  const int s = I::swz(row), c = ch / I::VE;
+  const char *p = img + row * I::RB;
+  if constexpr (sizeof(T) == 2) return *reinterpret_cast<const typename Vec8<T>::type *>(p + ((c ^ s) << 4));
+  else {
+    const f32x4 a = *reinterpret_cast<const f32x4 *>(p + ((c ^ s) << 4)), b = *reinterpret_cast<const f32x4 *>(p + (((c + 1) ^ s) << 4));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
-};
-// ... 4 x 4 pieces (4 tokens x 4 channels) that are turned into quads on their way to LDS
-template <typename T, int DP, int TK> struct QuadStage {
-  typedef typename Vec4<T>::type vec;
-  static constexpr int PER = DP / 4, N = TK / 4 * PER, NU = (N + 255) / 256;
-  vec r[NU][4];
-  template <typename F> __device__ __forceinline__ void load(F at, int D) {
+}
+// ... for a contraction over the 32 tokens from t0 (a multiple of 32): tokens t0 + 4 g .. + 3 and t0 + 16 + 4 g .. + 3 of channel
+// d0 + lane % 16, g = lane / 16
+template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type col_frag(const char *img, int t0, int d0, int lane) {
+  typedef Img<T, DP> I;
+  const int g = lane / 16, col = lane % 16;
+  if constexpr (sizeof(T) == 2) {
+    // transposing read: lane 4 q + p of a group of 16 points at row q, elements 4 p .. + 3 of a 4 x 16 block and gets column lane % 16 of it
+    const int row = 4 * g + col / 4, p = col % 4;
+    const char *a = img + (t0 + row) * I::RB + (((d0 / 8 + p / 2) ^ I::swz(row)) << 4) + (p % 2) * 8;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)a);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(a + 16 * I::RB));
+    const s16x8 both = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(typename Vec8<T>::type, both);
+  } else {
+    f32x8 r;
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int id = threadIdx.x + u * 256, quad = id / PER, ch = id % PER * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        vec t = {};
-        if (id < N) {
-          const T *p = at(quad * 4 + i);
-          if (p != nullptr && ch < D) t = *reinterpret_cast<const vec *>(p + ch);
-        }
-        r[u][i] = t;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int row = 4 * g + e;
+      const char *a = img + (t0 + row) * I::RB + (((d0 / 4 + col / 4) ^ I::swz(row)) << 4) + (col % 4) * 4;
+      r[e] = *reinterpret_cast<const float *>(a);
+      r[4 + e] = *reinterpret_cast<const float *>(a + 16 * I::RB);
     }
+    return r;
   }
-  __device__ __forceinline__ void store(T *lds) const {
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int id = threadIdx.x + u * 256, quad = id / PER, ch = id % PER * 4;
-      if (id >= N) continue;
-      T *p = lds + quad * Lay<T, DP>::QD + ch * 4;
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const vec t = {r[u][0][d], r[u][1][d], r[u][2][d], r[u][3][d]};
-        *reinterpret_cast<vec *>(p + d * 4) = t;
-      }
-    }
-  }
-};
+}
 
 // ------------------------------------------------------------------------------------------ the blocks of one group
 // blocks[0 .. top) of one group -> list[]: the valid indices, ascending, each once (a repeated index counts once, an index outside
@@ -183,26 +190,50 @@ __device__ __forceinline__ int group_blocks(const int32_t *blocks, int top, int 
 }
 
 // ------------------------------------------------------------------------------------------ forward
+// The keys of a group pass in segments of 64 (a block is one or two of them).
+struct Segment {
+  int key0;                                                      // first key, or -1: none
+  uint64_t mask;                                                 // bit r: key0 + r exists and is seen
+};
+// the raw parts of a segment: issued a tile before they are needed
+struct SegmentLoad { int key0; float seen; };
+struct KeySource {
+  const int *list;
+  const float *vis;
+  int n, lb, nk;                                                 // segments, log2 of the block, keys
+  __device__ __forceinline__ SegmentLoad load(int i) const {
+    SegmentLoad r{-1, 0.f};
+    if (i < n) {
+      const int per = lb - 6;
+      r.key0 = __builtin_amdgcn_readfirstlane((list[i >> per] << lb) + ((i & ((1 << per) - 1)) << 6));
+      const int key = r.key0 + (int)(threadIdx.x & 63);
+      if (key < nk) r.seen = vis ? vis[key] : 1.f;
+    }
+    return r;
+  }
+  __device__ __forceinline__ static Segment finish(const SegmentLoad &l) { return Segment{l.key0, __ballot(l.seen > 0.5f)}; }
+};
+
 // One workgroup: M = 16 NQ WM query rows of one group (a row = one query token and one head of the key head's group), 4 waves as WM
 // row sets x WN key sets.  The group's keys pass as one stream in tiles of TK = 32 WN; every wave keeps its own running maximum, sum
-// and output for its 32 keys of each tile, joined at the end, so the only meeting of the waves in the loop is the staging of the tile.
-template <typename T, int DP, int NQ, int WM, int WN>
-__global__ __launch_bounds__(256) void attend_fwd_kernel(AttnArgs a) {
-  constexpr int M = 16 * NQ * WM, TK = 32 * WN, KC = DP / 32, DT = DP / 16;
-  typedef Lay<T, DP> L;
+// and output for its 32 keys of each tile, joined at the end, so the only meeting of the waves in the loop is the hand-over of the tile.
+template <typename T, int DP, int NQ, int WM, int WN> struct FwdTile {
+  static constexpr int M = 16 * NQ * WM, TK = 32 * WN, NS = TK > 64 ? TK / 64 : 1;
+  static constexpr size_t img = (size_t)TK * Img<T, DP>::RB, tiles = 4 * img;          // K and V, twice
+  static constexpr size_t join = (size_t)M * (DP + 4) * 4 + (size_t)WN * M * 8;
+  static constexpr size_t body = tiles > join ? tiles : join;
+};
+template <typename T, int DP, int NQ, int WM, int WN, int OCC>
+__global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
+  typedef FwdTile<T, DP, NQ, WM, WN> F;
+  constexpr int M = F::M, TK = F::TK, NS = F::NS, KC = DP / 32, DT = DP / 16;
   typedef typename Vec8<T>::type frag;
-  extern __shared__ char smem[];
-  T *krows = reinterpret_cast<T *>(smem);
-  T *vquads = reinterpret_cast<T *>(smem + L::rows(TK));
-  constexpr size_t tiles = L::rows(TK) + L::quads(TK);
-  constexpr size_t join = (size_t)M * (DP + 4) * 4 + (size_t)WN * M * 8;
-  constexpr size_t body = tiles > join ? tiles : join;
-  float *lim = reinterpret_cast<float *>(smem + body);           // per key of the tile: +inf, or -inf where it is not seen
-  int *list = reinterpret_cast<int *>(lim + TK);
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  int *list = reinterpret_cast<int *>(smem + F::body);
   uint32_t *bits = reinterpret_cast<uint32_t *>(list + a.cap);
   __shared__ int n_list;
 
-  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, col = lane % 16, g = lane / 16;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % 16, g = lane / 16;
   const int wm = wave / WN, wn = wave % WN;
   unsigned item = xcd_remap(blockIdx.x, gridDim.x);
   const int split = (int)(item % a.splits);
@@ -215,7 +246,12 @@ __global__ __launch_bounds__(256) void attend_fwd_kernel(AttnArgs a) {
 
   const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + s) * a.top, a.top, a.nb, bits, list, &n_list);
   const int e0 = (int)((int64_t)n * split / a.splits), e1 = (int)((int64_t)n * (split + 1) / a.splits);
-  const int total = (e1 - e0) << a.lb, nt = (total + TK - 1) / TK;
+  const KeySource keys{list + e0, a.vis ? a.vis + (int64_t)b * a.Nk : nullptr, (e1 - e0) << (a.lb - 6), a.lb, a.Nk};
+  const int nt = (keys.n * 64 + TK - 1) / TK;
+  const char *kb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h);
+  const char *vb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h);
+  const int chunks = a.D / Img<T, DP>::VE;
+  const unsigned kst = (unsigned)(a.sk.n * sizeof(T)), vst = (unsigned)(a.sv.n * sizeof(T));   // host: 128 rows stay below 2^31
 
   // row r of the group: token q_block * s + r / G, head hk * G + r % G
   auto row_of = [&](int m, int &token, int &head) {
@@ -225,7 +261,34 @@ __global__ __launch_bounds__(256) void attend_fwd_kernel(AttnArgs a) {
     head = hk * a.G + (r - t * a.G);
     return r < a.rows && token < a.Nq;
   };
+  auto seg_load = [&](int t, SegmentLoad *r) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) r[i] = keys.load(t * TK / 64 + i);
+  };
+  auto issue = [&](int t, const Segment *sg) {
+    char *kd = smem + (t & 1) * 2 * F::img, *vd = kd + F::img;
+    const int off = TK < 64 ? (t * TK) & 63 : 0;                 // within the segment
+    auto at = [&](const char *base, int64_t n, unsigned st, int r) -> const char * {
+      const Segment &x = sg[NS > 1 ? r / 64 : 0];
+      const int rr = (r & 63) + off;
+      return (x.mask >> rr) & 1 ? base + (int64_t)x.key0 * n * (int64_t)sizeof(T) + (unsigned)rr * st : nullptr;
+    };
+    dma_rows<T, DP, TK>(kd, chunks, [&](int r) { return at(kb, a.sk.n, kst, r); });
+    dma_rows<T, DP, TK>(vd, chunks, [&](int r) { return at(vb, a.sv.n, vst, r); });
+  };
+
+  Segment cur[NS], nxt[NS];
+  SegmentLoad raw[NS];
+  seg_load(0, raw);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) cur[i] = KeySource::finish(raw[i]);
+  if (nt > 0) issue(0, cur);
+  seg_load(1, raw);
+
+  // the queries, as columns; a negative scale turns their sign, so that the largest product is the largest score
   frag qf[NQ][KC];
+  const bool neg = a.c < 0.f;
+  const float sc2 = fmaxf(fabsf(a.c), 1e-30f);                   // not 0: -inf times it has to stay -inf
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     int token, head;
@@ -236,33 +299,11 @@ __global__ __launch_bounds__(256) void attend_fwd_kernel(AttnArgs a) {
       const int ch = c * 32 + g * 8;
       frag t = {};
       if (ok && ch < a.D) t = *reinterpret_cast<const frag *>(p + ch);
-      qf[i][c] = t;
+      qf[i][c] = neg ? -t : t;
     }
   }
-
-  const T *kb = reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h;
-  const T *vb = reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h;
-  const float *vis = a.vis ? a.vis + (int64_t)b * a.Nk : nullptr;
-  // key of row r of the tile at t0, or -1
-  auto key_of = [&](int t0, int r) {
-    const int at = t0 + r;
-    if (at >= total) return -1;
-    const int key = (list[e0 + (at >> a.lb)] << a.lb) + (at & ((1 << a.lb) - 1));
-    if (key >= a.Nk) return -1;
-    if (vis && !(vis[key] > 0.5f)) return -1;
-    return key;
-  };
-  RowStage<T, DP, TK> ks;
-  QuadStage<T, DP, TK> vs;
-  float lim_r = kNegInf;
-  auto load = [&](int t0) {
-    ks.load([&](int r) { const int key = key_of(t0, r); return key < 0 ? nullptr : kb + (int64_t)key * a.sk.n; }, a.D);
-    vs.load([&](int r) { const int key = key_of(t0, r); return key < 0 ? nullptr : vb + (int64_t)key * a.sv.n; }, a.D);
-    if (tid < TK) lim_r = key_of(t0, tid) < 0 ? kNegInf : kPosInf;
-  };
-
   f32x4 o[NQ][DT];
-  float m[NQ], l[NQ];
+  float m[NQ], l[NQ];                                            // maximum in log2 units, sum of exp2(score - maximum)
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     m[i] = kNegInf;
@@ -270,14 +311,13 @@ __global__ __launch_bounds__(256) void attend_fwd_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (nt > 0) load(0);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) nxt[i] = KeySource::finish(raw[i]);
   for (int t = 0; t < nt; ++t) {
-    __syncthreads();                                             // the last tile has been read
-    ks.store(krows);
-    vs.store(vquads);
-    if (tid < TK) lim[tid] = lim_r;
-    __syncthreads();
-    if (t + 1 < nt) load((t + 1) * TK);
+    tile_barrier();                                              // tile t is there, tile t - 1 has been read
+    if (t + 1 < nt) issue(t + 1, nxt);
+    seg_load(t + 2, raw);
+    const char *krows = smem + (t & 1) * 2 * F::img, *vrows = krows + F::img;
     f32x4 sc[2][NQ];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -290,44 +330,56 @@ __global__ __launch_bounds__(256) void attend_fwd_kernel(AttnArgs a) {
         for (int i = 0; i < NQ; ++i) sc[u][i] = mma(kf, qf[i][c], sc[u][i]);
       }
     }
-    frag pf[NQ];
-    f32x4 lm[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) lm[u] = *reinterpret_cast<const f32x4 *>(lim + wn * 32 + u * 16 + g * 4);
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      float mx = kNegInf;
+    const uint64_t mask = cur[wn * 32 / 64 % NS].mask;
+    if (mask != ~0ull) {
+      const unsigned seen = (unsigned)(mask >> ((TK < 64 ? (t * TK) & 63 : wn * 32 & 63) + g * 4));
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[u][i][e] = fminf(sc[u][i][e] * a.c, lm[u][e]);      // log2 units; an unseen key's score becomes -inf
-          mx = fmaxf(mx, sc[u][i][e]);
-        }
+        for (int i = 0; i < NQ; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[u][i][e] = (seen >> (u * 16 + e)) & 1 ? sc[u][i][e] : kNegInf;
+    }
+    frag pf[NQ];
+    bool grew = false;
+    float f[NQ];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      float mx = fmaxf(fmaxf(fmaxf(sc[0][i][0], sc[0][i][1]), fmaxf(sc[0][i][2], sc[0][i][3])), fmaxf(fmaxf(sc[1][i][0], sc[1][i][1]), fmaxf(sc[1][i][2], sc[1][i][3])));
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m[i], mx);
+      const float mn = fmaxf(m[i], mx * sc2);
       const float ms = mn == kNegInf ? 0.f : mn;                 // nothing seen yet: exp2(-inf - 0) = 0
-      const float f = __builtin_amdgcn_exp2f(m[i] - ms);
+      f[i] = __builtin_amdgcn_exp2f(m[i] - ms);                  // exactly 1 while the maximum stays
+      grew |= mn > m[i];
       m[i] = mn;
       float sum = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(sc[u][i][e] - ms);
+          const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i][e], sc2, -ms));
           sum += p;
           pf[i][u * 4 + e] = (T)p;
         }
-      l[i] = l[i] * f + sum;
+      l[i] = fmaf(l[i], f[i], sum);
+    }
+    if (__any(grew)) {                                           // no maximum moved in most tiles behind the first ones
 #pragma unroll
-      for (int d = 0; d < DT; ++d) o[i][d] *= f;
+      for (int i = 0; i < NQ; ++i)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[i][d] *= f[i];
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const frag vf = quad_frag<T, DP>(vquads, wn * 32, g, d * 16 + col);
+      const frag vf = col_frag<T, DP>(vrows, wn * 32, d * 16, lane);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) o[i][d] = mma(vf, pf[i], o[i][d]);
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      cur[i] = nxt[i];
+      nxt[i] = KeySource::finish(raw[i]);
     }
   }
 
@@ -475,24 +527,24 @@ __global__ __launch_bounds__(256) void attend_invert_kernel(AttnArgs a) {
   if (j >= 0 && j < a.nb) atomicOr(&a.inv[(bh * a.nb + j) * a.words + (s >> 5)], 1u << (s & 31));
 }
 
-template <typename T, int DP, int NQ, int WM, int WN>
-__global__ __launch_bounds__(256) void attend_dq_kernel(AttnArgs a) {
-  constexpr int M = 16 * NQ * WM, TK = 32 * WN, KC = DP / 32, DT = DP / 16;
-  typedef Lay<T, DP> L;
+template <typename T, int DP, int NQ, int WM, int WN> struct DqTile {
+  static constexpr int M = 16 * NQ * WM, TK = 32 * WN;
+  static constexpr size_t img = (size_t)TK * Img<T, DP>::RB, tiles = 4 * img;
+  static constexpr size_t join = (size_t)M * (DP + 4) * 4;
+  static constexpr size_t body = tiles > join ? tiles : join;
+};
+template <typename T, int DP, int NQ, int WM, int WN, int OCC>
+__global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
+  typedef DqTile<T, DP, NQ, WM, WN> F;
+  constexpr int M = F::M, TK = F::TK, KC = DP / 32, DT = DP / 16;
+  static_assert(TK <= 64, "one segment per tile");
   typedef typename Vec8<T>::type frag;
-  extern __shared__ char smem[];
-  T *krows = reinterpret_cast<T *>(smem);
-  T *vrows = reinterpret_cast<T *>(smem + L::rows(TK));
-  T *kquads = reinterpret_cast<T *>(smem + 2 * L::rows(TK));
-  constexpr size_t tiles = 2 * L::rows(TK) + L::quads(TK);
-  constexpr size_t join = (size_t)M * (DP + 4) * 4;
-  constexpr size_t body = tiles > join ? tiles : join;
-  float *lim = reinterpret_cast<float *>(smem + body);
-  int *list = reinterpret_cast<int *>(lim + TK);
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  int *list = reinterpret_cast<int *>(smem + F::body);
   uint32_t *bits = reinterpret_cast<uint32_t *>(list + a.cap);
   __shared__ int n_list;
 
-  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, col = lane % 16, g = lane / 16;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % 16, g = lane / 16;
   const int wm = wave / WN, wn = wave % WN;
   unsigned item = xcd_remap(blockIdx.x, gridDim.x);
   const int chunk = (int)(item % a.chunks);
@@ -500,7 +552,12 @@ __global__ __launch_bounds__(256) void attend_dq_kernel(AttnArgs a) {
   const int s = (int)(item % a.S);
   const int bh = (int)(item / a.S), hk = bh % a.Hkv, b = bh / a.Hkv;
   const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + s) * a.top, a.top, a.nb, bits, list, &n_list);
-  const int total = n << a.lb, nt = (total + TK - 1) / TK;
+  const KeySource keys{list, a.vis ? a.vis + (int64_t)b * a.Nk : nullptr, n << (a.lb - 6), a.lb, a.Nk};
+  const int nt = keys.n * 64 / TK;
+  const char *kb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h);
+  const char *vb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h);
+  const int chunks = a.D / Img<T, DP>::VE;
+  const unsigned kst = (unsigned)(a.sk.n * sizeof(T)), vst = (unsigned)(a.sv.n * sizeof(T));
   auto row_of = [&](int m, int &token, int &head) {
     const int r = chunk * M + m;
     const int t = (int)a.by_g.div((unsigned)r);
@@ -508,6 +565,19 @@ __global__ __launch_bounds__(256) void attend_dq_kernel(AttnArgs a) {
     head = hk * a.G + (r - t * a.G);
     return r < a.rows && token < a.Nq;
   };
+  auto issue = [&](int t, const Segment &x) {
+    char *kd = smem + (t & 1) * 2 * F::img, *vd = kd + F::img;
+    const int off = (t * TK) & 63;
+    auto at = [&](const char *base, int64_t n, unsigned st, int r) -> const char * {
+      return (x.mask >> (r + off)) & 1 ? base + (int64_t)x.key0 * n * (int64_t)sizeof(T) + (unsigned)(r + off) * st : nullptr;
+    };
+    dma_rows<T, DP, TK>(kd, chunks, [&](int r) { return at(kb, a.sk.n, kst, r); });
+    dma_rows<T, DP, TK>(vd, chunks, [&](int r) { return at(vb, a.sv.n, vst, r); });
+  };
+  Segment cur = KeySource::finish(keys.load(0)), nxt;
+  if (nt > 0) issue(0, cur);
+  SegmentLoad raw = keys.load(TK / 64);
+
   frag qf[NQ][KC], df[NQ][KC];
   float lse2[NQ], delta[NQ];
 #pragma unroll
@@ -536,40 +606,17 @@ __global__ __launch_bounds__(256) void attend_dq_kernel(AttnArgs a) {
       df[i][c] = u;
     }
   }
-  const T *kb = reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h;
-  const T *vb = reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h;
-  const float *vis = a.vis ? a.vis + (int64_t)b * a.Nk : nullptr;
-  auto key_of = [&](int t0, int r) {
-    const int at = t0 + r;
-    if (at >= total) return -1;
-    const int key = (list[at >> a.lb] << a.lb) + (at & ((1 << a.lb) - 1));
-    if (key >= a.Nk) return -1;
-    if (vis && !(vis[key] > 0.5f)) return -1;
-    return key;
-  };
-  RowStage<T, DP, TK> ks, vs;
-  QuadStage<T, DP, TK> kq;
-  float lim_r = kNegInf;
-  auto load = [&](int t0) {
-    ks.load([&](int r) { const int key = key_of(t0, r); return key < 0 ? nullptr : kb + (int64_t)key * a.sk.n; }, a.D);
-    vs.load([&](int r) { const int key = key_of(t0, r); return key < 0 ? nullptr : vb + (int64_t)key * a.sv.n; }, a.D);
-    kq.load([&](int r) { const int key = key_of(t0, r); return key < 0 ? nullptr : kb + (int64_t)key * a.sk.n; }, a.D);
-    if (tid < TK) lim_r = key_of(t0, tid) < 0 ? kNegInf : kPosInf;
-  };
   f32x4 o[NQ][DT];
 #pragma unroll
   for (int i = 0; i < NQ; ++i)
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (nt > 0) load(0);
+  nxt = KeySource::finish(raw);
   for (int t = 0; t < nt; ++t) {
-    __syncthreads();
-    ks.store(krows);
-    vs.store(vrows);
-    kq.store(kquads);
-    if (tid < TK) lim[tid] = lim_r;
-    __syncthreads();
-    if (t + 1 < nt) load((t + 1) * TK);
+    tile_barrier();
+    if (t + 1 < nt) issue(t + 1, nxt);
+    raw = keys.load((t + 2) * TK / 64);
+    const char *krows = smem + (t & 1) * 2 * F::img, *vrows = krows + F::img;
     f32x4 sc[2][NQ], dp[2][NQ];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -587,23 +634,25 @@ __global__ __launch_bounds__(256) void attend_dq_kernel(AttnArgs a) {
       }
     }
     frag gf[NQ];
+    const unsigned seen = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32 + g * 4));
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const f32x4 lm = *reinterpret_cast<const f32x4 *>(lim + wn * 32 + u * 16 + g * 4);
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < NQ; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fminf(sc[u][i][e] * a.c, lm[e]) - lse2[i]);
+          float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i][e], a.c, -lse2[i]));
+          p = (seen >> (u * 16 + e)) & 1 ? p : 0.f;              // an unseen key's products are those of zeros
           gf[i][u * 4 + e] = (T)(p * (dp[u][i][e] - delta[i]) * a.scale);
         }
-    }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const frag kf = quad_frag<T, DP>(kquads, wn * 32, g, d * 16 + col);
+      const frag kf = col_frag<T, DP>(krows, wn * 32, d * 16, lane);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) o[i][d] = mma(kf, gf[i], o[i][d]);
     }
+    cur = nxt;
+    nxt = KeySource::finish(raw);
   }
   float *jo = reinterpret_cast<float *>(smem);
   __syncthreads();
@@ -640,24 +689,26 @@ __global__ __launch_bounds__(256) void attend_dq_kernel(AttnArgs a) {
 // S = Q K^T leaves a lane the probabilities of ITS key, the operand of dV^T = dout^T P and, as dS, of dK^T = Q^T dS.
 constexpr int kWindow = 32;   // words of group bits taken at a time: up to 1024 groups in the list
 
-template <typename T, int DP, int NK, int WM, int WN>
-__global__ __launch_bounds__(256) void attend_dkv_kernel(AttnArgs a) {
-  constexpr int M = 16 * NK * WM, TR = 32 * WN, KC = DP / 32, DT = DP / 16;
-  typedef Lay<T, DP> L;
+template <typename T, int DP, int NK, int WM, int WN> struct DkvTile {
+  static constexpr int M = 16 * NK * WM, TR = 32 * WN;
+  static constexpr size_t img = (size_t)TR * Img<T, DP>::RB, tiles = 4 * img;          // Q and dout, twice
+  static constexpr size_t join = (size_t)M * (DP + 4) * 4;
+  static constexpr size_t body = tiles > join ? tiles : join;
+  // behind the tiles: byte offsets of a tile's rows in q and dout, lse and delta (twice each), the list of groups
+  static constexpr size_t bytes = body + 2 * TR * 16 + 2 * TR * 8 + 32 * kWindow * 4;
+};
+template <typename T, int DP, int NK, int WM, int WN, int OCC>
+__global__ __launch_bounds__(256, OCC) void attend_dkv_kernel(AttnArgs a) {
+  typedef DkvTile<T, DP, NK, WM, WN> F;
+  constexpr int M = F::M, TR = F::TR, KC = DP / 32, DT = DP / 16;
   typedef typename Vec8<T>::type frag;
-  extern __shared__ char smem[];
-  T *qrows = reinterpret_cast<T *>(smem);
-  T *drows = reinterpret_cast<T *>(smem + L::rows(TR));
-  T *qquads = reinterpret_cast<T *>(smem + 2 * L::rows(TR));
-  T *dquads = reinterpret_cast<T *>(smem + 2 * L::rows(TR) + L::quads(TR));
-  constexpr size_t tiles = 2 * (L::rows(TR) + L::quads(TR));
-  constexpr size_t join = (size_t)M * (DP + 4) * 4;
-  constexpr size_t body = tiles > join ? tiles : join;
-  float *lse2 = reinterpret_cast<float *>(smem + body), *delta = lse2 + TR;
-  int *list = reinterpret_cast<int *>(delta + TR);               // [32 kWindow]
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  longlong2 *tab = reinterpret_cast<longlong2 *>(smem + F::body);                      // [2][TR], x < 0: no row
+  float *lse2 = reinterpret_cast<float *>(tab + 2 * TR), *delta = lse2 + 2 * TR;       // [2][TR] each
+  int *list = reinterpret_cast<int *>(delta + 2 * TR);                                 // [32 kWindow]
   __shared__ int n_list;
 
-  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, col = lane % 16, g = lane / 16;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % 16, g = lane / 16;
   const int wm = wave / WN, wn = wave % WN;
   const int tiles_of = (a.Nk + M - 1) / M;
   unsigned item = xcd_remap(blockIdx.x, gridDim.x);
@@ -666,12 +717,12 @@ __global__ __launch_bounds__(256) void attend_dkv_kernel(AttnArgs a) {
   const uint32_t *inv = a.inv + ((int64_t)bh * a.nb + (((int64_t)kt * M) >> a.lb)) * a.words;
 
   frag kf[NK][KC], vf[NK][KC];
-  float lim[NK];
+  bool seen[NK];
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
     const int key = kt * M + (wm * NK + i) * 16 + col;
     const bool ok = key < a.Nk && (!a.vis || a.vis[(int64_t)b * a.Nk + key] > 0.5f);
-    lim[i] = ok ? kPosInf : kNegInf;
+    seen[i] = ok;
     const T *p = reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)key * a.sk.n + (int64_t)hk * a.sk.h;
     const T *q = reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)key * a.sv.n + (int64_t)hk * a.sv.h;
 #pragma unroll
@@ -686,8 +737,9 @@ __global__ __launch_bounds__(256) void attend_dkv_kernel(AttnArgs a) {
       vf[i][c] = u;
     }
   }
-  const T *qb = reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sq.b;
-  const T *db = reinterpret_cast<const T *>(a.dout) + (int64_t)b * a.sdo.b;
+  const char *qb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sq.b);
+  const char *db = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.dout) + (int64_t)b * a.sdo.b);
+  const int chunks = a.D / Img<T, DP>::VE;
   f32x4 gk[NK][DT], gv[NK][DT];
 #pragma unroll
   for (int i = 0; i < NK; ++i)
@@ -695,10 +747,9 @@ __global__ __launch_bounds__(256) void attend_dkv_kernel(AttnArgs a) {
     for (int d = 0; d < DT; ++d) gk[i][d] = gv[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   for (int w0 = 0; w0 < a.words; w0 += kWindow) {
-    __syncthreads();                                             // the last window's list has been read
+    __syncthreads();                                             // the last window's list and tiles have been read
     if (tid < 64) {
-      const uint32_t bitsw = tid < kWindow && w0 + tid < a.words ? inv[w0 + tid] : 0;
-      uint32_t m = bitsw;
+      uint32_t m = tid < kWindow && w0 + tid < a.words ? inv[w0 + tid] : 0;
       int incl = __popc(m);
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -714,55 +765,64 @@ __global__ __launch_bounds__(256) void attend_dkv_kernel(AttnArgs a) {
     }
     __syncthreads();
     const int64_t total = (int64_t)n_list * a.rows;
-    const int64_t nt = (total + TR - 1) / TR;
-    // row r of the tile at t0: (token, head), or none
-    auto row_of = [&](int64_t t0, int r, int &token, int &head) {
-      const int64_t at = t0 + r;
-      if (at >= total) return false;
+    const int nt = (int)((total + TR - 1) / TR);                 // total < 2^30
+    if (nt == 0) continue;
+    // threads 0 .. TR - 1: where row tid of tile t lies, and where its statistics lie (< 0: no row)
+    auto locate = [&](int t, longlong2 &where) -> int64_t {
+      const int64_t at = (int64_t)t * TR + tid;
+      where = longlong2{-1, -1};
+      if (at >= total) return -1;
       const unsigned e = a.by_rows.div((unsigned)at), rr = (unsigned)at - e * (unsigned)a.rows;
-      const unsigned t = a.by_g.div(rr);
-      token = list[e] * a.q_block + (int)t;
-      head = hk * a.G + (int)(rr - t * (unsigned)a.G);
-      return token < a.Nq;
+      const unsigned tk = a.by_g.div(rr);
+      const int token = list[e] * a.q_block + (int)tk;
+      const int head = hk * a.G + (int)(rr - tk * (unsigned)a.G);
+      if (token >= a.Nq) return -1;
+      where.x = ((int64_t)token * a.sq.n + (int64_t)head * a.sq.h) * (int64_t)sizeof(T);
+      where.y = ((int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h) * (int64_t)sizeof(T);
+      return ((int64_t)b * a.Hq + head) * a.Nq + token;
     };
-    auto q_at = [&](int64_t t0, int r) -> const T * {
-      int token, head;
-      return row_of(t0, r, token, head) ? qb + (int64_t)token * a.sq.n + (int64_t)head * a.sq.h : nullptr;
-    };
-    auto d_at = [&](int64_t t0, int r) -> const T * {
-      int token, head;
-      return row_of(t0, r, token, head) ? db + (int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h : nullptr;
-    };
-    RowStage<T, DP, TR> qs, ds;
-    QuadStage<T, DP, TR> qq, dq;
-    float lse_r = kPosInf, delta_r = 0.f;
-    auto load = [&](int64_t t0) {
-      qs.load([&](int r) { return q_at(t0, r); }, a.D);
-      ds.load([&](int r) { return d_at(t0, r); }, a.D);
-      qq.load([&](int r) { return q_at(t0, r); }, a.D);
-      dq.load([&](int r) { return d_at(t0, r); }, a.D);
-      if (tid < TR) {
-        int token, head;
-        lse_r = kPosInf;
-        delta_r = 0.f;
-        if (row_of(t0, tid, token, head)) {
-          const int64_t at = ((int64_t)b * a.Hq + head) * a.Nq + token;
-          const float x = a.lse[at];
-          lse_r = x == kNegInf ? kPosInf : x * kLog2e - PScale<T>::bits;
-          delta_r = a.delta[at];
-        }
+    auto stat = [&](int64_t at, float &ls, float &de) {
+      ls = kPosInf;                                              // exp2(x - inf) = 0
+      de = 0.f;
+      if (at >= 0) {
+        const float x = a.lse[at];
+        ls = x == kNegInf ? kPosInf : x * kLog2e - PScale<T>::bits;
+        de = a.delta[at];
       }
     };
-    if (nt > 0) load(0);
-    for (int64_t t = 0; t < nt; ++t) {
-      __syncthreads();
-      qs.store(qrows);
-      ds.store(drows);
-      qq.store(qquads);
-      dq.store(dquads);
-      if (tid < TR) { lse2[tid] = lse_r; delta[tid] = delta_r; }
-      __syncthreads();
-      if (t + 1 < nt) load((t + 1) * TR);
+    auto issue = [&](int t) {
+      char *qd = smem + (t & 1) * 2 * F::img, *dd = qd + F::img;
+      const longlong2 *tb = tab + (t & 1) * TR;
+      dma_rows<T, DP, TR>(qd, chunks, [&](int r) -> const char * { const int64_t x = tb[r].x; return x < 0 ? nullptr : qb + x; });
+      dma_rows<T, DP, TR>(dd, chunks, [&](int r) -> const char * { const longlong2 x = tb[r]; return x.x < 0 ? nullptr : db + x.y; });
+    };
+    // rows of tiles 0 and 1, statistics of tile 0; from here on rows are located two tiles ahead, statistics fetched one ahead
+    int64_t st_next = -1;
+    if (tid < TR) {
+      longlong2 w;
+      float ls, de;
+      const int64_t at = locate(0, w);
+      tab[tid] = w;
+      stat(at, ls, de);
+      lse2[tid] = ls;
+      delta[tid] = de;
+      st_next = locate(1, w);
+      tab[TR + tid] = w;
+    }
+    __syncthreads();
+    issue(0);
+    for (int t = 0; t < nt; ++t) {
+      tile_barrier();
+      if (t + 1 < nt) issue(t + 1);
+      float ls_n, de_n;
+      int64_t st_next2 = -1;
+      if (tid < TR) {
+        stat(st_next, ls_n, de_n);
+        longlong2 w;
+        st_next2 = locate(t + 2, w);
+        tab[(t & 1) * TR + tid] = w;                             // tile t's rows are on their way already
+      }
+      const char *qrows = smem + (t & 1) * 2 * F::img, *drows = qrows + F::img;
       f32x4 sc[2][NK], dp[2][NK];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -782,27 +842,32 @@ __global__ __launch_bounds__(256) void attend_dkv_kernel(AttnArgs a) {
       frag pf[NK], gf[NK];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const f32x4 ls = *reinterpret_cast<const f32x4 *>(lse2 + wn * 32 + u * 16 + g * 4);
-        const f32x4 de = *reinterpret_cast<const f32x4 *>(delta + wn * 32 + u * 16 + g * 4);
+        const f32x4 ls = *reinterpret_cast<const f32x4 *>(lse2 + (t & 1) * TR + wn * 32 + u * 16 + g * 4);
+        const f32x4 de = *reinterpret_cast<const f32x4 *>(delta + (t & 1) * TR + wn * 32 + u * 16 + g * 4);
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fminf(sc[u][i][e] * a.c, lim[i]) - ls[e]);
+            const float p = seen[i] ? __builtin_amdgcn_exp2f(fmaf(sc[u][i][e], a.c, -ls[e])) : 0.f;
             pf[i][u * 4 + e] = (T)p;
             gf[i][u * 4 + e] = (T)(p * (dp[u][i][e] - de[e]) * (a.scale * PScale<T>::inv));
           }
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const frag df = quad_frag<T, DP>(dquads, wn * 32, g, d * 16 + col);
-        const frag qf = quad_frag<T, DP>(qquads, wn * 32, g, d * 16 + col);
+        const frag df = col_frag<T, DP>(drows, wn * 32, d * 16, lane);
+        const frag qf = col_frag<T, DP>(qrows, wn * 32, d * 16, lane);
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
           gv[i][d] = mma(df, pf[i], gv[i][d]);
           gk[i][d] = mma(qf, gf[i], gk[i][d]);
         }
       }
+      if (tid < TR) {
+        lse2[((t + 1) & 1) * TR + tid] = ls_n;
+        delta[((t + 1) & 1) * TR + tid] = de_n;
+      }
+      st_next = st_next2;
     }
   }
   float *jo = reinterpret_cast<float *>(smem);
@@ -841,54 +906,46 @@ __global__ __launch_bounds__(256) void attend_dkv_kernel(AttnArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------ host
-template <typename T, int DP, int NQ, int WM, int WN> static size_t fwd_lds(const AttnArgs &a) {
-  constexpr int M = 16 * NQ * WM, TK = 32 * WN;
-  const size_t tiles = Lay<T, DP>::rows(TK) + Lay<T, DP>::quads(TK), join = (size_t)M * (DP + 4) * 4 + (size_t)WN * M * 8;
-  return (tiles > join ? tiles : join) + TK * 4 + (size_t)a.cap * 4 + (size_t)(a.nb + 31) / 32 * 4;
-}
+// Tile shapes.  16-bit: 64 rows x 64 keys as 2 x 2 waves of 32 x 32 (every LDS fragment feeds two products); groups of up to 16 rows (one
+// token of a few heads) take 16 rows x 128 keys, the four waves sharing out the keys.  fp32, whose products take 16 times as long
+// per fragment: 64 rows x 32 keys as 4 x 1 waves of 16 x 32, few rows (up to 32) x 64 keys.
+constexpr int few_rows(bool f32) { return f32 ? 32 : 16; }
+static int fwd_rows(const AttnArgs &a, bool f32) { return a.rows <= few_rows(f32) ? few_rows(f32) : 64; }
+static int fwd_keys(const AttnArgs &a, bool f32) { return a.rows <= few_rows(f32) ? (f32 ? 64 : 128) : (f32 ? 32 : 64); }
 
-constexpr int kFewRows = 16;       // up to 16 rows in a group: the kernel whose four waves share the keys of 16 rows
-static int fwd_rows(const AttnArgs &a) { return a.rows <= kFewRows ? 16 : 64; }
+static size_t list_bytes(const AttnArgs &a) { return (size_t)a.cap * 4 + (size_t)(a.nb + 31) / 32 * 4; }
 
-template <typename T, int DP, int NQ, int WM, int WN> static int launch_fwd_tile(const AttnArgs &a, int64_t blocks, hipStream_t s) {
-  const auto kernel = attend_fwd_kernel<T, DP, NQ, WM, WN>;
-  const size_t lds = fwd_lds<T, DP, NQ, WM, WN>(a);
-  TCL_REQUIRE(lds_ready((const void *)kernel, lds), TCL_ERR_LAUNCH, "block_attention: the device refuses %zu bytes of LDS", lds);
+template <typename K> static int launch(K kernel, size_t lds, int64_t blocks, const AttnArgs &a, hipStream_t s, const char *what) {
+  TCL_REQUIRE(blocks < (1LL << 31), TCL_ERR_SHAPE, "%s: grid of %ld blocks", what, (long)blocks);
+  TCL_REQUIRE(lds_ready((const void *)kernel, lds), TCL_ERR_LAUNCH, "%s: the device refuses %zu bytes of LDS", what, lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, s, a);
-  return check_launch("block_attention");
+  return check_launch(what);
 }
 template <typename T, int DP> static int launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t s) {
-  return fwd_rows(a) == 16 ? launch_fwd_tile<T, DP, 1, 1, 4>(a, blocks, s) : launch_fwd_tile<T, DP, 2, 2, 2>(a, blocks, s);
+  const char *what = "block_attention";
+  const bool few = a.rows <= few_rows(sizeof(T) == 4);
+  if constexpr (sizeof(T) == 4) {
+    if (few) return launch(attend_fwd_kernel<T, DP, 1, 2, 2, 1>, FwdTile<T, DP, 1, 2, 2>::body + list_bytes(a), blocks, a, s, what);
+    return launch(attend_fwd_kernel<T, DP, 1, 4, 1, 2>, FwdTile<T, DP, 1, 4, 1>::body + list_bytes(a), blocks, a, s, what);
+  } else {
+    if (few) return launch(attend_fwd_kernel<T, DP, 1, 1, 4, 1>, FwdTile<T, DP, 1, 1, 4>::body + list_bytes(a), blocks, a, s, what);
+    return launch(attend_fwd_kernel<T, DP, 2, 2, 2, 2>, FwdTile<T, DP, 2, 2, 2>::body + list_bytes(a), blocks, a, s, what);
+  }
 }
-
-template <typename T, int DP, int NQ, int WM, int WN> static int launch_dq_tile(const AttnArgs &a, int64_t blocks, hipStream_t s) {
-  constexpr int M = 16 * NQ * WM, TK = 32 * WN;
-  const size_t tiles = 2 * Lay<T, DP>::rows(TK) + Lay<T, DP>::quads(TK), join = (size_t)M * (DP + 4) * 4;
-  const size_t lds = (tiles > join ? tiles : join) + TK * 4 + (size_t)a.cap * 4 + (size_t)(a.nb + 31) / 32 * 4;
-  const auto kernel = attend_dq_kernel<T, DP, NQ, WM, WN>;
-  TCL_REQUIRE(lds_ready((const void *)kernel, lds), TCL_ERR_LAUNCH, "block_attention: the device refuses %zu bytes of LDS", lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, s, a);
-  return check_launch("block_attention backward (queries)");
-}
-constexpr int kDqFewRows = 32;     // the same for the query gradient (three tile images: 64 keys at a time, 32 rows)
 template <typename T, int DP> static int launch_dq(AttnArgs a, hipStream_t s) {
-  const bool few = a.rows <= kDqFewRows;
+  const char *what = "block_attention backward (queries)";
+  const bool few = a.rows <= 32;
   a.chunks = (int)cdiv(a.rows, few ? 32 : 64);
   const int64_t blocks = (int64_t)a.B * a.Hkv * a.S * a.chunks;
-  TCL_REQUIRE(blocks < (1LL << 31), TCL_ERR_SHAPE, "block_attention backward: grid of %ld blocks", (long)blocks);
-  return few ? launch_dq_tile<T, DP, 1, 2, 2>(a, blocks, s) : launch_dq_tile<T, DP, 2, 2, 2>(a, blocks, s);
+  if (few) return launch(attend_dq_kernel<T, DP, 1, 2, 2, 1>, DqTile<T, DP, 1, 2, 2>::body + list_bytes(a), blocks, a, s, what);
+  if constexpr (sizeof(T) == 4) return launch(attend_dq_kernel<T, DP, 1, 4, 1, 1>, DqTile<T, DP, 1, 4, 1>::body + list_bytes(a), blocks, a, s, what);
+  else return launch(attend_dq_kernel<T, DP, 2, 2, 2, 2>, DqTile<T, DP, 2, 2, 2>::body + list_bytes(a), blocks, a, s, what);
 }
 template <typename T, int DP> static int launch_dkv(const AttnArgs &a, hipStream_t s) {
-  typedef Lay<T, DP> L;
-  constexpr int M = 64, TR = 64;
-  const size_t tiles = 2 * (L::rows(TR) + L::quads(TR)), join = (size_t)M * (DP + 4) * 4;
-  const size_t lds = (tiles > join ? tiles : join) + 2 * TR * 4 + 32 * kWindow * 4;
-  const int64_t blocks = cdiv(a.Nk, M) * a.B * a.Hkv;
-  TCL_REQUIRE(blocks < (1LL << 31), TCL_ERR_SHAPE, "block_attention backward: grid of %ld blocks", (long)blocks);
-  const auto kernel = attend_dkv_kernel<T, DP, 2, 2, 2>;
-  TCL_REQUIRE(lds_ready((const void *)kernel, lds), TCL_ERR_LAUNCH, "block_attention: the device refuses %zu bytes of LDS", lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, s, a);
-  return check_launch("block_attention backward (keys)");
+  const char *what = "block_attention backward (keys)";
+  const int64_t blocks = cdiv(a.Nk, 64) * a.B * a.Hkv;
+  if constexpr (sizeof(T) == 4) return launch(attend_dkv_kernel<T, DP, 1, 4, 1, 1>, DkvTile<T, DP, 1, 4, 1>::bytes, blocks, a, s, what);
+  else return launch(attend_dkv_kernel<T, DP, 2, 2, 2, 1>, DkvTile<T, DP, 2, 2, 2>::bytes, blocks, a, s, what);
 }
 
 // head sizes are padded to a multiple of 32 in LDS and registers
@@ -943,20 +1000,24 @@ static int attn_setup(AttnArgs &a, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq
 }
 
 // Splits of the keys of a forward work item: enough workgroups for two per CU, two tiles each at least.
-static int fwd_splits(const AttnArgs &a, int64_t works) {
-  const int tk = fwd_rows(a) == 16 ? 128 : 64;
-  const int64_t tiles = cdiv((int64_t)a.cap << a.lb, tk);
-  int64_t n = cdiv(2 * kNumCU, works > 0 ? works : 1);
+struct FwdPlan { int chunks, splits; int64_t works; size_t part; };
+static FwdPlan fwd_plan(const AttnArgs &a, bool f32) {
+  FwdPlan p;
+  p.chunks = (int)cdiv(a.rows, fwd_rows(a, f32));
+  p.works = (int64_t)a.B * a.Hkv * a.S * p.chunks;
+  const int64_t tiles = cdiv((int64_t)a.cap << a.lb, fwd_keys(a, f32));
+  int64_t n = cdiv(2 * kNumCU, p.works > 0 ? p.works : 1);
   if (n > tiles / 2) n = tiles / 2;
-  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-}
-static size_t fwd_part_bytes(const AttnArgs &a, int64_t works, int splits) {
-  return splits > 1 ? round_up((size_t)works * splits * fwd_rows(a) * (a.D + 2) * 4, 256) : 256;
+  p.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  p.part = p.splits > 1 ? round_up((size_t)p.works * p.splits * fwd_rows(a, f32) * (a.D + 2) * 4, 256) : 256;
+  return p;
 }
 static bool rows16(const void *p, const Str &s, int dtype) {
   const int64_t ve = dtype == TCL_DT_F32 ? 4 : 8;
   return aligned(p, 16) && s.b % ve == 0 && s.n % ve == 0 && s.h % ve == 0;
 }
+// the rows of a block are addressed by 32-bit byte offsets from its first
+static bool near_rows(const Str &s) { return s.n >= 0 && s.n < (1LL << 22); }
 
 }  // namespace tcl
 
@@ -966,8 +1027,8 @@ extern "C" size_t tcl_block_attention_fwd_workspace_bytes(int64_t B, int64_t Nq,
                                                           int64_t q_block) {
   AttnArgs a{};
   if (attn_setup(a, B, Nq, Nk, Hq, Hkv, D, top_k, block, q_block, 1.0, TCL_DT_F32) != TCL_OK) return 256;
-  const int64_t works = B * Hkv * a.S * cdiv(a.rows, fwd_rows(a));
-  return fwd_part_bytes(a, works, fwd_splits(a, works));
+  const FwdPlan p = fwd_plan(a, true), q = fwd_plan(a, false);   // either type's
+  return p.part > q.part ? p.part : q.part;
 }
 
 extern "C" int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh,
@@ -984,19 +1045,19 @@ extern "C" int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn
   a.sq = Str{q_sb, q_sn, q_sh}; a.sk = Str{k_sb, k_sn, k_sh}; a.sv = Str{v_sb, v_sn, v_sh}; a.so = Str{o_sb, o_sn, o_sh};
   TCL_REQUIRE(rows16(q, a.sq, dtype) && (Nk == 0 || (rows16(k, a.sk, dtype) && rows16(v, a.sv, dtype))) && rows16(out, a.so, dtype), TCL_ERR_ARG,
               "block_attention: rows must start on 16 bytes");
-  a.chunks = (int)cdiv(a.rows, fwd_rows(a));
-  const int64_t works = B * Hkv * a.S * a.chunks;
-  a.splits = fwd_splits(a, works);
-  const int64_t blocks_n = works * a.splits;
-  TCL_REQUIRE(blocks_n < (1LL << 31), TCL_ERR_SHAPE, "block_attention: grid of %ld blocks", (long)blocks_n);
-  const size_t need = fwd_part_bytes(a, works, a.splits);
-  TCL_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, TCL_ERR_WORKSPACE, "block_attention: workspace of %zu bytes needed", need);
+  TCL_REQUIRE(near_rows(a.sk) && near_rows(a.sv), TCL_ERR_UNSUPPORTED, "block_attention: keys lie more than 2^22 elements apart");
+  const bool f32 = dtype == TCL_DT_F32;
+  const FwdPlan plan = fwd_plan(a, f32);
+  a.chunks = plan.chunks;
+  a.splits = plan.splits;
+  const int64_t blocks_n = plan.works * a.splits;
+  TCL_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= plan.part, TCL_ERR_WORKSPACE, "block_attention: workspace of %zu bytes needed", plan.part);
   a.part = (float *)workspace;
   const hipStream_t s = (hipStream_t)stream;
   const int r = dtype == TCL_DT_F32 ? fwd_by_dim<float>(a, blocks_n, s) : dtype == TCL_DT_BF16 ? fwd_by_dim<__bf16>(a, blocks_n, s) : fwd_by_dim<_Float16>(a, blocks_n, s);
   if (r != TCL_OK || a.splits == 1) return r;
-  const int M = fwd_rows(a);
-  const dim3 grid((unsigned)cdiv(works * M, 4));
+  const int M = fwd_rows(a, f32);
+  const dim3 grid((unsigned)cdiv(plan.works * M, 4));
   if (dtype == TCL_DT_F32) hipLaunchKernelGGL((attend_join_kernel<float>), grid, dim3(256), 0, s, a, M);
   else if (dtype == TCL_DT_BF16) hipLaunchKernelGGL((attend_join_kernel<__bf16>), grid, dim3(256), 0, s, a, M);
   else hipLaunchKernelGGL((attend_join_kernel<_Float16>), grid, dim3(256), 0, s, a, M);
@@ -1029,6 +1090,7 @@ extern "C" int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64
   TCL_REQUIRE(rows16(q, a.sq, dtype) && rows16(k, a.sk, dtype) && rows16(v, a.sv, dtype) && rows16(out, a.so, dtype) && rows16(grad_out, a.sdo, dtype) &&
               (!g_q || rows16(g_q, a.sdq, dtype)) && (!g_k || rows16(g_k, a.sdk, dtype)) && (!g_v || rows16(g_v, a.sdv, dtype)), TCL_ERR_ARG,
               "block_attention backward: rows must start on 16 bytes");
+  TCL_REQUIRE(near_rows(a.sk) && near_rows(a.sv), TCL_ERR_UNSUPPORTED, "block_attention backward: keys lie more than 2^22 elements apart");
   const size_t need = tcl_block_attention_bwd_workspace_bytes(B, Nq, Nk, Hq, Hkv, D, top_k, block, q_block);
   TCL_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, TCL_ERR_WORKSPACE, "block_attention backward: workspace of %zu bytes needed", need);
   a.delta = (float *)workspace;
