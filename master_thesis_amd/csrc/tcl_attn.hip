@@ -100,19 +100,39 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// ROWS rows -> image.  at(row) -> pointer to the row's first channel, or null for a row of zeros; chunks beyond `chunks` are zeros.
-// Called by all 256 threads.
-template <typename T, int DP, int ROWS, typename F> __device__ __forceinline__ void dma_rows(char *img, int chunks, F at) {
+// Where the pieces of this thread lie: piece u of an image of ROWS rows is row u * RPU + threadIdx.x / NCH, chunk `ch` of it (the
+// same for every u, or one of two in turn where a step is 8 rows)
+template <typename T, int DP, int ROWS> struct Pieces {
   typedef Img<T, DP> I;
-  constexpr int PIECES = ROWS * I::NCH;
-  const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
+  static constexpr int RPU = 256 / I::NCH, NU = (ROWS * I::NCH + 255) / 256;
+  static constexpr bool whole = ROWS * I::NCH % 256 == 0;
+  __device__ __forceinline__ static int row(int u) { return u * RPU + (int)threadIdx.x / I::NCH; }
+  __device__ __forceinline__ static int chunk(int u) { return ((int)threadIdx.x % I::NCH) ^ I::swz(row(u)); }
+  __device__ __forceinline__ static bool any(int u, int wave) { return whole || u * 256 + wave * 64 < ROWS * I::NCH; }   // wave-uniform
+  __device__ __forceinline__ static char *dst(char *img, int u, int wave) { return img + (u * 256 + wave * 64) * 16; }
+};
+
+// ROWS rows that lie `st` bytes apart, from row `off` of the 64 that `mask` speaks of -> image; rows the mask leaves out and chunks
+// beyond `chunks` are zeros.  `base`, `st`, `mask`, `off` are uniform: a tile without holes costs no vector instruction but the loads.
+template <typename T, int DP, int ROWS> __device__ __forceinline__ void dma_segment(char *img, const char *base, unsigned st, uint64_t mask, int off, int chunks, int wave) {
+  typedef Pieces<T, DP, ROWS> P;
+  base += (size_t)((unsigned)off * st);
+  mask >>= off;
+  const uint64_t need = ROWS >= 64 ? ~0ull : (1ull << ROWS) - 1;
+  if ((mask & need) == need && chunks == DP / P::I::VE && P::I::NCH == DP / P::I::VE) {
 #pragma unroll
-  for (int u = 0; u < (PIECES + 255) / 256; ++u) {
-    const int first = u * 256 + (int)(threadIdx.x & ~63u);
-    if (PIECES % 256 && first >= PIECES) break;                  // wave-uniform
-    const int id = u * 256 + threadIdx.x, row = id / I::NCH, ch = (id % I::NCH) ^ I::swz(row);
-    const char *p = at(row);
-    dma16(p != nullptr && ch < chunks ? p + ch * 16 : zero, img + (size_t)__builtin_amdgcn_readfirstlane(first) * 16);
+    for (int u = 0; u < P::NU; ++u)
+      if (P::any(u, wave)) dma16(base + ((unsigned)P::row(u) * st + (unsigned)P::chunk(u) * 16), P::dst(img, u, wave));
+  } else {
+    const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
+#pragma unroll
+    for (int u = 0; u < P::NU; ++u)
+      if (P::any(u, wave)) {
+        const uint32_t half = P::RPU > 32 ? (P::row(u) < 32 ? (uint32_t)mask : (uint32_t)(mask >> 32)) : u * P::RPU < 32 ? (uint32_t)mask : (uint32_t)(mask >> 32);
+        const bool in = ((half >> (P::row(u) & 31)) & 1) && P::chunk(u) < chunks;
+        const char *p = base + ((unsigned)P::row(u) * st + (unsigned)P::chunk(u) * 16);
+        dma16(in ? p : zero, P::dst(img, u, wave));
+      }
   }
 }
 
@@ -195,23 +215,23 @@ struct Segment {
   int key0;                                                      // first key, or -1: none
   uint64_t mask;                                                 // bit r: key0 + r exists and is seen
 };
-// the raw parts of a segment: issued a tile before they are needed
+// The raw parts of a segment are asked for a tile before they are needed.  The load is unconditional (clamped): a load behind a
+// condition would be waited for where the paths meet, and with it the tile that is on its way.
 struct SegmentLoad { int key0; float seen; };
+static __device__ const float g_one = 1.f;
 struct KeySource {
   const int *list;
   const float *vis;
-  int n, lb, nk;                                                 // segments, log2 of the block, keys
-  __device__ __forceinline__ SegmentLoad load(int i) const {
-    SegmentLoad r{-1, 0.f};
-    if (i < n) {
-      const int per = lb - 6;
-      r.key0 = __builtin_amdgcn_readfirstlane((list[i >> per] << lb) + ((i & ((1 << per) - 1)) << 6));
-      const int key = r.key0 + (int)(threadIdx.x & 63);
-      if (key < nk) r.seen = vis ? vis[key] : 1.f;
-    }
-    return r;
+  int vis_step, n, lb, nk;                                       // segments, log2 of the block, keys
+  __device__ __forceinline__ SegmentLoad load(int i) const {     // n > 0
+    const int per = lb - 6, j = min(i, n - 1);
+    const int key0 = __builtin_amdgcn_readfirstlane((list[j >> per] << lb) + ((j & ((1 << per) - 1)) << 6));
+    const int key = min(key0 + (int)(threadIdx.x & 63), nk - 1);
+    return SegmentLoad{i < n ? key0 : -1, *(const __attribute__((address_space(1))) float *)(vis + (int64_t)key * vis_step)};
   }
-  __device__ __forceinline__ static Segment finish(const SegmentLoad &l) { return Segment{l.key0, __ballot(l.seen > 0.5f)}; }
+  __device__ __forceinline__ Segment finish(const SegmentLoad &l) const {
+    return Segment{l.key0, l.key0 < 0 ? 0ull : __ballot(l.seen > 0.5f && l.key0 + (int)(threadIdx.x & 63) < nk)};
+  }
 };
 
 // One workgroup: M = 16 NQ WM query rows of one group (a row = one query token and one head of the key head's group), 4 waves as WM
@@ -246,7 +266,7 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
 
   const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + s) * a.top, a.top, a.nb, bits, list, &n_list);
   const int e0 = (int)((int64_t)n * split / a.splits), e1 = (int)((int64_t)n * (split + 1) / a.splits);
-  const KeySource keys{list + e0, a.vis ? a.vis + (int64_t)b * a.Nk : nullptr, (e1 - e0) << (a.lb - 6), a.lb, a.Nk};
+  const KeySource keys{list + e0, a.vis ? a.vis + (int64_t)b * a.Nk : &g_one, a.vis != nullptr, (e1 - e0) << (a.lb - 6), a.lb, a.Nk};
   const int nt = (keys.n * 64 + TK - 1) / TK;
   const char *kb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h);
   const char *vb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h);
@@ -267,23 +287,24 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
   };
   auto issue = [&](int t, const Segment *sg) {
     char *kd = smem + (t & 1) * 2 * F::img, *vd = kd + F::img;
+    constexpr int R = TK < 64 ? TK : 64;
     const int off = TK < 64 ? (t * TK) & 63 : 0;                 // within the segment
-    auto at = [&](const char *base, int64_t n, unsigned st, int r) -> const char * {
-      const Segment &x = sg[NS > 1 ? r / 64 : 0];
-      const int rr = (r & 63) + off;
-      return (x.mask >> rr) & 1 ? base + (int64_t)x.key0 * n * (int64_t)sizeof(T) + (unsigned)rr * st : nullptr;
-    };
-    dma_rows<T, DP, TK>(kd, chunks, [&](int r) { return at(kb, a.sk.n, kst, r); });
-    dma_rows<T, DP, TK>(vd, chunks, [&](int r) { return at(vb, a.sv.n, vst, r); });
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      dma_segment<T, DP, R>(kd + i * 64 * Img<T, DP>::RB, kb + (int64_t)sg[i].key0 * a.sk.n * (int64_t)sizeof(T), kst, sg[i].mask, off, chunks, wave);
+      dma_segment<T, DP, R>(vd + i * 64 * Img<T, DP>::RB, vb + (int64_t)sg[i].key0 * a.sv.n * (int64_t)sizeof(T), vst, sg[i].mask, off, chunks, wave);
+    }
   };
 
-  Segment cur[NS], nxt[NS];
-  SegmentLoad raw[NS];
-  seg_load(0, raw);
+  Segment cur[NS] = {}, nxt[NS] = {};
+  SegmentLoad raw[NS] = {};
+  if (nt > 0) {
+    seg_load(0, raw);
 #pragma unroll
-  for (int i = 0; i < NS; ++i) cur[i] = KeySource::finish(raw[i]);
-  if (nt > 0) issue(0, cur);
-  seg_load(1, raw);
+    for (int i = 0; i < NS; ++i) cur[i] = keys.finish(raw[i]);
+    issue(0, cur);
+    seg_load(1, raw);
+  }
 
   // the queries, as columns; a negative scale turns their sign, so that the largest product is the largest score
   frag qf[NQ][KC];
@@ -312,7 +333,7 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 #pragma unroll
-  for (int i = 0; i < NS; ++i) nxt[i] = KeySource::finish(raw[i]);
+  for (int i = 0; i < NS; ++i) nxt[i] = keys.finish(raw[i]);
   for (int t = 0; t < nt; ++t) {
     tile_barrier();                                              // tile t is there, tile t - 1 has been read
     if (t + 1 < nt) issue(t + 1, nxt);
@@ -376,10 +397,11 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < NQ; ++i) o[i][d] = mma(vf, pf[i], o[i][d]);
     }
+    __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       cur[i] = nxt[i];
-      nxt[i] = KeySource::finish(raw[i]);
+      nxt[i] = keys.finish(raw[i]);
     }
   }
 
@@ -552,7 +574,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   const int s = (int)(item % a.S);
   const int bh = (int)(item / a.S), hk = bh % a.Hkv, b = bh / a.Hkv;
   const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + s) * a.top, a.top, a.nb, bits, list, &n_list);
-  const KeySource keys{list, a.vis ? a.vis + (int64_t)b * a.Nk : nullptr, n << (a.lb - 6), a.lb, a.Nk};
+  const KeySource keys{list, a.vis ? a.vis + (int64_t)b * a.Nk : &g_one, a.vis != nullptr, n << (a.lb - 6), a.lb, a.Nk};
   const int nt = keys.n * 64 / TK;
   const char *kb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h);
   const char *vb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h);
@@ -568,15 +590,16 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   auto issue = [&](int t, const Segment &x) {
     char *kd = smem + (t & 1) * 2 * F::img, *vd = kd + F::img;
     const int off = (t * TK) & 63;
-    auto at = [&](const char *base, int64_t n, unsigned st, int r) -> const char * {
-      return (x.mask >> (r + off)) & 1 ? base + (int64_t)x.key0 * n * (int64_t)sizeof(T) + (unsigned)(r + off) * st : nullptr;
-    };
-    dma_rows<T, DP, TK>(kd, chunks, [&](int r) { return at(kb, a.sk.n, kst, r); });
-    dma_rows<T, DP, TK>(vd, chunks, [&](int r) { return at(vb, a.sv.n, vst, r); });
+    dma_segment<T, DP, TK>(kd, kb + (int64_t)x.key0 * a.sk.n * (int64_t)sizeof(T), kst, x.mask, off, chunks, wave);
+    dma_segment<T, DP, TK>(vd, vb + (int64_t)x.key0 * a.sv.n * (int64_t)sizeof(T), vst, x.mask, off, chunks, wave);
   };
-  Segment cur = KeySource::finish(keys.load(0)), nxt;
-  if (nt > 0) issue(0, cur);
-  SegmentLoad raw = keys.load(TK / 64);
+  Segment cur = {}, nxt = {};
+  SegmentLoad raw = {};
+  if (nt > 0) {
+    cur = keys.finish(keys.load(0));
+    issue(0, cur);
+    raw = keys.load(TK / 64);
+  }
 
   frag qf[NQ][KC], df[NQ][KC];
   float lse2[NQ], delta[NQ];
@@ -611,7 +634,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   for (int i = 0; i < NQ; ++i)
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  nxt = KeySource::finish(raw);
+  nxt = keys.finish(raw);
   for (int t = 0; t < nt; ++t) {
     tile_barrier();
     if (t + 1 < nt) issue(t + 1, nxt);
@@ -651,8 +674,9 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < NQ; ++i) o[i][d] = mma(kf, gf[i], o[i][d]);
     }
+    __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
     cur = nxt;
-    nxt = KeySource::finish(raw);
+    nxt = keys.finish(raw);
   }
   float *jo = reinterpret_cast<float *>(smem);
   __syncthreads();
@@ -781,46 +805,57 @@ __global__ __launch_bounds__(256, OCC) void attend_dkv_kernel(AttnArgs a) {
       where.y = ((int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h) * (int64_t)sizeof(T);
       return ((int64_t)b * a.Hq + head) * a.Nq + token;
     };
-    auto stat = [&](int64_t at, float &ls, float &de) {
-      ls = kPosInf;                                              // exp2(x - inf) = 0
-      de = 0.f;
-      if (at >= 0) {
-        const float x = a.lse[at];
-        ls = x == kNegInf ? kPosInf : x * kLog2e - PScale<T>::bits;
-        de = a.delta[at];
+    // statistics of a row, asked for a tile before they are needed (unconditional, clamped loads)
+    auto stat_load = [&](int64_t at, float &ls, float &de) {
+      ls = a.lse[at < 0 ? 0 : at];
+      de = a.delta[at < 0 ? 0 : at];
+    };
+    auto stat_store = [&](int64_t at, float ls, float de, int slot) {
+      if (tid < TR) {
+        lse2[slot * TR + tid] = at < 0 || ls == kNegInf ? kPosInf : ls * kLog2e - PScale<T>::bits;   // exp2(x - inf) = 0
+        delta[slot * TR + tid] = at < 0 ? 0.f : de;
       }
     };
     auto issue = [&](int t) {
+      typedef Pieces<T, DP, TR> P;
       char *qd = smem + (t & 1) * 2 * F::img, *dd = qd + F::img;
       const longlong2 *tb = tab + (t & 1) * TR;
-      dma_rows<T, DP, TR>(qd, chunks, [&](int r) -> const char * { const int64_t x = tb[r].x; return x < 0 ? nullptr : qb + x; });
-      dma_rows<T, DP, TR>(dd, chunks, [&](int r) -> const char * { const longlong2 x = tb[r]; return x.x < 0 ? nullptr : db + x.y; });
+      const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
+      longlong2 x[P::NU];
+#pragma unroll
+      for (int u = 0; u < P::NU; ++u) x[u] = tb[P::whole ? P::row(u) : min(P::row(u), TR - 1)];
+#pragma unroll
+      for (int u = 0; u < P::NU; ++u)
+        if (P::any(u, wave)) {
+          const bool in = x[u].x >= 0 && P::chunk(u) < chunks;
+          dma16(in ? qb + (x[u].x + P::chunk(u) * 16) : zero, P::dst(qd, u, wave));
+          dma16(in ? db + (x[u].y + P::chunk(u) * 16) : zero, P::dst(dd, u, wave));
+        }
     };
-    // rows of tiles 0 and 1, statistics of tile 0; from here on rows are located two tiles ahead, statistics fetched one ahead
+    // rows of tiles 0 and 1, statistics of tile 0; from here on wave 0 locates rows two tiles ahead and fetches statistics one ahead
     int64_t st_next = -1;
-    if (tid < TR) {
+    if (wave == 0) {
       longlong2 w;
       float ls, de;
       const int64_t at = locate(0, w);
-      tab[tid] = w;
-      stat(at, ls, de);
-      lse2[tid] = ls;
-      delta[tid] = de;
+      if (tid < TR) tab[tid] = w;
+      stat_load(at, ls, de);
+      stat_store(at, ls, de, 0);
       st_next = locate(1, w);
-      tab[TR + tid] = w;
+      if (tid < TR) tab[TR + tid] = w;
     }
     __syncthreads();
     issue(0);
     for (int t = 0; t < nt; ++t) {
       tile_barrier();
       if (t + 1 < nt) issue(t + 1);
-      float ls_n, de_n;
+      float ls_n = 0.f, de_n = 0.f;
       int64_t st_next2 = -1;
-      if (tid < TR) {
-        stat(st_next, ls_n, de_n);
+      if (wave == 0) {
+        stat_load(st_next, ls_n, de_n);
         longlong2 w;
         st_next2 = locate(t + 2, w);
-        tab[(t & 1) * TR + tid] = w;                             // tile t's rows are on their way already
+        if (tid < TR) tab[(t & 1) * TR + tid] = w;               // tile t's rows are on their way already
       }
       const char *qrows = smem + (t & 1) * 2 * F::img, *drows = qrows + F::img;
       f32x4 sc[2][NK], dp[2][NK];
@@ -863,10 +898,8 @@ __global__ __launch_bounds__(256, OCC) void attend_dkv_kernel(AttnArgs a) {
           gk[i][d] = mma(qf, gf[i], gk[i][d]);
         }
       }
-      if (tid < TR) {
-        lse2[((t + 1) & 1) * TR + tid] = ls_n;
-        delta[((t + 1) & 1) * TR + tid] = de_n;
-      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (wave == 0) stat_store(st_next, ls_n, de_n, (t + 1) & 1);
       st_next = st_next2;
     }
   }
