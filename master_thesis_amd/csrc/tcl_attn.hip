@@ -93,6 +93,18 @@ static __device__ __attribute__((aligned(16))) const uint32_t g_zero_chunk[4] = 
 __device__ __forceinline__ void dma16(const char *src, char *lds) {   // lds: of the wave's first lane
   __builtin_amdgcn_global_load_lds((glb_cvptr)src, (lds_vptr)lds, 16, 0, 0);
 }
+// maximum without the quieting instructions of fmaxf (a NaN may come out as the other operand, as it may there)
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, kPosInf); }
+// maximum over lanes l, l ^ 16, l ^ 32, l ^ 48: the swaps leave rows (halves) of both halves in both operands
+__device__ __forceinline__ float quarter_max(float x) {
+  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+  const unsigned u = __float_as_uint(x);
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const float y = max2(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const unsigned w = __float_as_uint(y);
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return max2(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 // every LDS-DMA of this wave has landed and every LDS read of it has been served; then the workgroup meets
 __device__ __forceinline__ void tile_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -214,6 +226,7 @@ __device__ __forceinline__ int group_blocks(const int32_t *blocks, int top, int 
 struct Segment {
   int key0;                                                      // first key, or -1: none
   uint64_t mask;                                                 // bit r: key0 + r exists and is seen
+  __device__ __forceinline__ uint64_t there(int nk) const { return key0 < 0 ? 0ull : key0 + 64 <= nk ? ~0ull : (1ull << (nk - key0)) - 1; }
 };
 // The raw parts of a segment are asked for a tile before they are needed.  The load is unconditional (clamped): a load behind a
 // condition would be waited for where the paths meet, and with it the tile that is on its way.
@@ -291,7 +304,8 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     const int off = TK < 64 ? (t * TK) & 63 : 0;                 // within the segment
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      dma_segment<T, DP, R>(kd + i * 64 * Img<T, DP>::RB, kb + (int64_t)sg[i].key0 * a.sk.n * (int64_t)sizeof(T), kst, sg[i].mask, off, chunks, wave);
+      // a hidden key's score is overwritten, so its row may be anything; its value row is multiplied by a probability of 0
+      dma_segment<T, DP, R>(kd + i * 64 * Img<T, DP>::RB, kb + (int64_t)sg[i].key0 * a.sk.n * (int64_t)sizeof(T), kst, sg[i].there(a.Nk), off, chunks, wave);
       dma_segment<T, DP, R>(vd + i * 64 * Img<T, DP>::RB, vb + (int64_t)sg[i].key0 * a.sv.n * (int64_t)sizeof(T), vst, sg[i].mask, off, chunks, wave);
     }
   };
@@ -366,10 +380,11 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     float f[NQ];
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      float mx = fmaxf(fmaxf(fmaxf(sc[0][i][0], sc[0][i][1]), fmaxf(sc[0][i][2], sc[0][i][3])), fmaxf(fmaxf(sc[1][i][0], sc[1][i][1]), fmaxf(sc[1][i][2], sc[1][i][3])));
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m[i], mx * sc2);
+      float mx = max2(sc[0][i][0], sc[0][i][1]);
+#pragma unroll
+      for (int e = 2; e < 8; ++e) mx = max2(mx, sc[e / 4][i][e % 4]);
+      mx = quarter_max(mx);
+      const float mn = max2(m[i], mx * sc2);
       const float ms = mn == kNegInf ? 0.f : mn;                 // nothing seen yet: exp2(-inf - 0) = 0
       f[i] = __builtin_amdgcn_exp2f(m[i] - ms);                  // exactly 1 while the maximum stays
       grew |= mn > m[i];
@@ -469,35 +484,47 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
   }
 }
 
-// Joins the splits of a row: one wave per row, 4 rows per workgroup.
+// Joins the splits (at most 64) of a row: one workgroup per row.  Lane x of every wave holds split x's factor; the waves take the
+// splits in turn, a lane two channels of them, and are added up in wave order.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
-  const int64_t id = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  const int lane = threadIdx.x % 64;
-  const int64_t works = (int64_t)a.B * a.Hkv * a.S * a.chunks;
-  const int64_t work = id / M;
-  const int r = (int)(id - work * M);
-  if (work >= works) return;
+  __shared__ float2 sums[4][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int64_t work = blockIdx.x / (unsigned)M;
+  const int r = (int)(blockIdx.x - (unsigned)work * (unsigned)M);
   const int chunk = (int)(work % a.chunks), s = (int)(work / a.chunks % a.S);
   const int bh = (int)(work / a.chunks / a.S), hk = bh % a.Hkv, b = bh / a.Hkv;
   const int row = chunk * M + r, t = (int)a.by_g.div((unsigned)row), token = s * a.q_block + t, head = hk * a.G + (row - t * a.G);
   if (row >= a.rows || token >= a.Nq) return;
   const int64_t step = (int64_t)M * (a.D + 2);
   const float *p = a.part + work * a.splits * step;
-  float mx = kNegInf, sum = 0.f;
-  for (int x = 0; x < a.splits; ++x) mx = fmaxf(mx, p[x * step + (int64_t)M * a.D + r]);
-  for (int x = 0; x < a.splits; ++x) {
-    const float mi = p[x * step + (int64_t)M * a.D + r];
-    if (mi != kNegInf) sum += p[x * step + (int64_t)M * a.D + M + r] * __builtin_amdgcn_exp2f(mi - mx);
+  const int x = min(lane, a.splits - 1);
+  const float m = lane < a.splits ? p[x * step + (int64_t)M * a.D + r] : kNegInf;
+  const float l = p[x * step + (int64_t)M * a.D + M + r];
+  const float mx = wave_max(m);
+  const float w = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+  const float sum = wave_sum(m == kNegInf ? 0.f : l * w);
+  const int ch = min(lane * 2, a.D - 2);
+  float2 o = {0.f, 0.f};
+  for (int i = wave; i < a.splits; i += 4) {
+    const float2 v = *reinterpret_cast<const float2 *>(p + i * step + (int64_t)r * a.D + ch);
+    const float f = __shfl(w, i, 64);
+    o.x += f == 0.f ? 0.f : v.x * f;
+    o.y += f == 0.f ? 0.f : v.y * f;
+  }
+  sums[wave][lane] = o;
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    o.x += sums[i][lane].x;
+    o.y += sums[i][lane].y;
   }
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-  for (int ch = lane; ch < a.D; ch += 64) {
-    float o = 0.f;
-    for (int x = 0; x < a.splits; ++x) {
-      const float mi = p[x * step + (int64_t)M * a.D + r];
-      if (mi != kNegInf) o += p[x * step + (int64_t)r * a.D + ch] * __builtin_amdgcn_exp2f(mi - mx);
-    }
-    reinterpret_cast<T *>(a.out)[(int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch] = (T)(o * inv);
+  if (lane * 2 < a.D) {
+    T *y = reinterpret_cast<T *>(a.out) + (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch;
+    y[0] = (T)(o.x * inv);
+    y[1] = (T)(o.y * inv);
   }
   if (lane == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx + __builtin_log2f(sum)) * kLn2;
 }
@@ -977,8 +1004,7 @@ template <typename T, int DP> static int launch_dq(AttnArgs a, hipStream_t s) {
 template <typename T, int DP> static int launch_dkv(const AttnArgs &a, hipStream_t s) {
   const char *what = "block_attention backward (keys)";
   const int64_t blocks = cdiv(a.Nk, 64) * a.B * a.Hkv;
-  if constexpr (sizeof(T) == 4) return launch(attend_dkv_kernel<T, DP, 1, 4, 1, 1>, DkvTile<T, DP, 1, 4, 1>::bytes, blocks, a, s, what);
-  else return launch(attend_dkv_kernel<T, DP, 2, 2, 2, 1>, DkvTile<T, DP, 2, 2, 2>::bytes, blocks, a, s, what);
+  return launch(attend_dkv_kernel<T, DP, 1, 4, 1, 2>, DkvTile<T, DP, 1, 4, 1>::bytes, blocks, a, s, what);
 }
 
 // head sizes are padded to a multiple of 32 in LDS and registers
@@ -1090,7 +1116,8 @@ extern "C" int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn
   const int r = dtype == TCL_DT_F32 ? fwd_by_dim<float>(a, blocks_n, s) : dtype == TCL_DT_BF16 ? fwd_by_dim<__bf16>(a, blocks_n, s) : fwd_by_dim<_Float16>(a, blocks_n, s);
   if (r != TCL_OK || a.splits == 1) return r;
   const int M = fwd_rows(a, f32);
-  const dim3 grid((unsigned)cdiv(plan.works * M, 4));
+  TCL_REQUIRE(plan.works * M < (1LL << 31), TCL_ERR_SHAPE, "block_attention: too many rows for one call");
+  const dim3 grid((unsigned)(plan.works * M));
   if (dtype == TCL_DT_F32) hipLaunchKernelGGL((attend_join_kernel<float>), grid, dim3(256), 0, s, a, M);
   else if (dtype == TCL_DT_BF16) hipLaunchKernelGGL((attend_join_kernel<__bf16>), grid, dim3(256), 0, s, a, M);
   else hipLaunchKernelGGL((attend_join_kernel<_Float16>), grid, dim3(256), 0, s, a, M);
