@@ -105,9 +105,9 @@ __device__ __forceinline__ float quarter_max(float x) {
   const u32x2 b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
   return max2(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-// every LDS-DMA of this wave has landed and every LDS read of it has been served; then the workgroup meets
-__device__ __forceinline__ void tile_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+// all but the last N LDS-DMAs of this wave have landed and every LDS read of it has been served; then the workgroup meets
+template <int N> __device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
 #pragma unroll
   for (int i = 0; i < NS; ++i) nxt[i] = keys.finish(raw[i]);
   for (int t = 0; t < nt; ++t) {
-    tile_barrier();                                              // tile t is there, tile t - 1 has been read
+    tile_barrier<0>();                                              // tile t is there, tile t - 1 has been read
     if (t + 1 < nt) issue(t + 1, nxt);
     seg_load(t + 2, raw);
     const char *krows = smem + (t & 1) * 2 * F::img, *vrows = krows + F::img;
@@ -663,7 +663,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   nxt = keys.finish(raw);
   for (int t = 0; t < nt; ++t) {
-    tile_barrier();
+    tile_barrier<0>();
     if (t + 1 < nt) issue(t + 1, nxt);
     raw = keys.load((t + 2) * TK / 64);
     const char *krows = smem + (t & 1) * 2 * F::img, *vrows = krows + F::img;
@@ -693,7 +693,9 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
         for (int e = 0; e < 4; ++e) {
           float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i][e], a.c, -lse2[i]));
           p = (seen >> (u * 16 + e)) & 1 ? p : 0.f;              // an unseen key's products are those of zeros
-          gf[i][u * 4 + e] = (T)(p * (dp[u][i][e] - delta[i]) * a.scale);
+          float ds = p * (dp[u][i][e] - delta[i]);
+          if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= a.scale;   // fp16: small score gradients; else the scale comes last
+          gf[i][u * 4 + e] = (T)ds;
         }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -727,7 +729,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     const int r = id / per, ch = (id - r * per) * 4;
     int token, head;
     if (!row_of(r, token, head)) continue;
-    const f32x4 x = *reinterpret_cast<const f32x4 *>(jo + r * (DP + 4) + ch);
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(jo + r * (DP + 4) + ch) * (sizeof(T) == 2 && PScale<T>::bits > 0.f ? 1.f : a.scale);
     typename Vec4<T>::type y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
@@ -735,70 +737,74 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   }
 }
 
-// One workgroup: 16 NK WM keys (a tile of one block) against all query rows of the groups that chose the block.  The rows pass as a
-// stream (group after group, in ascending order) in tiles of TR = 32 WN; rows and keys have changed places with the forward:
+// One workgroup: 64 keys (a tile of one block), 16 per wave, against all query rows of the groups that chose the block.  The rows pass
+// as a stream (group after group, in ascending order) in tiles of 32; rows and keys have changed places with the forward:
 // S = Q K^T leaves a lane the probabilities of ITS key, the operand of dV^T = dout^T P and, as dS, of dK^T = Q^T dS.
-constexpr int kWindow = 32;   // words of group bits taken at a time: up to 1024 groups in the list
+// 16 keys a wave: with 32 (half the LDS reads per product) the two accumulators take 350 registers, one wave per SIMD, and
+// every wait shows (802 against 594 us for the training step of 63,600 keys).  Rows lie scattered, so their tiles come from a ring
+// of four, three tiles ahead; where the rows lie is worked out for 512 of them at a time, not in the loop.
+constexpr int kWindow = 32;    // words of group bits taken at a time: up to 1024 groups in the list
+constexpr int kBatch = 512;    // rows located at a time
 
-template <typename T, int DP, int NK, int WM, int WN> struct DkvTile {
-  static constexpr int M = 16 * NK * WM, TR = 32 * WN;
-  static constexpr size_t img = (size_t)TR * Img<T, DP>::RB, tiles = 4 * img;          // Q and dout, twice
+template <typename T, int DP> struct DkvTile {
+  static constexpr int M = 64, TR = 32, NB = sizeof(T) == 4 && DP > 64 ? 2 : 4;
+  static constexpr size_t img = (size_t)TR * Img<T, DP>::RB, tiles = NB * 2 * img;     // Q and dout
   static constexpr size_t join = (size_t)M * (DP + 4) * 4;
   static constexpr size_t body = tiles > join ? tiles : join;
-  // behind the tiles: byte offsets of a tile's rows in q and dout, lse and delta (twice each), the list of groups
-  static constexpr size_t bytes = body + 2 * TR * 16 + 2 * TR * 8 + 32 * kWindow * 4;
+  // behind the tiles: where a row lies in q and dout (in 16 bytes), lse and delta, the list of groups
+  static constexpr size_t bytes = body + kBatch * 16 + 32 * kWindow * 4;
 };
-template <typename T, int DP, int NK, int WM, int WN, int OCC>
-__global__ __launch_bounds__(256, OCC) void attend_dkv_kernel(AttnArgs a) {
-  typedef DkvTile<T, DP, NK, WM, WN> F;
-  constexpr int M = F::M, TR = F::TR, KC = DP / 32, DT = DP / 16;
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
+  typedef DkvTile<T, DP> F;
+  typedef Pieces<T, DP, F::TR> P;
+  constexpr int M = F::M, TR = F::TR, NB = F::NB, KC = DP / 32, DT = DP / 16, PER = 2 * P::NU;
   typedef typename Vec8<T>::type frag;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  longlong2 *tab = reinterpret_cast<longlong2 *>(smem + F::body);                      // [2][TR], x < 0: no row
-  float *lse2 = reinterpret_cast<float *>(tab + 2 * TR), *delta = lse2 + 2 * TR;       // [2][TR] each
-  int *list = reinterpret_cast<int *>(delta + 2 * TR);                                 // [32 kWindow]
+  uint2 *tab = reinterpret_cast<uint2 *>(smem + F::body);                              // [kBatch], x = ~0: no row
+  float *lse2 = reinterpret_cast<float *>(tab + kBatch), *delta = lse2 + kBatch;       // [kBatch] each
+  int *list = reinterpret_cast<int *>(delta + kBatch);                                 // [32 kWindow]
   __shared__ int n_list;
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % 16, g = lane / 16;
-  const int wm = wave / WN, wn = wave % WN;
   const int tiles_of = (a.Nk + M - 1) / M;
   unsigned item = xcd_remap(blockIdx.x, gridDim.x);
   const int kt = (int)(item % tiles_of);
   const int bh = (int)(item / tiles_of), hk = bh % a.Hkv, b = bh / a.Hkv;
   const uint32_t *inv = a.inv + ((int64_t)bh * a.nb + (((int64_t)kt * M) >> a.lb)) * a.words;
 
-  frag kf[NK][KC], vf[NK][KC];
-  bool seen[NK];
-#pragma unroll
-  for (int i = 0; i < NK; ++i) {
-    const int key = kt * M + (wm * NK + i) * 16 + col;
-    const bool ok = key < a.Nk && (!a.vis || a.vis[(int64_t)b * a.Nk + key] > 0.5f);
-    seen[i] = ok;
+  // this lane's key.  A hidden key's row is taken as zeros: whatever its probabilities come to stays in its own column, which is
+  // not written.
+  frag kf[KC], vf[KC];
+  const int key = kt * M + wave * 16 + col;
+  const bool seen = key < a.Nk && (!a.vis || a.vis[(int64_t)b * a.Nk + key] > 0.5f);
+  {
     const T *p = reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)key * a.sk.n + (int64_t)hk * a.sk.h;
     const T *q = reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)key * a.sv.n + (int64_t)hk * a.sv.h;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
       const int ch = c * 32 + g * 8;
       frag t = {}, u = {};
-      if (ok && ch < a.D) {
+      if (seen && ch < a.D) {
         t = *reinterpret_cast<const frag *>(p + ch);
         u = *reinterpret_cast<const frag *>(q + ch);
       }
-      kf[i][c] = t;
-      vf[i][c] = u;
+      kf[c] = t;
+      vf[c] = u;
     }
   }
   const char *qb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sq.b);
   const char *db = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.dout) + (int64_t)b * a.sdo.b);
-  const int chunks = a.D / Img<T, DP>::VE;
-  f32x4 gk[NK][DT], gv[NK][DT];
+  const int chunks = a.D / P::I::VE;
+  // fp16: scale on each score gradient (they stay small); else once, on the sums
+  const float each = sizeof(T) == 2 && PScale<T>::bits > 0.f ? a.scale * PScale<T>::inv : 1.f;
+  const float k_scale = sizeof(T) == 2 && PScale<T>::bits > 0.f ? 1.f : a.scale;
+  f32x4 gk[DT], gv[DT];
 #pragma unroll
-  for (int i = 0; i < NK; ++i)
-#pragma unroll
-    for (int d = 0; d < DT; ++d) gk[i][d] = gv[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < DT; ++d) gk[d] = gv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   for (int w0 = 0; w0 < a.words; w0 += kWindow) {
-    __syncthreads();                                             // the last window's list and tiles have been read
+    __syncthreads();                                             // the last window's list has been read
     if (tid < 64) {
       uint32_t m = tid < kWindow && w0 + tid < a.words ? inv[w0 + tid] : 0;
       int incl = __popc(m);
@@ -815,121 +821,92 @@ __global__ __launch_bounds__(256, OCC) void attend_dkv_kernel(AttnArgs a) {
       }
     }
     __syncthreads();
-    const int64_t total = (int64_t)n_list * a.rows;
-    const int nt = (int)((total + TR - 1) / TR);                 // total < 2^30
-    if (nt == 0) continue;
-    // threads 0 .. TR - 1: where row tid of tile t lies, and where its statistics lie (< 0: no row)
-    auto locate = [&](int t, longlong2 &where) -> int64_t {
-      const int64_t at = (int64_t)t * TR + tid;
-      where = longlong2{-1, -1};
-      if (at >= total) return -1;
-      const unsigned e = a.by_rows.div((unsigned)at), rr = (unsigned)at - e * (unsigned)a.rows;
-      const unsigned tk = a.by_g.div(rr);
-      const int token = list[e] * a.q_block + (int)tk;
-      const int head = hk * a.G + (int)(rr - tk * (unsigned)a.G);
-      if (token >= a.Nq) return -1;
-      where.x = ((int64_t)token * a.sq.n + (int64_t)head * a.sq.h) * (int64_t)sizeof(T);
-      where.y = ((int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h) * (int64_t)sizeof(T);
-      return ((int64_t)b * a.Hq + head) * a.Nq + token;
-    };
-    // statistics of a row, asked for a tile before they are needed (unconditional, clamped loads)
-    auto stat_load = [&](int64_t at, float &ls, float &de) {
-      ls = a.lse[at < 0 ? 0 : at];
-      de = a.delta[at < 0 ? 0 : at];
-    };
-    auto stat_store = [&](int64_t at, float ls, float de, int slot) {
-      if (tid < TR) {
-        lse2[slot * TR + tid] = at < 0 || ls == kNegInf ? kPosInf : ls * kLog2e - PScale<T>::bits;   // exp2(x - inf) = 0
-        delta[slot * TR + tid] = at < 0 ? 0.f : de;
-      }
-    };
-    auto issue = [&](int t) {
-      typedef Pieces<T, DP, TR> P;
-      char *qd = smem + (t & 1) * 2 * F::img, *dd = qd + F::img;
-      const longlong2 *tb = tab + (t & 1) * TR;
-      const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
-      longlong2 x[P::NU];
+    const unsigned total = (unsigned)n_list * (unsigned)a.rows;  // < 2^31
+    for (unsigned r0 = 0; r0 < total; r0 += kBatch) {
+      __syncthreads();                                           // the last batch's tables and tiles have been read
+      const int in_batch = (int)min((unsigned)kBatch, total - r0), nt = (in_batch + TR - 1) / TR;
 #pragma unroll
-      for (int u = 0; u < P::NU; ++u) x[u] = tb[P::whole ? P::row(u) : min(P::row(u), TR - 1)];
-#pragma unroll
-      for (int u = 0; u < P::NU; ++u)
-        if (P::any(u, wave)) {
-          const bool in = x[u].x >= 0 && P::chunk(u) < chunks;
-          dma16(in ? qb + (x[u].x + P::chunk(u) * 16) : zero, P::dst(qd, u, wave));
-          dma16(in ? db + (x[u].y + P::chunk(u) * 16) : zero, P::dst(dd, u, wave));
-        }
-    };
-    // rows of tiles 0 and 1, statistics of tile 0; from here on wave 0 locates rows two tiles ahead and fetches statistics one ahead
-    int64_t st_next = -1;
-    if (wave == 0) {
-      longlong2 w;
-      float ls, de;
-      const int64_t at = locate(0, w);
-      if (tid < TR) tab[tid] = w;
-      stat_load(at, ls, de);
-      stat_store(at, ls, de, 0);
-      st_next = locate(1, w);
-      if (tid < TR) tab[TR + tid] = w;
-    }
-    __syncthreads();
-    issue(0);
-    for (int t = 0; t < nt; ++t) {
-      tile_barrier();
-      if (t + 1 < nt) issue(t + 1);
-      float ls_n = 0.f, de_n = 0.f;
-      int64_t st_next2 = -1;
-      if (wave == 0) {
-        stat_load(st_next, ls_n, de_n);
-        longlong2 w;
-        st_next2 = locate(t + 2, w);
-        if (tid < TR) tab[(t & 1) * TR + tid] = w;               // tile t's rows are on their way already
-      }
-      const char *qrows = smem + (t & 1) * 2 * F::img, *drows = qrows + F::img;
-      f32x4 sc[2][NK], dp[2][NK];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int i = 0; i < NK; ++i) sc[u][i] = dp[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const frag qf = row_frag<T, DP>(qrows, wn * 32 + u * 16 + col, c * 32 + g * 8);
-          const frag df = row_frag<T, DP>(drows, wn * 32 + u * 16 + col, c * 32 + g * 8);
-#pragma unroll
-          for (int i = 0; i < NK; ++i) {
-            sc[u][i] = mma(qf, kf[i][c], sc[u][i]);
-            dp[u][i] = mma(df, vf[i][c], dp[u][i]);
+      for (int u = 0; u < kBatch / 256; ++u) {
+        const int r = u * 256 + tid;
+        uint2 where = {~0u, ~0u};
+        float ls = kPosInf, de = 0.f;                            // exp2(x - inf) = 0
+        if (r < in_batch) {
+          const unsigned e = a.by_rows.div(r0 + r), rr = r0 + r - e * (unsigned)a.rows;
+          const unsigned tk = a.by_g.div(rr);
+          const int token = list[e] * a.q_block + (int)tk;
+          const int head = hk * a.G + (int)(rr - tk * (unsigned)a.G);
+          if (token < a.Nq) {
+            constexpr int64_t u16 = 16 / sizeof(T);              // strides are multiples of 16 bytes
+            where.x = (unsigned)(((int64_t)token * a.sq.n + (int64_t)head * a.sq.h) / u16);
+            where.y = (unsigned)(((int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h) / u16);
+            const int64_t at = ((int64_t)b * a.Hq + head) * a.Nq + token;
+            const float x = a.lse[at];
+            if (x != kNegInf) ls = x * kLog2e - PScale<T>::bits;
+            de = a.delta[at];
           }
         }
+        tab[r] = where;
+        lse2[r] = ls;
+        delta[r] = de;
       }
-      frag pf[NK], gf[NK];
+      __syncthreads();
+      auto issue = [&](int t) {
+        char *qd = smem + (t % NB) * 2 * F::img, *dd = qd + F::img;
+        const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
+        uint2 x[P::NU];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const f32x4 ls = *reinterpret_cast<const f32x4 *>(lse2 + (t & 1) * TR + wn * 32 + u * 16 + g * 4);
-        const f32x4 de = *reinterpret_cast<const f32x4 *>(delta + (t & 1) * TR + wn * 32 + u * 16 + g * 4);
+        for (int u = 0; u < P::NU; ++u) x[u] = tab[t * TR + (P::whole ? P::row(u) : min(P::row(u), TR - 1))];
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+        for (int u = 0; u < P::NU; ++u)
+          if (P::any(u, wave)) {
+            const bool in = x[u].x != ~0u && P::chunk(u) < chunks;
+            dma16(in ? qb + ((uint64_t)x[u].x + P::chunk(u)) * 16 : zero, P::dst(qd, u, wave));
+            dma16(in ? db + ((uint64_t)x[u].y + P::chunk(u)) * 16 : zero, P::dst(dd, u, wave));
+          }
+      };
+#pragma unroll
+      for (int t = 0; t < NB - 1; ++t)
+        if (t < nt) issue(t);
+      for (int t = 0; t < nt; ++t) {
+        // tile t is there (the NB - 2 behind it may be on their way) and tile t - 1, whose place tile t + NB - 1 takes, has been read
+        if (NB == 4 && t + 2 < nt) tile_barrier<NB == 4 ? 2 * PER : 0>();
+        else if (NB == 4 && t + 1 < nt) tile_barrier<NB == 4 ? PER : 0>();
+        else tile_barrier<0>();
+        if (t + NB - 1 < nt) issue(t + NB - 1);
+        const char *qrows = smem + (t % NB) * 2 * F::img, *drows = qrows + F::img;
+        f32x4 sc[2], dp[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          sc[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            sc[u] = mma(row_frag<T, DP>(qrows, u * 16 + col, c * 32 + g * 8), kf[c], sc[u]);
+            dp[u] = mma(row_frag<T, DP>(drows, u * 16 + col, c * 32 + g * 8), vf[c], dp[u]);
+          }
+        }
+        frag pf, gf;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const f32x4 ls = *reinterpret_cast<const f32x4 *>(lse2 + t * TR + u * 16 + g * 4);
+          const f32x4 de = *reinterpret_cast<const f32x4 *>(delta + t * TR + u * 16 + g * 4);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = seen[i] ? __builtin_amdgcn_exp2f(fmaf(sc[u][i][e], a.c, -ls[e])) : 0.f;
-            pf[i][u * 4 + e] = (T)p;
-            gf[i][u * 4 + e] = (T)(p * (dp[u][i][e] - de[e]) * (a.scale * PScale<T>::inv));
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][e], a.c, -ls[e]));
+            float ds = p * (dp[u][e] - de[e]);
+            if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= each;
+            pf[u * 4 + e] = (T)p;
+            gf[u * 4 + e] = (T)ds;
           }
-      }
+        }
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const frag df = col_frag<T, DP>(drows, wn * 32, d * 16, lane);
-        const frag qf = col_frag<T, DP>(qrows, wn * 32, d * 16, lane);
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          gv[i][d] = mma(df, pf[i], gv[i][d]);
-          gk[i][d] = mma(qf, gf[i], gk[i][d]);
+        for (int d = 0; d < DT; ++d) {
+          gv[d] = mma(col_frag<T, DP>(drows, 0, d * 16, lane), pf, gv[d]);
+          gk[d] = mma(col_frag<T, DP>(qrows, 0, d * 16, lane), gf, gk[d]);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
-      if (wave == 0) stat_store(st_next, ls_n, de_n, (t + 1) & 1);
-      st_next = st_next2;
     }
   }
+  // out through LDS, for whole rows
   float *jo = reinterpret_cast<float *>(smem);
   const int per = a.D / 4;
 #pragma unroll
@@ -937,22 +914,16 @@ __global__ __launch_bounds__(256, OCC) void attend_dkv_kernel(AttnArgs a) {
     T *out = reinterpret_cast<T *>(which ? a.dv : a.dk);
     if (out == nullptr) continue;
     const Str st = which ? a.sdv : a.sdk;
-    const float f = which ? PScale<T>::inv : 1.f;
+    const float f = which ? PScale<T>::inv : k_scale;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WN; ++w) {
-      if (wn == w) {
+    for (int d = 0; d < DT; ++d) {
+      f32x4 x = which ? gv[d] : gk[d];
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            f32x4 *p = reinterpret_cast<f32x4 *>(jo + ((wm * NK + i) * 16 + col) * (DP + 4) + d * 16 + g * 4);
-            const f32x4 x = (which ? gv[i][d] : gk[i][d]) * f;
-            *p = w == 0 ? x : *p + x;
-          }
-      }
-      __syncthreads();
+      for (int e = 0; e < 4; ++e) x[e] = seen ? x[e] * f : 0.f;
+      *reinterpret_cast<f32x4 *>(jo + (wave * 16 + col) * (DP + 4) + d * 16 + g * 4) = x;
     }
+    __syncthreads();
     for (int id = tid; id < M * per; id += 256) {
       const int r = id / per, ch = (id - r * per) * 4, key = kt * M + r;
       if (key >= a.Nk) continue;
@@ -1004,7 +975,7 @@ template <typename T, int DP> static int launch_dq(AttnArgs a, hipStream_t s) {
 template <typename T, int DP> static int launch_dkv(const AttnArgs &a, hipStream_t s) {
   const char *what = "block_attention backward (keys)";
   const int64_t blocks = cdiv(a.Nk, 64) * a.B * a.Hkv;
-  return launch(attend_dkv_kernel<T, DP, 1, 4, 1, 2>, DkvTile<T, DP, 1, 4, 1>::bytes, blocks, a, s, what);
+  return launch(attend_dkv_kernel<T, DP>, DkvTile<T, DP>::bytes, blocks, a, s, what);
 }
 
 // head sizes are padded to a multiple of 32 in LDS and registers
@@ -1077,6 +1048,11 @@ static bool rows16(const void *p, const Str &s, int dtype) {
 }
 // the rows of a block are addressed by 32-bit byte offsets from its first
 static bool near_rows(const Str &s) { return s.n >= 0 && s.n < (1LL << 22); }
+// the query rows of a batch item by 32-bit counts of 16 bytes
+static bool near_batch(const Str &s, const AttnArgs &a, int dtype) {
+  const int64_t last = (int64_t)(a.Nq - 1) * s.n + (int64_t)(a.Hq - 1) * s.h;
+  return s.n >= 0 && s.h >= 0 && s.n < (1LL << 31) && s.h < (1LL << 31) && last / (dtype == TCL_DT_F32 ? 4 : 8) < (1LL << 32) - 64;
+}
 
 }  // namespace tcl
 
@@ -1151,6 +1127,7 @@ extern "C" int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64
               (!g_q || rows16(g_q, a.sdq, dtype)) && (!g_k || rows16(g_k, a.sdk, dtype)) && (!g_v || rows16(g_v, a.sdv, dtype)), TCL_ERR_ARG,
               "block_attention backward: rows must start on 16 bytes");
   TCL_REQUIRE(near_rows(a.sk) && near_rows(a.sv), TCL_ERR_UNSUPPORTED, "block_attention backward: keys lie more than 2^22 elements apart");
+  TCL_REQUIRE(near_batch(a.sq, a, dtype) && near_batch(a.sdo, a, dtype), TCL_ERR_UNSUPPORTED, "block_attention backward: the query rows of a batch item span more than 64 GB");
   const size_t need = tcl_block_attention_bwd_workspace_bytes(B, Nq, Nk, Hq, Hkv, D, top_k, block, q_block);
   TCL_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, TCL_ERR_WORKSPACE, "block_attention backward: workspace of %zu bytes needed", need);
   a.delta = (float *)workspace;
