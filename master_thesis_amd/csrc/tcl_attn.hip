@@ -353,18 +353,29 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     if (t + 1 < nt) issue(t + 1, nxt);
     seg_load(t + 2, raw);
     const char *krows = smem + (t & 1) * 2 * F::img, *vrows = krows + F::img;
+    // all fragments of a product are asked for before its first step, those of the second product before the softmax: an LDS read
+    // takes longer than a product, and there are only a few waves to hide it behind
+    frag kf[2][KC];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kf[u][c] = row_frag<T, DP>(krows, wn * 32 + u * 16 + col, c * 32 + g * 8);
+    __builtin_amdgcn_sched_barrier(0);
     f32x4 sc[2][NQ];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
       for (int i = 0; i < NQ; ++i) sc[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const frag kf = row_frag<T, DP>(krows, wn * 32 + u * 16 + col, c * 32 + g * 8);
+      for (int c = 0; c < KC; ++c)
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) sc[u][i] = mma(kf, qf[i][c], sc[u][i]);
-      }
+        for (int i = 0; i < NQ; ++i) sc[u][i] = mma(kf[u][c], qf[i][c], sc[u][i]);
     }
+    constexpr int AH = sizeof(T) == 2 ? DT : DT / 2;             // fp32 fragments are twice as large, and their products 16 times as long
+    frag vf[AH];
+#pragma unroll
+    for (int d = 0; d < AH; ++d) vf[d] = col_frag<T, DP>(vrows, wn * 32, d * 16, lane);
+    __builtin_amdgcn_sched_barrier(0);
     const uint64_t mask = cur[wn * 32 / 64 % NS].mask;
     if (mask != ~0ull) {
       const unsigned seen = (unsigned)(mask >> ((TK < 64 ? (t * TK) & 63 : wn * 32 & 63) + g * 4));
@@ -408,9 +419,9 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const frag vf = col_frag<T, DP>(vrows, wn * 32, d * 16, lane);
+      const frag v = d < AH ? vf[d % AH] : col_frag<T, DP>(vrows, wn * 32, d * 16, lane);
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) o[i][d] = mma(vf, pf[i], o[i][d]);
+      for (int i = 0; i < NQ; ++i) o[i][d] = mma(v, pf[i], o[i][d]);
     }
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
 #pragma unroll
@@ -668,21 +679,35 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     raw = keys.load((t + 2) * TK / 64);
     const char *krows = smem + (t & 1) * 2 * F::img, *vrows = krows + F::img;
     f32x4 sc[2][NQ], dp[2][NQ];
+    frag kf[KC], vf[KC];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      kf[c] = row_frag<T, DP>(krows, wn * 32 + col, c * 32 + g * 8);
+      vf[c] = row_frag<T, DP>(vrows, wn * 32 + col, c * 32 + g * 8);
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) sc[u][i] = dp[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        const frag kf = row_frag<T, DP>(krows, wn * 32 + u * 16 + col, c * 32 + g * 8);
-        const frag vf = row_frag<T, DP>(vrows, wn * 32 + u * 16 + col, c * 32 + g * 8);
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
-          sc[u][i] = mma(kf, qf[i][c], sc[u][i]);
-          dp[u][i] = mma(vf, df[i][c], dp[u][i]);
+          sc[u][i] = mma(kf[c], qf[i][c], sc[u][i]);
+          dp[u][i] = mma(vf[c], df[i][c], dp[u][i]);
+        }
+        if (u == 0) {                                            // the other 16 keys' fragments take the place of the used ones
+          kf[c] = row_frag<T, DP>(krows, wn * 32 + 16 + col, c * 32 + g * 8);
+          vf[c] = row_frag<T, DP>(vrows, wn * 32 + 16 + col, c * 32 + g * 8);
         }
       }
     }
+    constexpr int AH = DT / 2;
+    frag ka[AH];
+#pragma unroll
+    for (int d = 0; d < AH; ++d) ka[d] = col_frag<T, DP>(krows, wn * 32, d * 16, lane);
+    __builtin_amdgcn_sched_barrier(0);
     frag gf[NQ];
     const unsigned seen = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32 + g * 4));
 #pragma unroll
@@ -699,9 +724,10 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
         }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const frag kf = col_frag<T, DP>(krows, wn * 32, d * 16, lane);
+      const frag k = ka[d % AH];
+      if (d < AH) ka[d % AH] = col_frag<T, DP>(krows, wn * 32, (d + AH) * 16, lane);
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) o[i][d] = mma(kf, gf[i], o[i][d]);
+      for (int i = 0; i < NQ; ++i) o[i][d] = mma(k, gf[i], o[i][d]);
     }
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
     cur = nxt;
@@ -874,34 +900,59 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
         else tile_barrier<0>();
         if (t + NB - 1 < nt) issue(t + NB - 1);
         const char *qrows = smem + (t % NB) * 2 * F::img, *drows = qrows + F::img;
+        frag qf[2][KC], df[2][KC];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            qf[u][c] = row_frag<T, DP>(qrows, u * 16 + col, c * 32 + g * 8);
+            df[u][c] = row_frag<T, DP>(drows, u * 16 + col, c * 32 + g * 8);
+          }
+        f32x4 ls[2], de[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          ls[u] = *reinterpret_cast<const f32x4 *>(lse2 + t * TR + u * 16 + g * 4);
+          de[u] = *reinterpret_cast<const f32x4 *>(delta + t * TR + u * 16 + g * 4);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         f32x4 sc[2], dp[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           sc[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < KC; ++c) {
-            sc[u] = mma(row_frag<T, DP>(qrows, u * 16 + col, c * 32 + g * 8), kf[c], sc[u]);
-            dp[u] = mma(row_frag<T, DP>(drows, u * 16 + col, c * 32 + g * 8), vf[c], dp[u]);
+            sc[u] = mma(qf[u][c], kf[c], sc[u]);
+            dp[u] = mma(df[u][c], vf[c], dp[u]);
           }
         }
+        constexpr int AH = DT / 2;
+        frag da[AH], qa[AH];
+#pragma unroll
+        for (int d = 0; d < AH; ++d) {
+          da[d] = col_frag<T, DP>(drows, 0, d * 16, lane);
+          qa[d] = col_frag<T, DP>(qrows, 0, d * 16, lane);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         frag pf, gf;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const f32x4 ls = *reinterpret_cast<const f32x4 *>(lse2 + t * TR + u * 16 + g * 4);
-          const f32x4 de = *reinterpret_cast<const f32x4 *>(delta + t * TR + u * 16 + g * 4);
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][e], a.c, -ls[e]));
-            float ds = p * (dp[u][e] - de[e]);
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][e], a.c, -ls[u][e]));
+            float ds = p * (dp[u][e] - de[u][e]);
             if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= each;
             pf[u * 4 + e] = (T)p;
             gf[u * 4 + e] = (T)ds;
           }
-        }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          gv[d] = mma(col_frag<T, DP>(drows, 0, d * 16, lane), pf, gv[d]);
-          gk[d] = mma(col_frag<T, DP>(qrows, 0, d * 16, lane), gf, gk[d]);
+          const frag x = da[d % AH], y = qa[d % AH];
+          if (d < AH) {
+            da[d % AH] = col_frag<T, DP>(drows, 0, (d + AH) * 16, lane);
+            qa[d % AH] = col_frag<T, DP>(qrows, 0, (d + AH) * 16, lane);
+          }
+          gv[d] = mma(x, pf, gv[d]);
+          gk[d] = mma(y, gf, gk[d]);
         }
       }
     }
