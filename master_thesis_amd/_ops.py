@@ -750,7 +750,7 @@ def select_blocks(q, means, counts, top_k, q_block=64):
     mc = _side("means", means, dev, (torch.float32,), (b, hk, nb, d))
     cc = _side("counts", counts, dev, (torch.int32,), (b, nb))
     s = -(-n // q_block)
-    qc = q.detach() if q.stride(3) == 1 else q.detach().contiguous()
+    qc = _rows16(q.detach())
     blocks = torch.empty((b, hk, s, top_k), dtype=torch.int32, device=dev)
     ws = _workspace(_lib.lib().tcl_select_blocks_workspace_bytes(b, hk, s, nb, d), dev)
     with _on(dev):

@@ -61,6 +61,9 @@ struct AttnArgs {
   float *lse;                      // (B, Hq, Nq), natural logarithm
   float *delta;                    // (B, Hq, Nq)
   uint32_t *inv;                   // (B, Hkv, nb, words): which groups chose the block
+  uint32_t *chosen;                // (B, Hkv, nb): by how many entries, directly behind inv
+  int32_t *order;                  // (B, Hkv, nb): the blocks, often chosen ones first
+  int64_t plan_words;              // of inv and chosen
   float *part;                     // partial results of split work
   Str sq, sk, sv, so, sdo, sdq, sdk, sdv;
   int B, Nq, Nk, Hq, Hkv, G, D, S, top, nb, lb, q_block, rows, chunks, splits, words, cap;
@@ -549,7 +552,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
 template <typename T> struct PScale { static constexpr float bits = 0.f, inv = 1.f; };
 template <> struct PScale<_Float16> { static constexpr float bits = 10.f, inv = 0x1p-10f; };
 
-// delta of every row: 16 lanes per row, 8 channels each
+// delta of every row: 16 lanes per row, 8 channels each; and the plan of the key / value gradients (inv, chosen) is cleared
 template <typename T>
 __global__ __launch_bounds__(256) void attend_delta_kernel(AttnArgs a) {
   const int64_t id = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
@@ -570,13 +573,10 @@ __global__ __launch_bounds__(256) void attend_delta_kernel(AttnArgs a) {
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if (live && ch == 0) a.delta[((int64_t)b * a.Hq + head) * a.Nq + token] = sum;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.plan_words; i += (int64_t)gridDim.x * 256) a.inv[i] = 0;
 }
 
-// which groups chose each block: one bit per (block, group)
-__global__ __launch_bounds__(256) void attend_clear_kernel(uint32_t *p, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) p[i] = 0;
-}
+// which groups chose each block: one bit per (block, group), and (for the order of the work only) how many entries named it
 __global__ __launch_bounds__(256) void attend_invert_kernel(AttnArgs a) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (int64_t)a.B * a.Hkv * a.S * a.top) return;
@@ -584,7 +584,41 @@ __global__ __launch_bounds__(256) void attend_invert_kernel(AttnArgs a) {
   const int64_t row = i / a.top;
   const int s = (int)(row % a.S);
   const int64_t bh = row / a.S;
-  if (j >= 0 && j < a.nb) atomicOr(&a.inv[(bh * a.nb + j) * a.words + (s >> 5)], 1u << (s & 31));
+  if (j < 0 || j >= a.nb) return;
+  atomicOr(&a.inv[(bh * a.nb + j) * a.words + (s >> 5)], 1u << (s & 31));
+  atomicAdd(&a.chosen[bh * a.nb + j], 1u);
+}
+// The blocks of one (item, key head), often chosen ones first: the work per block differs by a factor of four and more, and a long one
+// that starts last keeps the GPU waiting (517 -> 445 us for the training step of 63,600 keys).  Counting sort into 256 classes; the
+// order within a class does not matter.  One workgroup per (item, key head).
+__global__ __launch_bounds__(1024) void attend_order_kernel(AttnArgs a) {
+  __shared__ unsigned start[256], most;
+  const uint32_t *cnt = a.chosen + (int64_t)blockIdx.x * a.nb;
+  int32_t *order = a.order + (int64_t)blockIdx.x * a.nb;
+  if (threadIdx.x < 256) start[threadIdx.x] = 0;
+  if (threadIdx.x == 0) most = 0;
+  __syncthreads();
+  for (int j = threadIdx.x; j < a.nb; j += 1024) atomicMax(&most, cnt[j]);
+  __syncthreads();
+  const unsigned top = most + 1;
+  auto cls = [&](unsigned c) { return 255 - (unsigned)((uint64_t)c * 256 / top); };
+  for (int j = threadIdx.x; j < a.nb; j += 1024) atomicAdd(&start[cls(cnt[j])], 1u);
+  __syncthreads();
+  if (threadIdx.x < 64) {                                        // exclusive prefix sums, 4 classes a lane
+    unsigned v[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = sum; sum += start[threadIdx.x * 4 + i]; }
+    unsigned incl = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned t = __shfl_up(incl, o, 64);
+      if ((int)threadIdx.x >= o) incl += t;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) start[threadIdx.x * 4 + i] = incl - sum + v[i];
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < a.nb; j += 1024) order[atomicAdd(&start[cls(cnt[j])], 1u)] = j;
 }
 
 template <typename T, int DP, int NQ, int WM, int WN> struct DqTile {
@@ -725,7 +759,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const frag k = ka[d % AH];
-      if (d < AH) ka[d % AH] = col_frag<T, DP>(krows, wn * 32, (d + AH) * 16, lane);
+      if (d + AH < DT) ka[d % AH] = col_frag<T, DP>(krows, wn * 32, (d + AH) * 16, lane);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) o[i][d] = mma(k, gf[i], o[i][d]);
     }
@@ -775,8 +809,7 @@ constexpr int kBatch = 512;    // rows located at a time
 template <typename T, int DP> struct DkvTile {
   static constexpr int M = 64, TR = 32, NB = sizeof(T) == 4 && DP > 64 ? 2 : 4;
   static constexpr size_t img = (size_t)TR * Img<T, DP>::RB, tiles = NB * 2 * img;     // Q and dout
-  static constexpr size_t join = (size_t)M * (DP + 4) * 4;
-  static constexpr size_t body = tiles > join ? tiles : join;
+  static constexpr size_t body = tiles;
   // behind the tiles: where a row lies in q and dout (in 16 bytes), lse and delta, the list of groups
   static constexpr size_t bytes = body + kBatch * 16 + 32 * kWindow * 4;
 };
@@ -793,32 +826,32 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
   __shared__ int n_list;
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % 16, g = lane / 16;
-  const int tiles_of = (a.Nk + M - 1) / M;
+  const int per_block = 1 << (a.lb - 6), tiles_of = a.nb * per_block;
   unsigned item = xcd_remap(blockIdx.x, gridDim.x);
-  const int kt = (int)(item % tiles_of);
-  const int bh = (int)(item / tiles_of), hk = bh % a.Hkv, b = bh / a.Hkv;
-  const uint32_t *inv = a.inv + ((int64_t)bh * a.nb + (((int64_t)kt * M) >> a.lb)) * a.words;
+  const int bh = (int)(item / tiles_of), hk = bh % a.Hkv, b = bh / a.Hkv, at_ = (int)(item % tiles_of);
+  const int block = __builtin_amdgcn_readfirstlane(a.order[(int64_t)bh * a.nb + at_ / per_block]), kt = block * per_block + at_ % per_block;
+  if (kt * M >= a.Nk) return;                                    // the second half of a block that ends in its first
+  const uint32_t *inv = a.inv + ((int64_t)bh * a.nb + block) * a.words;
 
   // this lane's key.  A hidden key's row is taken as zeros: whatever its probabilities come to stays in its own column, which is
-  // not written.
+  // not written.  Its loads are unconditional and not waited for before the first rows are on their way.
+  const uint32_t first_word = tid < kWindow && tid < a.words ? inv[tid] : 0;
   frag kf[KC], vf[KC];
   const int key = kt * M + wave * 16 + col;
-  const bool seen = key < a.Nk && (!a.vis || a.vis[(int64_t)b * a.Nk + key] > 0.5f);
+  const float see = a.vis ? a.vis[(int64_t)b * a.Nk + min(key, a.Nk - 1)] : 1.f;
   {
-    const T *p = reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)key * a.sk.n + (int64_t)hk * a.sk.h;
-    const T *q = reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)key * a.sv.n + (int64_t)hk * a.sv.h;
+    const int row = min(key, a.Nk - 1);
+    const T *p = reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)row * a.sk.n + (int64_t)hk * a.sk.h;
+    const T *q = reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)row * a.sv.n + (int64_t)hk * a.sv.h;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      const int ch = c * 32 + g * 8;
-      frag t = {}, u = {};
-      if (seen && ch < a.D) {
-        t = *reinterpret_cast<const frag *>(p + ch);
-        u = *reinterpret_cast<const frag *>(q + ch);
-      }
-      kf[c] = t;
-      vf[c] = u;
+      const int ch = min(c * 32 + g * 8, a.D - 8);
+      kf[c] = *reinterpret_cast<const frag *>(p + ch);
+      vf[c] = *reinterpret_cast<const frag *>(q + ch);
     }
   }
+  bool fresh = true;                                             // kf, vf as loaded
+  bool seen = false;
   const char *qb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sq.b);
   const char *db = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.dout) + (int64_t)b * a.sdo.b);
   const int chunks = a.D / P::I::VE;
@@ -832,7 +865,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
   for (int w0 = 0; w0 < a.words; w0 += kWindow) {
     __syncthreads();                                             // the last window's list has been read
     if (tid < 64) {
-      uint32_t m = tid < kWindow && w0 + tid < a.words ? inv[w0 + tid] : 0;
+      uint32_t m = w0 == 0 ? first_word : tid < kWindow && w0 + tid < a.words ? inv[w0 + tid] : 0;
       int incl = __popc(m);
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -876,12 +909,14 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
         delta[r] = de;
       }
       __syncthreads();
+      uint2 x[P::NU];                                            // where the rows of the next tile lie, read a tile before they are asked for
+      auto locate = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < P::NU; ++u) x[u] = tab[min(t, kBatch / TR - 1) * TR + (P::whole ? P::row(u) : min(P::row(u), TR - 1))];
+      };
       auto issue = [&](int t) {
         char *qd = smem + (t % NB) * 2 * F::img, *dd = qd + F::img;
         const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
-        uint2 x[P::NU];
-#pragma unroll
-        for (int u = 0; u < P::NU; ++u) x[u] = tab[t * TR + (P::whole ? P::row(u) : min(P::row(u), TR - 1))];
 #pragma unroll
         for (int u = 0; u < P::NU; ++u)
           if (P::any(u, wave)) {
@@ -892,40 +927,60 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
       };
 #pragma unroll
       for (int t = 0; t < NB - 1; ++t)
-        if (t < nt) issue(t);
+        if (t < nt) {
+          locate(t);
+          issue(t);
+        }
+      locate(NB - 1);
+      if (fresh) {
+        fresh = false;
+        seen = key < a.Nk && see > 0.5f;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool in = seen && c * 32 + g * 8 < a.D;
+            kf[c][e] = in ? kf[c][e] : (T)0.f;
+            vf[c][e] = in ? vf[c][e] : (T)0.f;
+          }
+      }
       for (int t = 0; t < nt; ++t) {
         // tile t is there (the NB - 2 behind it may be on their way) and tile t - 1, whose place tile t + NB - 1 takes, has been read
         if (NB == 4 && t + 2 < nt) tile_barrier<NB == 4 ? 2 * PER : 0>();
         else if (NB == 4 && t + 1 < nt) tile_barrier<NB == 4 ? PER : 0>();
         else tile_barrier<0>();
         if (t + NB - 1 < nt) issue(t + NB - 1);
+        locate(t + NB);
         const char *qrows = smem + (t % NB) * 2 * F::img, *drows = qrows + F::img;
+        constexpr bool ahead = sizeof(T) == 2 || DP <= 64;        // all fragments before the first product (fp32: registers for 64 channels)
         frag qf[2][KC], df[2][KC];
+        if constexpr (ahead) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int c = 0; c < KC; ++c) {
-            qf[u][c] = row_frag<T, DP>(qrows, u * 16 + col, c * 32 + g * 8);
-            df[u][c] = row_frag<T, DP>(drows, u * 16 + col, c * 32 + g * 8);
-          }
+            for (int c = 0; c < KC; ++c) {
+              qf[u][c] = row_frag<T, DP>(qrows, u * 16 + col, c * 32 + g * 8);
+              df[u][c] = row_frag<T, DP>(drows, u * 16 + col, c * 32 + g * 8);
+            }
+        }
         f32x4 ls[2], de[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           ls[u] = *reinterpret_cast<const f32x4 *>(lse2 + t * TR + u * 16 + g * 4);
           de[u] = *reinterpret_cast<const f32x4 *>(delta + t * TR + u * 16 + g * 4);
         }
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (ahead) __builtin_amdgcn_sched_barrier(0);
         f32x4 sc[2], dp[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           sc[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < KC; ++c) {
-            sc[u] = mma(qf[u][c], kf[c], sc[u]);
-            dp[u] = mma(df[u][c], vf[c], dp[u]);
+            sc[u] = mma(ahead ? qf[u][c] : row_frag<T, DP>(qrows, u * 16 + col, c * 32 + g * 8), kf[c], sc[u]);
+            dp[u] = mma(ahead ? df[u][c] : row_frag<T, DP>(drows, u * 16 + col, c * 32 + g * 8), vf[c], dp[u]);
           }
         }
-        constexpr int AH = DT / 2;
+        constexpr int AH = ahead ? DT / 2 : 1;
         frag da[AH], qa[AH];
 #pragma unroll
         for (int d = 0; d < AH; ++d) {
@@ -947,7 +1002,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const frag x = da[d % AH], y = qa[d % AH];
-          if (d < AH) {
+          if (d + AH < DT) {
             da[d % AH] = col_frag<T, DP>(drows, 0, (d + AH) * 16, lane);
             qa[d % AH] = col_frag<T, DP>(qrows, 0, (d + AH) * 16, lane);
           }
@@ -957,32 +1012,22 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
       }
     }
   }
-  // out through LDS, for whole rows
-  float *jo = reinterpret_cast<float *>(smem);
-  const int per = a.D / 4;
+  // a lane holds 4 channels of its key per 16: the 4 quarters together write 32 (fp32: 64) bytes of 16 rows at a time
+  if (key >= a.Nk) return;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     T *out = reinterpret_cast<T *>(which ? a.dv : a.dk);
     if (out == nullptr) continue;
     const Str st = which ? a.sdv : a.sdk;
     const float f = which ? PScale<T>::inv : k_scale;
-    __syncthreads();
+    T *row = out + (int64_t)b * st.b + (int64_t)key * st.n + (int64_t)hk * st.h + g * 4;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      f32x4 x = which ? gv[d] : gk[d];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = seen ? x[e] * f : 0.f;
-      *reinterpret_cast<f32x4 *>(jo + (wave * 16 + col) * (DP + 4) + d * 16 + g * 4) = x;
-    }
-    __syncthreads();
-    for (int id = tid; id < M * per; id += 256) {
-      const int r = id / per, ch = (id - r * per) * 4, key = kt * M + r;
-      if (key >= a.Nk) continue;
-      const f32x4 x = *reinterpret_cast<const f32x4 *>(jo + r * (DP + 4) + ch);
+      if (d * 16 + g * 4 >= a.D) continue;
       typename Vec4<T>::type y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
-      *reinterpret_cast<typename Vec4<T>::type *>(out + (int64_t)b * st.b + (int64_t)key * st.n + (int64_t)hk * st.h + ch) = y;
+      for (int e = 0; e < 4; ++e) y[e] = (T)(seen ? (which ? gv[d][e] : gk[d][e]) * f : 0.f);
+      *reinterpret_cast<typename Vec4<T>::type *>(row + d * 16) = y;
     }
   }
 }
@@ -1025,7 +1070,7 @@ template <typename T, int DP> static int launch_dq(AttnArgs a, hipStream_t s) {
 }
 template <typename T, int DP> static int launch_dkv(const AttnArgs &a, hipStream_t s) {
   const char *what = "block_attention backward (keys)";
-  const int64_t blocks = cdiv(a.Nk, 64) * a.B * a.Hkv;
+  const int64_t blocks = ((int64_t)a.nb << (a.lb - 6)) * a.B * a.Hkv;
   return launch(attend_dkv_kernel<T, DP>, DkvTile<T, DP>::bytes, blocks, a, s, what);
 }
 
@@ -1155,7 +1200,7 @@ extern "C" size_t tcl_block_attention_bwd_workspace_bytes(int64_t B, int64_t Nq,
                                                           int64_t q_block) {
   AttnArgs a{};
   if (attn_setup(a, B, Nq, Nk, Hq, Hkv, D, top_k, block, q_block, 1.0, TCL_DT_F32) != TCL_OK) return 256;
-  return round_up((size_t)B * Hq * Nq * 4, 256) + round_up((size_t)B * Hkv * a.nb * a.words * 4, 256) + 256;
+  return round_up((size_t)B * Hq * Nq * 4, 256) + round_up((size_t)B * Hkv * a.nb * (a.words + 1) * 4, 256) + round_up((size_t)B * Hkv * a.nb * 4, 256) + 256;
 }
 
 extern "C" int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64_t g_sn, int64_t g_sh, const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
@@ -1184,8 +1229,11 @@ extern "C" int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64
   a.delta = (float *)workspace;
   a.inv = (uint32_t *)((char *)workspace + round_up((size_t)B * Hq * Nq * 4, 256));
   const hipStream_t s = (hipStream_t)stream;
-  const int64_t dblocks = cdiv(B * Nq * Hq, 16), inv_n = (int64_t)B * Hkv * a.nb * a.words, sel_n = (int64_t)B * Hkv * a.S * a.top;
-  TCL_REQUIRE(dblocks < (1LL << 31) && cdiv(inv_n, 256) < (1LL << 31) && cdiv(sel_n, 256) < (1LL << 31), TCL_ERR_SHAPE, "block_attention backward: too many rows for one call");
+  const int64_t bh = B * Hkv, dblocks = cdiv(B * Nq * Hq, 16), sel_n = bh * a.S * a.top;
+  a.plan_words = g_k || g_v ? bh * a.nb * (a.words + 1) : 0;
+  a.chosen = a.inv + bh * a.nb * a.words;
+  a.order = (int32_t *)((char *)a.inv + round_up((size_t)bh * a.nb * (a.words + 1) * 4, 256));
+  TCL_REQUIRE(dblocks < (1LL << 31) && cdiv(sel_n, 256) < (1LL << 31) && bh < (1LL << 31), TCL_ERR_SHAPE, "block_attention backward: too many rows for one call");
   if (dtype == TCL_DT_F32) hipLaunchKernelGGL((attend_delta_kernel<float>), dim3((unsigned)dblocks), dim3(256), 0, s, a);
   else if (dtype == TCL_DT_BF16) hipLaunchKernelGGL((attend_delta_kernel<__bf16>), dim3((unsigned)dblocks), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((attend_delta_kernel<_Float16>), dim3((unsigned)dblocks), dim3(256), 0, s, a);
@@ -1194,7 +1242,7 @@ extern "C" int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64
     if (r != TCL_OK) return r;
   }
   if (!g_k && !g_v) return check_launch("block_attention backward");
-  hipLaunchKernelGGL(attend_clear_kernel, dim3((unsigned)cdiv(inv_n, 256)), dim3(256), 0, s, a.inv, inv_n);
   hipLaunchKernelGGL(attend_invert_kernel, dim3((unsigned)cdiv(sel_n, 256)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(attend_order_kernel, dim3((unsigned)bh), dim3(1024), 0, s, a);
   return dtype == TCL_DT_F32 ? dkv_by_dim<float>(a, s) : dtype == TCL_DT_BF16 ? dkv_by_dim<__bf16>(a, s) : dkv_by_dim<_Float16>(a, s);
 }

@@ -96,23 +96,51 @@ struct SelectArgs {
   uint64_t *keys;      // (B, Hkv, S, nb)
   int64_t sb, sn, sh;
   int B, N, H, Hkv, G, D, nb, top, q_block, S;
+  FastDiv by_g;
 };
 
-// sum of the queries of one group, 64 bits.  One wave per (item, key head, group); a lane owns channels lane and lane + 64.
+// sum of the queries of one group, 64 bits.  One wave per (item, key head, group): a row takes D / VE lanes, the wave's 64 / (D / VE) row
+// sets are joined through LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void select_pool_kernel(SelectArgs a) {
+  constexpr int VE = 4;
+  typedef typename SelVec<T, VE>::type vec;
+  __shared__ double part[4][64 * VE];
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
-  if (id >= (int64_t)a.B * a.Hkv * a.S) return;
-  const int s = (int)(id % a.S);
-  const int64_t bh = id / a.S;
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.S, id = (int64_t)blockIdx.x * 4 + wave;
+  const bool live = id < rows;
+  const int64_t w = live ? id : rows - 1;
+  const int s = (int)(w % a.S);
+  const int64_t bh = w / a.S;
   const int hk = (int)(bh % a.Hkv), b = (int)(bh / a.Hkv);
   const T *q = reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sb + (int64_t)hk * a.G * a.sh;
-  const int n0 = (int)((int64_t)s * a.q_block), n1 = (int)min((int64_t)a.N, (int64_t)n0 + a.q_block);
+  const int n0 = (int)((int64_t)s * a.q_block), n = (int)(min((int64_t)a.N, (int64_t)n0 + a.q_block) - n0) * a.G;   // (token, head) rows
+  const int lr = a.D / VE, rp = 64 / lr, rg = lane / lr, ch = (lane - rg * lr) * VE;
+  const bool in = rg < rp;
+  double acc[VE] = {};
+  for (int r0 = 0; r0 < n; r0 += 4 * rp) {
+    vec t[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = min(r0 + u * rp + (in ? rg : 0), n - 1), tk = (int)a.by_g.div((unsigned)r);
+      t[u] = *reinterpret_cast<const vec *>(q + (int64_t)(n0 + tk) * a.sn + (int64_t)(r - tk * a.G) * a.sh + ch);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool use = in && r0 + u * rp + rg < n;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[e] += use ? (double)(float)t[u][e] : 0.0;
+    }
+  }
+  if (in) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) part[wave][rg * a.D + ch + e] = acc[e];
+  }
+  __syncthreads();
+  if (!live) return;
   for (int c = lane; c < a.D; c += 64) {
     double sum = 0.0;
-    for (int n = n0; n < n1; ++n)
-      for (int g = 0; g < a.G; ++g) sum += (double)(float)q[(int64_t)n * a.sn + (int64_t)g * a.sh + c];
+    for (int g = 0; g < rp; ++g) sum += part[wave][g * a.D + c];
     a.pooled[id * a.D + c] = sum;
   }
 }
@@ -125,39 +153,175 @@ __device__ __forceinline__ uint64_t score_key(double s, bool can) {
   return can && s > -__builtin_inf() ? m : 0ull;
 }
 
-// scores of 16 groups x 16 blocks per wave with v_mfma_f64_16x16x4: lane l holds row (column) l % 16 of both operands and, in a
+// scores of 16 groups x 64 blocks per wave with v_mfma_f64_16x16x4: lane l holds row (column) l % 16 of both operands and, in a
 // slice of 16 channels, channels 4 (l / 16) .. + 3, one of them per instruction.
+constexpr int kScoreTiles = 4;
 __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   const int r = lane % 16, g = lane / 16;
   const int64_t bh = blockIdx.z;
-  const int s0 = blockIdx.y * 16, j0 = (blockIdx.x * 4 + wave) * 16;
+  const int s0 = blockIdx.y * 16, j0 = (blockIdx.x * 4 + wave) * 16 * kScoreTiles;
   if (j0 >= a.nb) return;
   const int b = (int)(bh / a.Hkv);
-  const int s = min(s0 + r, a.S - 1), j = min(j0 + r, a.nb - 1);
+  const int s = min(s0 + r, a.S - 1);
   const double *qp = a.pooled + (bh * a.S + s) * a.D;
-  const float *mp = a.means + (bh * a.nb + j) * a.D;
-  f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+  f64x4 acc[kScoreTiles] = {};
   for (int c0 = 0; c0 < a.D; c0 += 16) {
     const int c = c0 + 4 * g;
     const bool in = c < a.D;                                    // D is a multiple of 8
     double qv[4];
-    float mv[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      qv[e] = in ? qp[c + e] : 0.0;
-      mv[e] = in ? mp[c + e] : 0.f;
+    for (int e = 0; e < 4; ++e) qv[e] = in ? qp[c + e] : 0.0;
+#pragma unroll
+    for (int t = 0; t < kScoreTiles; ++t) {
+      const float *mp = a.means + (bh * a.nb + min(j0 + t * 16 + r, a.nb - 1)) * a.D;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t] = __builtin_amdgcn_mfma_f64_16x16x4f64(qv[e], in ? (double)mp[c + e] : 0.0, acc[t], 0, 0, 0);
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(qv[e], (double)mv[e], acc, 0, 0, 0);
   }
   // result: column l % 16, rows l / 16 + 4 i
-  const int col = j0 + r;
-  const bool can = col < a.nb && a.counts[(int64_t)b * a.nb + col] > 0;
+#pragma unroll
+  for (int t = 0; t < kScoreTiles; ++t) {
+    const int col = j0 + t * 16 + r;
+    const bool can = col < a.nb && a.counts[(int64_t)b * a.nb + col] > 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = s0 + g + 4 * i;
+      if (row < a.S && col < a.nb) a.keys[(bh * a.S + row) * a.nb + col] = score_key(acc[t][i], can);
+    }
+  }
+}
+
+// Scores and choice of 16 groups by one wave, up to 16 NT blocks, without a score leaving the registers: after the products lane l
+// holds, for block column l % 16 of every tile, the keys of rows l / 16 + 4 i.  The 16 lanes of a quarter hold one whole row for each
+// i, so the four quarters search the thresholds of four rows at once: how many keys of the row are >= the candidate (sum over the
+// quarter), bit by bit from the top of the upper 32 bits; the lower ones are looked at only by a row whose upper bits do not settle it.
+// DIRECT: the group's few queries are summed here; otherwise they come from the workspace.  DS: slices of 16 channels.
+// Keeping the scores in registers against writing them out and reading them back: 330 -> TBD us (65,536 groups x 256 blocks).
+__device__ __forceinline__ int quarter_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);   // row_ror:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xf, 0xf, false);   // row_ror:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x122, 0xf, 0xf, false);   // row_ror:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x121, 0xf, 0xf, false);   // row_ror:1
+  return v;
+}
+template <typename T, bool DIRECT, int NT, int DS>
+__global__ __launch_bounds__(256) void select_fused_kernel(SelectArgs a) {
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int r = lane % 16, g = lane / 16;
+  const int stiles = (a.S + 15) / 16;
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+  if (id >= (int64_t)a.B * a.Hkv * stiles) return;
+  const int64_t bh = id / stiles;
+  const int s0 = (int)(id - bh * stiles) * 16, hk = (int)(bh % a.Hkv), b = (int)(bh / a.Hkv);
+  // the groups' query sums: this lane's row r, channels 16 c + 4 g .. + 3
+  double q[DS][4];
+  const int s = min(s0 + r, a.S - 1);
+  if (DIRECT) {
+    typedef typename SelVec<T, 4>::type vec;
+    const T *qp = reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sb + (int64_t)hk * a.G * a.sh;
+    const int n0 = (int)((int64_t)s * a.q_block), n1 = (int)min((int64_t)a.N, (int64_t)n0 + a.q_block);
+#pragma unroll
+    for (int c = 0; c < DS; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[c][e] = 0.0;
+    for (int n = n0; n < n1; ++n)
+      for (int h = 0; h < a.G; ++h)
+#pragma unroll
+        for (int c = 0; c < DS; ++c) {
+          const int ch = c * 16 + g * 4;
+          const vec t = *reinterpret_cast<const vec *>(qp + (int64_t)n * a.sn + (int64_t)h * a.sh + min(ch, a.D - 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[c][e] += ch < a.D ? (double)(float)t[e] : 0.0;
+        }
+  } else {
+#pragma unroll
+    for (int c = 0; c < DS; ++c) {
+      const int ch = c * 16 + g * 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[c][e] = ch < a.D ? a.pooled[(bh * a.S + s) * a.D + ch + e] : 0.0;
+    }
+  }
+  uint32_t hi[NT][4], lo[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int j = t * 16 + r;
+    const float *mp = a.means + (bh * a.nb + min(j, a.nb - 1)) * a.D;
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    f4 mv[DS];
+#pragma unroll
+    for (int c = 0; c < DS; ++c) mv[c] = *reinterpret_cast<const f4 *>(mp + min(c * 16 + g * 4, a.D - 4));
+    const bool can = a.counts[(int64_t)b * a.nb + min(j, a.nb - 1)] > 0 && j < a.nb;
+    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int c = 0; c < DS; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(q[c][e], c * 16 + g * 4 < a.D ? (double)mv[c][e] : 0.0, acc, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t k = score_key(acc[i], can);
+      hi[t][i] = (uint32_t)(k >> 32);
+      lo[t][i] = (uint32_t)k;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = s0 + g + 4 * i;
-    if (row < a.S && col < a.nb) a.keys[(bh * a.S + row) * a.nb + col] = score_key(acc[i], can);
+    int valid = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) valid += (hi[t][i] | lo[t][i]) != 0;
+    valid = quarter_sum(valid);
+    const int want = min(a.top, valid);
+    // th: the largest value that at least `want` upper halves reach; a row whose count is exact is done
+    uint32_t th = 0;
+    int have = -1;
+    for (int bit = 31; bit >= 0 && __any(have != want); --bit) {
+      const uint32_t cand = th | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) n += hi[t][i] >= cand;
+      n = quarter_sum(n);
+      if (n >= want && have != want) { th = cand; have = n; }
+    }
+    if (have < 0) have = 16 * NT;                                // no bit set: every upper half reaches 0
+    // upper halves equal to th: by the lower half, then by index
+    uint32_t tl = 0;
+    int stay = 16 * NT;                                          // of the keys equal to (th, tl), how many stay in, from the lowest index
+    if (__any(have != want)) {
+      int over = 0, equal = 0;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) over += hi[t][i] > th;
+      over = quarter_sum(over);
+      const int need = want - over;                              // of the upper halves equal to th
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t cand = tl | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) n += hi[t][i] == th && lo[t][i] >= cand;
+        n = quarter_sum(n);
+        if (have != want && n >= need) tl = cand;
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) equal += hi[t][i] == th && lo[t][i] > tl;
+      equal = quarter_sum(equal);
+      if (have != want) stay = need - equal;
+    }
+    int at = 0, eq = 0;
+    int32_t *out = a.blocks + (bh * a.S + row) * a.top;
+    const uint32_t below = (1u << r) - 1;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const bool ok = (hi[t][i] | lo[t][i]) != 0 && want > 0;
+      const bool same = hi[t][i] == th && lo[t][i] == tl && stay < 16 * NT;
+      const uint32_t sm = (uint32_t)(__ballot(same) >> (16 * g)) & 0xffffu;
+      const bool in = ok && (hi[t][i] > th || (hi[t][i] == th && lo[t][i] >= tl)) && (!same || eq + __popc(sm & below) < stay);
+      const uint32_t m = (uint32_t)(__ballot(in) >> (16 * g)) & 0xffffu;
+      if (in && row < a.S) out[at + __popc(m & below)] = t * 16 + r;
+      at += __popc(m);
+      eq += __popc(sm);
+    }
+    if (row < a.S)
+      for (int x = at + r; x < a.top; x += 16) out[x] = -1;
   }
 }
 
@@ -272,12 +436,20 @@ __global__ __launch_bounds__(256) void select_topk_block_kernel(SelectArgs a) {
 }
 
 constexpr int64_t kMaxBlocks = 16384;   // keys of one row in LDS: 128 KB
-constexpr int kWaveKeys = 8;            // up to 512 blocks a wave holds the row in registers
+constexpr int kWaveKeys = 8;            // up to 512 blocks a wave holds the row's keys in registers
+constexpr int kFusedBlocks = 256;       // up to 256 blocks a wave holds the keys of 16 rows
+constexpr int kDirectRows = 8;          // groups of up to 8 query rows are summed where they are used
 
 static size_t pooled_bytes(int64_t B, int64_t Hkv, int64_t S, int64_t D) { return round_up((size_t)(B * Hkv * S * D) * sizeof(double), 256); }
 
-template <typename T> static void launch_pool(const SelectArgs &a, unsigned blocks, hipStream_t s) {
-  hipLaunchKernelGGL((select_pool_kernel<T>), dim3(blocks), dim3(256), 0, s, a);
+template <typename T, bool DIRECT> static void launch_fused(const SelectArgs &a, dim3 wg, hipStream_t s) {
+  if (a.nb <= 64) {
+    if (a.D <= 64) hipLaunchKernelGGL((select_fused_kernel<T, DIRECT, 4, 4>), wg, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((select_fused_kernel<T, DIRECT, 4, 8>), wg, dim3(256), 0, s, a);
+  } else {
+    if (a.D <= 64) hipLaunchKernelGGL((select_fused_kernel<T, DIRECT, 16, 4>), wg, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((select_fused_kernel<T, DIRECT, 16, 8>), wg, dim3(256), 0, s, a);
+  }
 }
 
 }  // namespace tcl
@@ -307,7 +479,7 @@ extern "C" int tcl_block_means(const void *k, int64_t k_sb, int64_t k_sn, int64_
 
 extern "C" size_t tcl_select_blocks_workspace_bytes(int64_t B, int64_t Hkv, int64_t S, int64_t nb, int64_t D) {
   if (B <= 0 || Hkv <= 0 || S <= 0 || nb <= 0 || D <= 0) return 256;
-  return pooled_bytes(B, Hkv, S, D) + round_up((size_t)(B * Hkv * S * nb) * sizeof(uint64_t), 256);
+  return pooled_bytes(B, Hkv, S, D) + (nb <= kFusedBlocks ? 0 : round_up((size_t)(B * Hkv * S * nb) * sizeof(uint64_t), 256));
 }
 
 extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const float *means, const int32_t *counts, int32_t *blocks,
@@ -321,6 +493,9 @@ extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int6
   const int64_t S = cdiv(N, q_block), rows = B * Hkv * S;
   if (rows == 0) return TCL_OK;
   TCL_REQUIRE(q && blocks && (nb == 0 || (means && counts)), TCL_ERR_ARG, "select_blocks: null pointer");
+  const size_t size = dtype == TCL_DT_F32 ? 4 : 2;
+  TCL_REQUIRE(aligned(q, 4 * size) && q_sb % 4 == 0 && q_sn % 4 == 0 && q_sh % 4 == 0 && aligned(means, 16), TCL_ERR_ARG,
+              "select_blocks: query rows must start on 4 elements, means on 16 bytes");
   TCL_REQUIRE(rows < (1LL << 31) && B * Hkv < 65536 && cdiv(S, 16) < 65536, TCL_ERR_SHAPE, "select_blocks: %ld groups are too many for one call", (long)rows);
   const size_t need = tcl_select_blocks_workspace_bytes(B, Hkv, S, nb, D);
   TCL_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, TCL_ERR_WORKSPACE, "select_blocks: workspace of %zu bytes needed", need);
@@ -328,17 +503,26 @@ extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int6
                (int)top_k, (int)q_block, (int)S};
   a.keys = (uint64_t *)((char *)workspace + pooled_bytes(B, Hkv, S, D));
   const hipStream_t s = (hipStream_t)stream;
-  if (nb > 0) {
-    const unsigned pb = (unsigned)cdiv(rows, 4);
-    if (dtype == TCL_DT_F32) launch_pool<float>(a, pb, s);
-    else if (dtype == TCL_DT_BF16) launch_pool<__bf16>(a, pb, s);
-    else launch_pool<_Float16>(a, pb, s);
-    hipLaunchKernelGGL(select_score_kernel, dim3((unsigned)cdiv(nb, 64), (unsigned)cdiv(S, 16), (unsigned)(B * Hkv)), dim3(256), 0, s, a);
+  a.by_g = make_fastdiv((uint32_t)a.G);
+  const int64_t per_group = (q_block < N ? q_block : N) * a.G;
+  TCL_REQUIRE(per_group < (1LL << 31), TCL_ERR_SHAPE, "select_blocks: groups of %ld query rows", (long)per_group);
+  const bool fused = nb > 0 && nb <= kFusedBlocks, direct = fused && per_group <= kDirectRows;
+  if (nb > 0 && !direct) {
+    const dim3 pool((unsigned)cdiv(rows, 4));
+    if (dtype == TCL_DT_F32) hipLaunchKernelGGL((select_pool_kernel<float>), pool, dim3(256), 0, s, a);
+    else if (dtype == TCL_DT_BF16) hipLaunchKernelGGL((select_pool_kernel<__bf16>), pool, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((select_pool_kernel<_Float16>), pool, dim3(256), 0, s, a);
   }
-  const dim3 wg((unsigned)cdiv(rows, 4));
-  if (nb <= 64) hipLaunchKernelGGL((select_topk_wave_kernel<1>), wg, dim3(256), 0, s, a);
-  else if (nb <= 256) hipLaunchKernelGGL((select_topk_wave_kernel<4>), wg, dim3(256), 0, s, a);
-  else if (nb <= 64 * kWaveKeys) hipLaunchKernelGGL((select_topk_wave_kernel<kWaveKeys>), wg, dim3(256), 0, s, a);
+  if (fused) {
+    const dim3 wg((unsigned)cdiv(B * Hkv * cdiv(S, 16), 4));
+    if (!direct) launch_fused<double, false>(a, wg, s);
+    else if (dtype == TCL_DT_F32) launch_fused<float, true>(a, wg, s);
+    else if (dtype == TCL_DT_BF16) launch_fused<__bf16, true>(a, wg, s);
+    else launch_fused<_Float16, true>(a, wg, s);
+    return check_launch("select_blocks");
+  }
+  if (nb > 0) hipLaunchKernelGGL(select_score_kernel, dim3((unsigned)cdiv(nb, 64 * kScoreTiles), (unsigned)cdiv(S, 16), (unsigned)(B * Hkv)), dim3(256), 0, s, a);
+  if (nb <= 64 * kWaveKeys) hipLaunchKernelGGL((select_topk_wave_kernel<kWaveKeys>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a);
   else {
     const size_t lds = (size_t)(nb + 255) / 256 * 256 * sizeof(uint64_t);
     TCL_REQUIRE(lds_ready((const void *)select_topk_block_kernel, lds), TCL_ERR_LAUNCH, "select_blocks: the device refuses %zu bytes of LDS", lds);
