@@ -192,28 +192,63 @@ __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
   }
 }
 
-// Scores and choice of 16 groups by one wave, up to 16 NT blocks, without a score leaving the registers: after the products lane l
-// holds, for block column l % 16 of every tile, the keys of rows l / 16 + 4 i.  The 16 lanes of a quarter hold one whole row for each
-// i, so the four quarters search the thresholds of four rows at once: how many keys of the row are >= the candidate (sum over the
-// quarter), bit by bit from the top of the upper 32 bits; the lower ones are looked at only by a row whose upper bits do not settle it.
-// DIRECT: the group's few queries are summed here; otherwise they come from the workspace.  DS: slices of 16 channels.
-// Keeping the scores in registers against writing them out and reading them back: 330 -> TBD us (65,536 groups x 256 blocks).
-__device__ __forceinline__ int quarter_sum(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);   // row_ror:8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xf, 0xf, false);   // row_ror:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x122, 0xf, 0xf, false);   // row_ror:2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x121, 0xf, 0xf, false);   // row_ror:1
-  return v;
+// The top_k largest of the keys a wave holds (R per lane, key i of a lane has index 64 i + lane): ties to the lower index, ascending,
+// -1 behind the last.  The threshold is found bit by bit from the top (how many keys are >= the candidate?), and the search ends
+// as soon as exactly the wanted number passes: after some 20 bits, as scores go.
+template <int R> __device__ __forceinline__ void choose(const uint64_t (&key)[R], int top, int32_t *out) {
+  const int lane = threadIdx.x % 64;
+  int valid = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) valid += __popcll(__ballot(key[i] != 0));
+  const int want = min(top, valid);
+  uint64_t t = 1;                                               // everything that can be chosen
+  int have = valid;
+  if (have > want) {
+    t = 0;
+    for (int bit = 63; bit >= 0 && have != want; --bit) {
+      const uint64_t cand = t | (1ull << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= cand));
+      if (n >= want) { t = cand; have = n; }
+    }
+  }
+  const int spare = have - want;                                // keys equal to t that have to stay out: the last ones
+  int equal = 0;
+  if (spare > 0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) equal += __popcll(__ballot(key[i] == t));
+    equal -= spare;                                             // how many of them stay in
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  int at = 0, eq = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const bool same = spare > 0 && key[i] == t;
+    const uint64_t sm = __ballot(same);
+    const bool in = key[i] >= t && want > 0 && (!same || eq + __popcll(sm & below) < equal);
+    const uint64_t m = __ballot(in);
+    if (in) out[at + __popcll(m & below)] = i * 64 + lane;
+    at += __popcll(m);
+    eq += __popcll(sm);
+  }
+  for (int i = at + lane; i < top; i += 64) out[i] = -1;
 }
-template <typename T, bool DIRECT, int NT, int DS>
+
+// Scores and choice of 16 groups by one workgroup, up to 64 R blocks: the four waves share out the products' block tiles, the keys meet
+// in LDS, and every wave chooses for four of the groups.  DIRECT: the groups' few queries are summed here; otherwise the sums come
+// from the workspace.  DS: slices of 16 channels.
+// Against scores written out and read back by a second kernel 330 -> 111 us (65,536 groups x 256 blocks, one wave per 16 groups with the keys
+// in registers), -> TBD us with the waves sharing the work as here.
+template <typename T, bool DIRECT, int R, int DS>
 __global__ __launch_bounds__(256) void select_fused_kernel(SelectArgs a) {
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  constexpr int LD = R * 64 + 16;
+  extern __shared__ uint64_t lkey[];                            // [16][LD]
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int r = lane % 16, g = lane / 16;
   const int stiles = (a.S + 15) / 16;
-  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
-  if (id >= (int64_t)a.B * a.Hkv * stiles) return;
-  const int64_t bh = id / stiles;
-  const int s0 = (int)(id - bh * stiles) * 16, hk = (int)(bh % a.Hkv), b = (int)(bh / a.Hkv);
+  const int64_t bh = blockIdx.x / (unsigned)stiles;
+  const int s0 = (int)(blockIdx.x - (unsigned)bh * (unsigned)stiles) * 16, hk = (int)(bh % a.Hkv), b = (int)(bh / a.Hkv);
   // the groups' query sums: this lane's row r, channels 16 c + 4 g .. + 3
   double q[DS][4];
   const int s = min(s0 + r, a.S - 1);
@@ -242,12 +277,11 @@ __global__ __launch_bounds__(256) void select_fused_kernel(SelectArgs a) {
       for (int e = 0; e < 4; ++e) q[c][e] = ch < a.D ? a.pooled[(bh * a.S + s) * a.D + ch + e] : 0.0;
     }
   }
-  uint32_t hi[NT][4], lo[NT][4];
+  typedef float f4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int j = t * 16 + r;
+  for (int t = 0; t < R; ++t) {
+    const int j = (t * 4 + wave) * 16 + r;
     const float *mp = a.means + (bh * a.nb + min(j, a.nb - 1)) * a.D;
-    typedef float f4 __attribute__((ext_vector_type(4)));
     f4 mv[DS];
 #pragma unroll
     for (int c = 0; c < DS; ++c) mv[c] = *reinterpret_cast<const f4 *>(mp + min(c * 16 + g * 4, a.D - 4));
@@ -258,126 +292,21 @@ __global__ __launch_bounds__(256) void select_fused_kernel(SelectArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(q[c][e], c * 16 + g * 4 < a.D ? (double)mv[c][e] : 0.0, acc, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint64_t k = score_key(acc[i], can);
-      hi[t][i] = (uint32_t)(k >> 32);
-      lo[t][i] = (uint32_t)k;
-    }
+    for (int i = 0; i < 4; ++i) lkey[(g + 4 * i) * LD + j] = score_key(acc[i], can);
   }
+  __syncthreads();
+#pragma unroll 1
+  for (int x = 0; x < 4; ++x) {
+    const int row = wave * 4 + x;
+    if (s0 + row >= a.S) break;
+    uint64_t key[R];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = s0 + g + 4 * i;
-    int valid = 0;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) valid += (hi[t][i] | lo[t][i]) != 0;
-    valid = quarter_sum(valid);
-    const int want = min(a.top, valid);
-    // th: the largest value that at least `want` upper halves reach; a row whose count is exact is done
-    uint32_t th = 0;
-    int have = -1;
-    for (int bit = 31; bit >= 0 && __any(have != want); --bit) {
-      const uint32_t cand = th | (1u << bit);
-      int n = 0;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) n += hi[t][i] >= cand;
-      n = quarter_sum(n);
-      if (n >= want && have != want) { th = cand; have = n; }
-    }
-    if (have < 0) have = 16 * NT;                                // no bit set: every upper half reaches 0
-    // upper halves equal to th: by the lower half, then by index
-    uint32_t tl = 0;
-    int stay = 16 * NT;                                          // of the keys equal to (th, tl), how many stay in, from the lowest index
-    if (__any(have != want)) {
-      int over = 0, equal = 0;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) over += hi[t][i] > th;
-      over = quarter_sum(over);
-      const int need = want - over;                              // of the upper halves equal to th
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t cand = tl | (1u << bit);
-        int n = 0;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) n += hi[t][i] == th && lo[t][i] >= cand;
-        n = quarter_sum(n);
-        if (have != want && n >= need) tl = cand;
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) equal += hi[t][i] == th && lo[t][i] > tl;
-      equal = quarter_sum(equal);
-      if (have != want) stay = need - equal;
-    }
-    int at = 0, eq = 0;
-    int32_t *out = a.blocks + (bh * a.S + row) * a.top;
-    const uint32_t below = (1u << r) - 1;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const bool ok = (hi[t][i] | lo[t][i]) != 0 && want > 0;
-      const bool same = hi[t][i] == th && lo[t][i] == tl && stay < 16 * NT;
-      const uint32_t sm = (uint32_t)(__ballot(same) >> (16 * g)) & 0xffffu;
-      const bool in = ok && (hi[t][i] > th || (hi[t][i] == th && lo[t][i] >= tl)) && (!same || eq + __popc(sm & below) < stay);
-      const uint32_t m = (uint32_t)(__ballot(in) >> (16 * g)) & 0xffffu;
-      if (in && row < a.S) out[at + __popc(m & below)] = t * 16 + r;
-      at += __popc(m);
-      eq += __popc(sm);
-    }
-    if (row < a.S)
-      for (int x = at + r; x < a.top; x += 16) out[x] = -1;
+    for (int i = 0; i < R; ++i) key[i] = lkey[row * LD + i * 64 + lane];
+    choose<R>(key, a.top, a.blocks + (bh * a.S + s0 + row) * a.top);
   }
 }
 
-// The top_k largest keys of one row, ties to the lower index, ascending, -1 behind the last.  One wave per row, R keys per lane.
-// The threshold is found bit by bit from the top (how many keys are >= the candidate?), and the search ends as soon as exactly
-// the wanted number passes.
-template <int R>
-__global__ __launch_bounds__(256) void select_topk_wave_kernel(SelectArgs a) {
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-  if (row >= (int64_t)a.B * a.Hkv * a.S) return;
-  uint64_t key[R];
-  int valid = 0;
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int j = i * 64 + lane;
-    key[i] = j < a.nb ? a.keys[row * a.nb + j] : 0ull;
-    valid += __popcll(__ballot(key[i] != 0));
-  }
-  const int want = min(a.top, valid);
-  uint64_t t = 1;                                               // everything that can be chosen
-  int have = valid;
-  if (have > want) {
-    t = 0;
-    for (int bit = 63; bit >= 0 && have != want; --bit) {
-      const uint64_t cand = t | (1ull << bit);
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= cand));
-      if (n >= want) { t = cand; have = n; }
-    }
-  }
-  int spare = have - want;                                      // keys equal to t that have to stay out: the last ones
-  int equal = 0;
-  if (spare > 0) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) equal += __popcll(__ballot(key[i] == t));
-    equal -= spare;                                             // how many of them stay in
-  }
-  int32_t *out = a.blocks + row * a.top;
-  const uint64_t below = (1ull << lane) - 1;
-  int at = 0, eq = 0;
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const bool same = spare > 0 && key[i] == t;
-    const uint64_t sm = __ballot(same);
-    const bool in = key[i] >= t && want > 0 && (!same || eq + __popcll(sm & below) < equal);
-    const uint64_t m = __ballot(in);
-    if (in) out[at + __popcll(m & below)] = i * 64 + lane;
-    at += __popcll(m);
-    eq += __popcll(sm);
-  }
-  for (int i = at + lane; i < a.top; i += 64) out[i] = -1;
-}
-
-// The same for long rows: one workgroup per row, the keys in LDS.
+// The choice for long rows: one workgroup per row, its keys in LDS.
 __global__ __launch_bounds__(256) void select_topk_block_kernel(SelectArgs a) {
   extern __shared__ uint64_t lkey[];
   __shared__ int lsum[2][4];
@@ -436,20 +365,22 @@ __global__ __launch_bounds__(256) void select_topk_block_kernel(SelectArgs a) {
 }
 
 constexpr int64_t kMaxBlocks = 16384;   // keys of one row in LDS: 128 KB
-constexpr int kWaveKeys = 8;            // up to 512 blocks a wave holds the row's keys in registers
-constexpr int kFusedBlocks = 256;       // up to 256 blocks a wave holds the keys of 16 rows
+constexpr int kFusedBlocks = 512;       // up to 512 blocks the keys of 16 groups stay in LDS (68 KB)
 constexpr int kDirectRows = 8;          // groups of up to 8 query rows are summed where they are used
 
 static size_t pooled_bytes(int64_t B, int64_t Hkv, int64_t S, int64_t D) { return round_up((size_t)(B * Hkv * S * D) * sizeof(double), 256); }
 
-template <typename T, bool DIRECT> static void launch_fused(const SelectArgs &a, dim3 wg, hipStream_t s) {
-  if (a.nb <= 64) {
-    if (a.D <= 64) hipLaunchKernelGGL((select_fused_kernel<T, DIRECT, 4, 4>), wg, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((select_fused_kernel<T, DIRECT, 4, 8>), wg, dim3(256), 0, s, a);
-  } else {
-    if (a.D <= 64) hipLaunchKernelGGL((select_fused_kernel<T, DIRECT, 16, 4>), wg, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((select_fused_kernel<T, DIRECT, 16, 8>), wg, dim3(256), 0, s, a);
-  }
+template <typename T, bool DIRECT, int R> static int launch_fused_r(const SelectArgs &a, dim3 wg, hipStream_t s) {
+  const size_t lds = (size_t)16 * (R * 64 + 16) * sizeof(uint64_t);
+  const auto kernel = a.D <= 64 ? select_fused_kernel<T, DIRECT, R, 4> : select_fused_kernel<T, DIRECT, R, 8>;
+  TCL_REQUIRE(lds_ready((const void *)kernel, lds), TCL_ERR_LAUNCH, "select_blocks: the device refuses %zu bytes of LDS", lds);
+  hipLaunchKernelGGL(kernel, wg, dim3(256), lds, s, a);
+  return check_launch("select_blocks");
+}
+template <typename T, bool DIRECT> static int launch_fused(const SelectArgs &a, dim3 wg, hipStream_t s) {
+  if (a.nb <= 64) return launch_fused_r<T, DIRECT, 1>(a, wg, s);
+  if (a.nb <= 256) return launch_fused_r<T, DIRECT, 4>(a, wg, s);
+  return launch_fused_r<T, DIRECT, 8>(a, wg, s);
 }
 
 }  // namespace tcl
@@ -514,19 +445,16 @@ extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int6
     else hipLaunchKernelGGL((select_pool_kernel<_Float16>), pool, dim3(256), 0, s, a);
   }
   if (fused) {
-    const dim3 wg((unsigned)cdiv(B * Hkv * cdiv(S, 16), 4));
-    if (!direct) launch_fused<double, false>(a, wg, s);
-    else if (dtype == TCL_DT_F32) launch_fused<float, true>(a, wg, s);
-    else if (dtype == TCL_DT_BF16) launch_fused<__bf16, true>(a, wg, s);
-    else launch_fused<_Float16, true>(a, wg, s);
-    return check_launch("select_blocks");
+    TCL_REQUIRE(B * Hkv * cdiv(S, 16) < (1LL << 31), TCL_ERR_SHAPE, "select_blocks: %ld groups are too many for one call", (long)rows);
+    const dim3 wg((unsigned)(B * Hkv * cdiv(S, 16)));
+    if (!direct) return launch_fused<double, false>(a, wg, s);
+    if (dtype == TCL_DT_F32) return launch_fused<float, true>(a, wg, s);
+    if (dtype == TCL_DT_BF16) return launch_fused<__bf16, true>(a, wg, s);
+    return launch_fused<_Float16, true>(a, wg, s);
   }
   if (nb > 0) hipLaunchKernelGGL(select_score_kernel, dim3((unsigned)cdiv(nb, 64 * kScoreTiles), (unsigned)cdiv(S, 16), (unsigned)(B * Hkv)), dim3(256), 0, s, a);
-  if (nb <= 64 * kWaveKeys) hipLaunchKernelGGL((select_topk_wave_kernel<kWaveKeys>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a);
-  else {
-    const size_t lds = (size_t)(nb + 255) / 256 * 256 * sizeof(uint64_t);
-    TCL_REQUIRE(lds_ready((const void *)select_topk_block_kernel, lds), TCL_ERR_LAUNCH, "select_blocks: the device refuses %zu bytes of LDS", lds);
-    hipLaunchKernelGGL(select_topk_block_kernel, dim3((unsigned)rows), dim3(256), lds, s, a);
-  }
+  const size_t lds = (size_t)(nb + 255) / 256 * 256 * sizeof(uint64_t);
+  TCL_REQUIRE(lds_ready((const void *)select_topk_block_kernel, lds), TCL_ERR_LAUNCH, "select_blocks: the device refuses %zu bytes of LDS", lds);
+  hipLaunchKernelGGL(select_topk_block_kernel, dim3((unsigned)rows), dim3(256), lds, s, a);
   return check_launch("select_blocks");
 }
