@@ -192,45 +192,92 @@ __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
   }
 }
 
+// maximum over the wave of an unsigned value
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+#define TCL_DPP(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false))
+  TCL_DPP(0x111, 0xf);   // row_shr:1, 2, 4, 8: lane 15 of each row of 16 has the row's maximum
+  TCL_DPP(0x112, 0xf);
+  TCL_DPP(0x114, 0xf);
+  TCL_DPP(0x118, 0xf);
+  TCL_DPP(0x142, 0xa);   // row_bcast:15 into rows 1 and 3
+  TCL_DPP(0x143, 0xc);   // row_bcast:31 into rows 2 and 3
+#undef TCL_DPP
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // The top_k largest of the keys a wave holds (R per lane, key i of a lane has index 64 i + lane): ties to the lower index, ascending,
-// -1 behind the last.  The threshold is found bit by bit from the top (how many keys are >= the candidate?), and the search ends
-// as soon as exactly the wanted number passes: after some 20 bits, as scores go.
+// -1 behind the last.  The threshold is found bit by bit (how many keys are >= the candidate?), and the search ends as soon as
+// exactly the wanted number passes.  The sign and exponent come from the largest key downwards (the threshold is seldom more than
+// a few binades below it; if it is, the search starts at the top bit), then the upper half's other 20 bits; the lower half is looked at
+// only if keys share the threshold's upper half.
 template <int R> __device__ __forceinline__ void choose(const uint64_t (&key)[R], int top, int32_t *out) {
   const int lane = threadIdx.x % 64;
+  uint32_t hi[R], most = 0;
   int valid = 0;
 #pragma unroll
-  for (int i = 0; i < R; ++i) valid += __popcll(__ballot(key[i] != 0));
+  for (int i = 0; i < R; ++i) {
+    hi[i] = (uint32_t)(key[i] >> 32);
+    most = max(most, hi[i]);
+    valid += __popcll(__ballot(key[i] != 0));
+  }
   const int want = min(top, valid);
+  auto reach = [&](uint32_t c) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) n += __popcll(__ballot(hi[i] >= c));
+    return n;
+  };
   uint64_t t = 1;                                               // everything that can be chosen
   int have = valid;
   if (have > want) {
-    t = 0;
-    for (int bit = 63; bit >= 0 && have != want; --bit) {
-      const uint64_t cand = t | (1ull << bit);
-      int n = 0;
+    uint32_t th = (wave_umax(most) >> 20) << 20, bit = 1u << 31;
+    for (int tries = 0; tries < 4 && th >= 1u << 20; ++tries, th -= 1u << 20) {
+      have = reach(th);
+      if (have >= want) { bit = 1u << 19; break; }
+    }
+    if (bit != 1u << 19) { th = 0; have = -1; }
+    while (have != want && bit) {
+      const int n = reach(th | bit);
+      if (n >= want) { th |= bit; have = n; }
+      bit >>= 1;
+    }
+    t = (uint64_t)th << 32;
+    if (have != want) {
+      for (int low = 31; low >= 0 && have != want; --low) {
+        const uint64_t cand = t | (1ull << low);
+        int n = 0;
 #pragma unroll
-      for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= cand));
-      if (n >= want) { t = cand; have = n; }
+        for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= cand));
+        if (n >= want) { t = cand; have = n; }
+      }
     }
   }
-  const int spare = have - want;                                // keys equal to t that have to stay out: the last ones
-  int equal = 0;
-  if (spare > 0) {
+  int at = 0;
+  if (have == want) {
+    if (want > 0) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) equal += __popcll(__ballot(key[i] == t));
-    equal -= spare;                                             // how many of them stay in
-  }
-  const uint64_t below = (1ull << lane) - 1;
-  int at = 0, eq = 0;
+      for (int i = 0; i < R; ++i) {
+        const bool in = key[i] >= t;
+        const uint64_t m = __ballot(in);
+        if (in) out[__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, at))] = i * 64 + lane;
+        at += __popcll(m);
+      }
+    }
+  } else {                                                      // keys equal to t, some of which have to stay out: the last ones
+    int stay = want - have, eq = 0;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const bool same = spare > 0 && key[i] == t;
-    const uint64_t sm = __ballot(same);
-    const bool in = key[i] >= t && want > 0 && (!same || eq + __popcll(sm & below) < equal);
-    const uint64_t m = __ballot(in);
-    if (in) out[at + __popcll(m & below)] = i * 64 + lane;
-    at += __popcll(m);
-    eq += __popcll(sm);
+    for (int i = 0; i < R; ++i) stay += __popcll(__ballot(key[i] == t));
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const bool same = key[i] == t;
+      const uint64_t sm = __ballot(same);
+      const bool in = key[i] >= t && (!same || eq + __popcll(sm & below) < stay);
+      const uint64_t m = __ballot(in);
+      if (in) out[at + __popcll(m & below)] = i * 64 + lane;
+      at += __popcll(m);
+      eq += __popcll(sm);
+    }
   }
   for (int i = at + lane; i < top; i += 64) out[i] = -1;
 }
