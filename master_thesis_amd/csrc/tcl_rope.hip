@@ -17,15 +17,16 @@ namespace tcl {
 
 constexpr int kRopeMaxPairs = 128;   // dim <= 256
 constexpr int kRopeMaxAxes = 4;
+constexpr int kRopeBlocks = kNumCU * 16;   // workgroups of a large call
 
-struct RotateArgs {
+struct RotateArgs {   // passed by value
   const void *x;
   void *y;
   const void *pos;
   int64_t x_sb, x_sn, x_sh, y_sb, y_sn, y_sh, p_sb;
   int N, H, chunks, heads_per_thread, axes, pos_int, interleaved;
-  int64_t total;                       // threads of work per head group: B * N * chunks
-  FastDiv by_chunks;
+  unsigned rows, threads, step;        // B * N; threads at work: step tokens x chunks
+  FastDiv by_chunks, by_n;
   float sign;
   // per pair: frequency in turns (0 = the channels pass through), axis, channel of the first and the second half
   double turns[kRopeMaxPairs];
@@ -58,48 +59,51 @@ template <typename T, int V> __device__ __forceinline__ void rope_st(T *p, const
 
 // V pairs per thread.  IL: a pair is two neighbouring channels (2 V consecutive elements: one access, two where they pass 16
 // bytes or nothing is known of their alignment, V = 1); otherwise the two halves of a section (V elements in each).
+// A thread keeps its pairs and walks tokens `step` apart, so frequencies and channel numbers are read once.
 template <typename T, int V, bool IL>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= a.total) return;
-  const unsigned row = a.by_chunks.div((unsigned)id);          // item * N + token (host: total < 2^31)
-  const int c = (int)((unsigned)id - row * (unsigned)a.chunks);
-  const int b = (int)(row / (unsigned)a.N), n = (int)(row - (unsigned)b * (unsigned)a.N);
-  float cs[V], sn[V];
-  bool turn[V];
+  const unsigned id = blockIdx.x * 256 + threadIdx.x;
+  if (id >= a.threads) return;
+  const unsigned row0 = a.by_chunks.div(id);                     // item * N + token (host: < 2^31)
+  const int c = (int)(id - row0 * (unsigned)a.chunks);
+  double f[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int pair = c * V + i;
-    const double f = a.turns[pair];
-    const int64_t at = (int64_t)b * a.p_sb + (int64_t)n * a.axes + a.axis[pair];
-    const double p = a.pos_int ? (double)reinterpret_cast<const int32_t *>(a.pos)[at] : (double)reinterpret_cast<const float *>(a.pos)[at];
-    const double w = p * f;
-    const float r = (float)(w - rint(w));                       // fraction of a turn
-    turn[i] = f != 0.0;
-    if (sizeof(T) == 4) sincospif(2.f * r, &sn[i], &cs[i]);
-    else { sn[i] = __builtin_amdgcn_sinf(r); cs[i] = __builtin_amdgcn_cosf(r); }
-    sn[i] *= a.sign;
-  }
+  for (int i = 0; i < V; ++i) f[i] = a.turns[c * V + i];
+  const bool turn = f[0] != 0.0;                                 // a chunk lies within one section
+  const int axis = a.axis[c * V], o0 = a.first[c * V], o1 = a.second[c * V];
   const int h0 = blockIdx.y * a.heads_per_thread, h1 = min(a.H, h0 + a.heads_per_thread);
-  const T *x = reinterpret_cast<const T *>(a.x) + (int64_t)b * a.x_sb + (int64_t)n * a.x_sn;
-  T *y = reinterpret_cast<T *>(a.y) + (int64_t)b * a.y_sb + (int64_t)n * a.y_sn;
-  const int o0 = a.first[c * V], o1 = a.second[c * V];
-  for (int h = h0; h < h1; ++h) {
-    float u[2 * V], r[2 * V];
-    const T *xp = x + (int64_t)h * a.x_sh;
-    T *yp = y + (int64_t)h * a.y_sh;
-    constexpr int W = IL && V > 1 && 2 * V * sizeof(T) <= 16 ? 2 * V : V;   // elements of one access
-    rope_ld<T, W>(xp + o0, u);
-    if (W == V) rope_ld<T, V>(xp + (IL ? o0 + V : o1), u + V);
+  constexpr int W = IL && V > 1 && 2 * V * sizeof(T) <= 16 ? 2 * V : V;   // elements of one access
+  for (unsigned row = row0; row < a.rows; row += a.step) {
+    const unsigned b = a.by_n.div(row), n = row - b * (unsigned)a.N;
+    const int64_t at = (int64_t)b * a.p_sb + (int64_t)n * a.axes + axis;
+    const double p = a.pos_int ? (double)reinterpret_cast<const int32_t *>(a.pos)[at] : (double)reinterpret_cast<const float *>(a.pos)[at];
+    const T *x = reinterpret_cast<const T *>(a.x) + (int64_t)b * a.x_sb + (int64_t)n * a.x_sn;
+    T *y = reinterpret_cast<T *>(a.y) + (int64_t)b * a.y_sb + (int64_t)n * a.y_sn;
+    float cs[V], sn[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int ia = IL ? 2 * i : i, ib = IL ? 2 * i + 1 : V + i;
-      const float p = u[ia], q = u[ib];
-      r[ia] = turn[i] ? p * cs[i] - q * sn[i] : p;
-      r[ib] = turn[i] ? q * cs[i] + p * sn[i] : q;
+      const double w = p * f[i];
+      const float r = (float)(w - rint(w));                       // fraction of a turn
+      if (sizeof(T) == 4) sincospif(2.f * r, &sn[i], &cs[i]);
+      else { sn[i] = __builtin_amdgcn_sinf(r); cs[i] = __builtin_amdgcn_cosf(r); }
+      sn[i] *= a.sign;
     }
-    rope_st<T, W>(yp + o0, r);
-    if (W == V) rope_st<T, V>(yp + (IL ? o0 + V : o1), r + V);
+    for (int h = h0; h < h1; ++h) {
+      float u[2 * V], r[2 * V];
+      const T *xp = x + (int64_t)h * a.x_sh;
+      T *yp = y + (int64_t)h * a.y_sh;
+      rope_ld<T, W>(xp + o0, u);
+      if (W == V) rope_ld<T, V>(xp + (IL ? o0 + V : o1), u + V);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int ia = IL ? 2 * i : i, ib = IL ? 2 * i + 1 : V + i;
+        const float p = u[ia], q = u[ib];
+        r[ia] = turn ? p * cs[i] - q * sn[i] : p;
+        r[ib] = turn ? q * cs[i] + p * sn[i] : q;
+      }
+      rope_st<T, W>(yp + o0, r);
+      if (W == V) rope_st<T, V>(yp + (IL ? o0 + V : o1), r + V);
+    }
   }
 }
 
@@ -113,14 +117,19 @@ template <typename T> static int rotate_launch(RotateArgs &a, int64_t B, int pai
   int V = sizeof(T) == 4 ? 4 : 8;
   while (V > 1 && unit % (a.interleaved ? 2 * V : V)) V /= 2;
   a.chunks = pairs / V;
-  a.total = B * a.N * a.chunks;
-  TCL_REQUIRE(a.total < (1LL << 31), TCL_ERR_SHAPE, "rotate_positions: %ld tokens are too many for one call", (long)(B * a.N));
+  TCL_REQUIRE(B * a.N < (1LL << 31), TCL_ERR_SHAPE, "rotate_positions: %ld tokens are too many for one call", (long)(B * a.N));
+  a.rows = (unsigned)(B * a.N);
   a.by_chunks = make_fastdiv((uint32_t)a.chunks);
-  // heads per thread: all of them share the angles, but a small call is split over the heads until it fills the CUs
-  const int64_t blocks = cdiv(a.total, 256);
-  int groups = (int)(blocks >= kNumCU * 4 ? 1 : cdiv(kNumCU * 4, blocks));
+  a.by_n = make_fastdiv((uint32_t)a.N);
+  // All heads of a token share the angles, but a small call is split over the heads until it fills the CUs; a large one gives every
+  // thread several tokens (the frequencies are then read once for them)
+  const int64_t all = cdiv((int64_t)a.rows * a.chunks, 256);
+  int groups = (int)(all >= kNumCU * 4 ? 1 : cdiv(kNumCU * 4, all));
   if (groups > a.H) groups = a.H;
   a.heads_per_thread = (int)cdiv(a.H, groups);
+  const int64_t blocks = all < kRopeBlocks ? all : kRopeBlocks;
+  a.step = (unsigned)(blocks * 256 / a.chunks);
+  a.threads = a.step * (unsigned)a.chunks;
   const dim3 grid((unsigned)blocks, (unsigned)cdiv(a.H, a.heads_per_thread));
   switch (V) {
     case 8: if constexpr (sizeof(T) == 2) rotate_launch_v<T, 8>(a, grid, s); break;
