@@ -282,8 +282,8 @@ int tcl_block_means(const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh, con
 /*   The blocks each group of queries attends to.  A group is q_block consecutive tokens with the G query heads of one key head; its
  *   score of block j is <sum of its queries, means[j]> in 64 bits.  blocks int32 (B,Hkv,S,top_k), S = ceil(N / q_block): the top_k
  *   best blocks with counts > 0 (ties to the lower index; a score of -inf or NaN is not chosen), in ascending order, -1 behind the
- *   last.  nb up to 16,384. */
-size_t tcl_select_blocks_workspace_bytes(int64_t B, int64_t Hkv, int64_t S, int64_t nb, int64_t D);
+ *   last.  nb up to 16,384.  A workspace of 0 bytes may be NULL. */
+size_t tcl_select_blocks_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t Hkv, int64_t D, int64_t nb, int64_t q_block);
 int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const float *means, const int32_t *counts, int32_t *blocks,
                       int64_t B, int64_t N, int64_t H, int64_t Hkv, int64_t D, int64_t nb, int64_t top_k, int64_t q_block, int dtype,
                       void *workspace, size_t workspace_bytes, void *stream);
@@ -292,7 +292,7 @@ int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, c
  *   lse = -inf.  visible as in tcl_block_means; blocks (B,Hkv,S,top_k) int32: an index outside [0, nb) is no block, a repeated one
  *   counts once, order does not matter.  lse (B,Hq,Nq) fp32, natural logarithm, nullable (the backward pass needs it).
  *   Limits: top_k <= 2048, nb <= 65,536, q_block * G <= 2^20 (q_block beyond Nq counts as Nq).
- *   Contents of invisible keys do not matter (NaN and infinities included). */
+ *   Contents of invisible keys do not matter (NaN and infinities included).  A workspace of 0 bytes may be NULL. */
 size_t tcl_block_attention_fwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block,
                                                int64_t q_block);
 int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh,

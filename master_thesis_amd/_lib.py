@@ -54,7 +54,7 @@ SIGNATURES = {
     "tcl_resize_flow": (_INT, [_P] * 2 + [_I64] * 5 + [_P]),
     "tcl_rotate_positions": (_INT, [_P] + [_I64] * 3 + [_P, _INT, _I64, _P] + [_I64] * 7 + [_P, _I64, _c.c_double, _INT, _INT, _INT, _P]),
     "tcl_block_means": (_INT, [_P] + [_I64] * 3 + [_P] * 3 + [_I64] * 5 + [_INT, _P]),
-    "tcl_select_blocks_workspace_bytes": (_SZ, [_I64] * 5),
+    "tcl_select_blocks_workspace_bytes": (_SZ, [_I64] * 7),
     "tcl_select_blocks": (_INT, [_P] + [_I64] * 3 + [_P] * 3 + [_I64] * 8 + [_INT, _P, _SZ, _P]),
     "tcl_block_attention_fwd_workspace_bytes": (_SZ, [_I64] * 9),
     "tcl_block_attention_fwd": (_INT, ([_P] + [_I64] * 3) * 3 + [_P] * 2 + [_P] + [_I64] * 3 + [_P] + [_I64] * 9 + [_c.c_double, _INT, _P, _SZ, _P]),
@@ -97,4 +97,6 @@ def check(rc, what):
 
 
 def call(name, *args):
-    check(getattr(lib(), name)(*args), name)
+    rc = getattr(_lib or lib(), name)(*args)
+    if rc:
+        check(rc, name)

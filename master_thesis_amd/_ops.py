@@ -57,7 +57,8 @@ def _on(dev):
 
 
 def _stream(dev):
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    # the raw handle of torch.cuda.current_stream(dev), without the Stream object around it (1.9 us a call, a tenth of a small op)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
 
 
 _WS_CACHE = {}   # (device, stream, bytes) -> buffer, for calls no backward pass will follow
@@ -650,17 +651,40 @@ def _visible(visible, dev, b, n):
 
 def _strides(t):
     """(batch, token, head) strides; the stride of a dimension of size one is never used."""
-    return tuple(0 if t.shape[i] == 1 else t.stride(i) for i in range(3))
+    (b, n, h, _), (sb, sn, sh, _) = t.shape, t.stride()
+    return 0 if b == 1 else sb, 0 if n == 1 else sn, 0 if h == 1 else sh
 
 
 def _rows16(t):
     """t itself if its channels are dense, every row starts on 16 bytes and tokens lie less than 2^22 elements apart, else a dense
     copy."""
-    per, st = 16 // t.element_size(), _strides(t)
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in st) and st[1] < 1 << 22:
+    per, (sb, sn, sh) = 16 // t.element_size(), _strides(t)
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and sb % per == 0 and sn % per == 0 and sh % per == 0 and sn < 1 << 22:
         return t
     c = t.contiguous()
     return c.clone() if c.data_ptr() % 16 else c
+
+
+_SECTIONS = {}   # sections -> the host array the C ABI takes
+
+
+def _rotate(x, positions, sections, base, interleaved, inverse):
+    b, n, h, d = x.shape
+    x = x if x.stride(3) == 1 or d == 1 else x.contiguous()
+    y = torch.empty_like(x)                   # keeps the order of x's dimensions; dense where x is an expanded view
+    if y.stride(3) != 1:
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    secs = _SECTIONS.get(sections)
+    if secs is None:
+        if len(_SECTIONS) >= 64:
+            _SECTIONS.clear()
+        secs = _SECTIONS[sections] = (ctypes.c_int32 * len(sections))(*sections)
+    dev = x.device
+    with _on(dev):
+        _lib.call("tcl_rotate_positions", x.data_ptr(), *_strides(x), positions.data_ptr(), positions.dtype == torch.int32,
+                  n * len(sections) if positions.dim() == 3 else 0, y.data_ptr(), *_strides(y), b, n, h, d, secs, len(sections), base,
+                  interleaved, inverse, _DT[x.dtype], _stream(dev))
+    return y
 
 
 class RotatePositionsFn(torch.autograd.Function):
@@ -679,20 +703,6 @@ class RotatePositionsFn(torch.autograd.Function):
         return _rotate(g, positions, *ctx.meta, True), None, None, None, None
 
 
-def _rotate(x, positions, sections, base, interleaved, inverse):
-    b, n, h, d = x.shape
-    x = x if x.stride(3) == 1 or d == 1 else x.contiguous()
-    y = torch.empty_like(x)                   # keeps the order of x's dimensions; dense where x is an expanded view
-    if y.stride(3) != 1:
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    secs = (ctypes.c_int32 * len(sections))(*sections)
-    with _on(x.device):
-        _lib.call("tcl_rotate_positions", _p(x), *_strides(x), _p(positions), int(positions.dtype == torch.int32),
-                  n * len(sections) if positions.dim() == 3 else 0, _p(y), *_strides(y), b, n, h, d, secs, len(sections), base,
-                  int(interleaved), int(inverse), _DT[x.dtype], _stream(x.device))
-    return y
-
-
 def rotate_positions(x, positions, sections, base=10000.0, interleaved=False):
     dev = _tokens_device("rotate_positions", x)
     b, n, h, d = x.shape
@@ -707,6 +717,8 @@ def rotate_positions(x, positions, sections, base=10000.0, interleaved=False):
         raise TclError("positions are data: no gradient flows to them")
     shape = (n, len(sections)) if positions.dim() == 2 else (b, n, len(sections))
     pos = _side("positions", positions, dev, (torch.float32, torch.int32), shape)
+    if not (x.requires_grad and torch.is_grad_enabled()):
+        return _rotate(x.detach(), pos, sections, float(base), bool(interleaved), False)
     return RotatePositionsFn.apply(x, pos, sections, float(base), bool(interleaved))
 
 
@@ -733,7 +745,7 @@ def block_means(k, visible=None, block=64):
     means = torch.empty((b, h, nb, d), dtype=torch.float32, device=dev)
     counts = torch.empty((b, nb), dtype=torch.int32, device=dev)
     with _on(dev):
-        _lib.call("tcl_block_means", _p(kc), *_strides(kc), _p(vis), _p(means), _p(counts), b, n, h, d, block, _DT[k.dtype], _stream(dev))
+        _lib.call("tcl_block_means", kc.data_ptr(), *_strides(kc), _p(vis), means.data_ptr(), counts.data_ptr(), b, n, h, d, block, _DT[k.dtype], _stream(dev))
     return means, counts
 
 
@@ -752,36 +764,43 @@ def select_blocks(q, means, counts, top_k, q_block=64):
     s = -(-n // q_block)
     qc = _rows16(q.detach())
     blocks = torch.empty((b, hk, s, top_k), dtype=torch.int32, device=dev)
-    ws = _workspace(_lib.lib().tcl_select_blocks_workspace_bytes(b, hk, s, nb, d), dev)
+    nbytes = _lib.lib().tcl_select_blocks_workspace_bytes(b, n, h, hk, d, nb, q_block)
+    ws = _workspace(nbytes, dev) if nbytes else None
     with _on(dev):
-        _lib.call("tcl_select_blocks", _p(qc), *_strides(qc), _p(mc), _p(cc), _p(blocks), b, n, h, hk, d, nb, top_k, q_block, _DT[q.dtype],
-                  _p(ws), ws.numel(), _stream(dev))
+        _lib.call("tcl_select_blocks", qc.data_ptr(), *_strides(qc), mc.data_ptr(), cc.data_ptr(), blocks.data_ptr(), b, n, h, hk, d, nb, top_k, q_block, _DT[q.dtype],
+                  _p(ws), nbytes, _stream(dev))
     return blocks
 
 
+def _attend(q, k, v, blocks, visible, block, q_block, scale, want_lse):
+    """-> out (B,Nq,Hq,D), lse (B,Hq,Nq) | None; q, k, v as _rows16 left them."""
+    dev = q.device
+    b, nq, hq, d = q.shape
+    nk, hk = k.shape[1], k.shape[2]
+    top = blocks.shape[3]
+    out = torch.empty((b, nq, hq, d), dtype=q.dtype, device=dev)
+    lse = torch.empty((b, hq, nq), dtype=torch.float32, device=dev) if want_lse else None
+    nbytes = _lib.lib().tcl_block_attention_fwd_workspace_bytes(b, nq, nk, hq, hk, d, top, block, q_block)
+    ws = _workspace(nbytes, dev) if nbytes else None      # only for few tokens, whose keys are split
+    with _on(dev):
+        _lib.call("tcl_block_attention_fwd", q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), _p(visible),
+                  blocks.data_ptr(), out.data_ptr(), *_strides(out), _p(lse), b, nq, nk, hq, hk, d, top, block, q_block, scale, _DT[q.dtype],
+                  _p(ws), nbytes, _stream(dev))
+    return out, lse
+
+
 class BlockAttentionFn(torch.autograd.Function):
-    """-> out (B,Nq,Hq,D), lse (B,Hq,Nq) | None.  Gradients flow to q, k and v through out; blocks and visible are data, lse is a
+    """-> out (B,Nq,Hq,D), lse (B,Hq,Nq).  Gradients flow to q, k and v through out; blocks and visible are data, lse is a
     statistic."""
 
     @staticmethod
     @_plain_fwd
-    def forward(ctx, q, k, v, blocks, visible, block, q_block, scale, want_lse):
-        dev = q.device
-        b, nq, hq, d = q.shape
-        nk, hk = k.shape[1], k.shape[2]
-        top = blocks.shape[3]
+    def forward(ctx, q, k, v, blocks, visible, block, q_block, scale):
         qc, kc, vc = _rows16(q), _rows16(k), _rows16(v)
-        out = torch.empty((b, nq, hq, d), dtype=q.dtype, device=dev)
-        lse = torch.empty((b, hq, nq), dtype=torch.float32, device=dev) if want_lse or any(ctx.needs_input_grad[:3]) else None
-        ws = _workspace(_lib.lib().tcl_block_attention_fwd_workspace_bytes(b, nq, nk, hq, hk, d, top, block, q_block), dev)
-        with _on(dev):
-            _lib.call("tcl_block_attention_fwd", _p(qc), *_strides(qc), _p(kc), *_strides(kc), _p(vc), *_strides(vc), _p(visible), _p(blocks),
-                      _p(out), *_strides(out), _p(lse), b, nq, nk, hq, hk, d, top, block, q_block, scale, _DT[q.dtype],
-                      _p(ws), ws.numel(), _stream(dev))
+        out, lse = _attend(qc, kc, vc, blocks, visible, block, q_block, scale, True)
         ctx.save_for_backward(qc, kc, vc, blocks, visible, out, lse)
         ctx.meta = (block, q_block, scale)
-        if lse is not None:
-            ctx.mark_non_differentiable(lse)
+        ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
@@ -804,7 +823,7 @@ class BlockAttentionFn(torch.autograd.Function):
                       _p(g_q), *(none if g_q is None else _strides(g_q)), _p(g_k), *(none if g_k is None else _strides(g_k)),
                       _p(g_v), *(none if g_v is None else _strides(g_v)),
                       b, nq, nk, hq, hk, d, top, block, q_block, scale, _DT[q.dtype], _p(ws), ws.numel(), _stream(dev))
-        return g_q, g_k, g_v, None, None, None, None, None, None
+        return g_q, g_k, g_v, None, None, None, None, None
 
 
 def block_attention(q, k, v, blocks, visible=None, block=64, q_block=64, scale=None, return_lse=False):
@@ -824,5 +843,9 @@ def block_attention(q, k, v, blocks, visible=None, block=64, q_block=64, scale=N
         raise ValueError("blocks must be (batch, key head, group, choice), got %s" % (tuple(blocks.shape),))
     bl = _side("blocks", blocks, dev, (torch.int32,), (b, hk, -(-nq // q_block), blocks.shape[3]))
     vis = _visible(visible, dev, b, nk)
-    out, lse = BlockAttentionFn.apply(q, k, v, bl, vis, block, q_block, float(d ** -0.5 if scale is None else scale), bool(return_lse))
+    scale = float(d ** -0.5 if scale is None else scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = BlockAttentionFn.apply(q, k, v, bl, vis, block, q_block, scale)
+    else:
+        out, lse = _attend(_rows16(q.detach()), _rows16(k.detach()), _rows16(v.detach()), bl, vis, block, q_block, scale, return_lse)
     return (out, lse) if return_lse else out

@@ -1135,7 +1135,7 @@ static FwdPlan fwd_plan(const AttnArgs &a, bool f32) {
   int64_t n = cdiv(2 * kNumCU, p.works > 0 ? p.works : 1);
   if (n > tiles / 2) n = tiles / 2;
   p.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-  p.part = p.splits > 1 ? round_up((size_t)p.works * p.splits * fwd_rows(a, f32) * (a.D + 2) * 4, 256) : 256;
+  p.part = p.splits > 1 ? round_up((size_t)p.works * p.splits * fwd_rows(a, f32) * (a.D + 2) * 4, 256) : 0;
   return p;
 }
 static bool rows16(const void *p, const Str &s, int dtype) {
@@ -1157,7 +1157,7 @@ using namespace tcl;
 extern "C" size_t tcl_block_attention_fwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block,
                                                           int64_t q_block) {
   AttnArgs a{};
-  if (attn_setup(a, B, Nq, Nk, Hq, Hkv, D, top_k, block, q_block, 1.0, TCL_DT_F32) != TCL_OK) return 256;
+  if (attn_setup(a, B, Nq, Nk, Hq, Hkv, D, top_k, block, q_block, 1.0, TCL_DT_F32) != TCL_OK) return 0;
   const FwdPlan p = fwd_plan(a, true), q = fwd_plan(a, false);   // either type's
   return p.part > q.part ? p.part : q.part;
 }
@@ -1182,7 +1182,7 @@ extern "C" int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn
   a.chunks = plan.chunks;
   a.splits = plan.splits;
   const int64_t blocks_n = plan.works * a.splits;
-  TCL_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= plan.part, TCL_ERR_WORKSPACE, "block_attention: workspace of %zu bytes needed", plan.part);
+  TCL_REQUIRE(plan.part == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= plan.part), TCL_ERR_WORKSPACE, "block_attention: workspace of %zu bytes needed", plan.part);
   a.part = (float *)workspace;
   const hipStream_t s = (hipStream_t)stream;
   const int r = dtype == TCL_DT_F32 ? fwd_by_dim<float>(a, blocks_n, s) : dtype == TCL_DT_BF16 ? fwd_by_dim<__bf16>(a, blocks_n, s) : fwd_by_dim<_Float16>(a, blocks_n, s);

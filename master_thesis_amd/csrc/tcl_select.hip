@@ -455,9 +455,17 @@ extern "C" int tcl_block_means(const void *k, int64_t k_sb, int64_t k_sn, int64_
   return check_launch("block_means");
 }
 
-extern "C" size_t tcl_select_blocks_workspace_bytes(int64_t B, int64_t Hkv, int64_t S, int64_t nb, int64_t D) {
-  if (B <= 0 || Hkv <= 0 || S <= 0 || nb <= 0 || D <= 0) return 256;
-  return pooled_bytes(B, Hkv, S, D) + (nb <= kFusedBlocks ? 0 : round_up((size_t)(B * Hkv * S * nb) * sizeof(uint64_t), 256));
+// the choice without a score in memory, and its groups' sums formed where they are used
+static bool select_is_fused(int64_t nb) { return nb > 0 && nb <= kFusedBlocks; }
+static bool select_is_direct(int64_t N, int64_t H, int64_t Hkv, int64_t nb, int64_t q_block) {
+  return select_is_fused(nb) && (q_block < N ? q_block : N) * (H / Hkv) <= kDirectRows;
+}
+
+extern "C" size_t tcl_select_blocks_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t Hkv, int64_t D, int64_t nb, int64_t q_block) {
+  if (B <= 0 || N <= 0 || H <= 0 || Hkv <= 0 || D <= 0 || nb <= 0 || q_block <= 0) return 0;
+  const int64_t S = cdiv(N, q_block);
+  if (select_is_direct(N, H, Hkv, nb, q_block)) return 0;
+  return pooled_bytes(B, Hkv, S, D) + (select_is_fused(nb) ? 0 : round_up((size_t)(B * Hkv * S * nb) * sizeof(uint64_t), 256));
 }
 
 extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const float *means, const int32_t *counts, int32_t *blocks,
@@ -475,8 +483,8 @@ extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int6
   TCL_REQUIRE(aligned(q, 4 * size) && q_sb % 4 == 0 && q_sn % 4 == 0 && q_sh % 4 == 0 && aligned(means, 16), TCL_ERR_ARG,
               "select_blocks: query rows must start on 4 elements, means on 16 bytes");
   TCL_REQUIRE(rows < (1LL << 31) && B * Hkv < 65536 && cdiv(S, 16) < 65536, TCL_ERR_SHAPE, "select_blocks: %ld groups are too many for one call", (long)rows);
-  const size_t need = tcl_select_blocks_workspace_bytes(B, Hkv, S, nb, D);
-  TCL_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, TCL_ERR_WORKSPACE, "select_blocks: workspace of %zu bytes needed", need);
+  const size_t need = tcl_select_blocks_workspace_bytes(B, N, H, Hkv, D, nb, q_block);
+  TCL_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), TCL_ERR_WORKSPACE, "select_blocks: workspace of %zu bytes needed", need);
   SelectArgs a{q, means, counts, blocks, (double *)workspace, nullptr, q_sb, q_sn, q_sh, (int)B, (int)N, (int)H, (int)Hkv, (int)(H / Hkv), (int)D, (int)nb,
                (int)top_k, (int)q_block, (int)S};
   a.keys = (uint64_t *)((char *)workspace + pooled_bytes(B, Hkv, S, D));
@@ -484,7 +492,7 @@ extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int6
   a.by_g = make_fastdiv((uint32_t)a.G);
   const int64_t per_group = (q_block < N ? q_block : N) * a.G;
   TCL_REQUIRE(per_group < (1LL << 31), TCL_ERR_SHAPE, "select_blocks: groups of %ld query rows", (long)per_group);
-  const bool fused = nb > 0 && nb <= kFusedBlocks, direct = fused && per_group <= kDirectRows;
+  const bool fused = select_is_fused(nb), direct = select_is_direct(N, H, Hkv, nb, q_block);
   if (nb > 0 && !direct) {
     const dim3 pool((unsigned)cdiv(rows, 4));
     if (dtype == TCL_DT_F32) hipLaunchKernelGGL((select_pool_kernel<float>), pool, dim3(256), 0, s, a);

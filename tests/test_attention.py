@@ -145,12 +145,12 @@ def test_c_entries_refuse_without_gpu():
     means = lambda k=one, n=64, d=8, block=64, st=8: lib.tcl_block_means(k, 512, st, 8, None, one, one, 1, n, 1, d, block, 1, None)   # noqa: E731
     assert means(n=0) == 0 and means(d=12) == 5 and means(d=136) == 5 and means(block=96) == 5 and means(k=off) == 2 and means(st=12) == 2
     sel = lambda nb=4, top=1, d=8, hk=1, ws=one, wsb=1 << 20: lib.tcl_select_blocks(one, 16, 8, 8, one, one, one, 1, 2, 2, hk, d, nb, top, 1, 0, ws, wsb, None)   # noqa: E731
-    assert sel(nb=16385) == 5 and sel(top=0) == 1 and sel(hk=3) == 1 and sel(d=9) == 5 and sel(wsb=8) == 3 and sel(ws=None) == 3
-    fwd = lambda q=one, nk=64, d=8, top=1, block=64, qb=1, hk=1, wsb=1 << 20, dt=0, b=1: lib.tcl_block_attention_fwd(   # noqa: E731
+    assert sel(nb=16385) == 5 and sel(top=0) == 1 and sel(hk=3) == 1 and sel(d=9) == 5 and sel(nb=600, wsb=8) == 3 and sel(nb=600, ws=None) == 3
+    fwd = lambda q=one, nk=64, d=8, top=1, block=64, qb=1, hk=1, wsb=0, dt=0, b=1: lib.tcl_block_attention_fwd(   # noqa: E731
         q, 16, 8, 8, one, 512, 8, 8, one, 512, 8, 8, None, one, one, 16, 8, 8, None, b, 2, nk, 2, hk, d, top, block, qb, 1.0, dt, one, wsb, None)
     assert fwd(b=0) == 0
     assert fwd(d=4) == 5 and fwd(d=136) == 5 and fwd(top=2049) == 5 and fwd(block=32) == 5 and fwd(nk=64 * 65537) == 5 and fwd(dt=9) == 5
-    assert fwd(hk=3) == 1 and fwd(qb=0) == 1 and fwd(q=off) == 2 and fwd(q=None) == 2 and fwd(wsb=0) == 3
+    assert fwd(hk=3) == 1 and fwd(qb=0) == 1 and fwd(q=off) == 2 and fwd(q=None) == 2 and fwd(nk=1 << 16, top=100) == 3
     need = lib.tcl_block_attention_bwd_workspace_bytes(1, 2, 64, 2, 1, 8, 1, 64, 1)
     bwd = lambda wsb, go=one: lib.tcl_block_attention_bwd(go, 16, 8, 8, one, 16, 8, 8, one, 512, 8, 8, one, 512, 8, 8, None, one, one, 16, 8, 8, one,   # noqa: E731
                                                           None, 0, 0, 0, None, 0, 0, 0, None, 0, 0, 0, 1, 2, 64, 2, 1, 8, 1, 64, 1, 1.0, 0, one, wsb, None)
