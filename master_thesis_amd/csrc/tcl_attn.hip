@@ -69,7 +69,7 @@ struct AttnArgs {
   int B, Nq, Nk, Hq, Hkv, G, D, S, top, nb, lb, q_block, rows, chunks, splits, words, cap;
   float c;                         // scale * log2(e)
   float scale;
-  FastDiv by_g, by_rows;
+  FastDiv by_g, by_rows, by_d4;
 };
 
 // LDS image of token rows of DP channels: NCH chunks of 16 bytes per row (a power of two)
@@ -127,24 +127,37 @@ template <typename T, int DP, int ROWS> struct Pieces {
   __device__ __forceinline__ static char *dst(char *img, int u, int wave) { return img + (u * 256 + wave * 64) * 16; }
 };
 
-// ROWS rows that lie `st` bytes apart, from row `off` of the 64 that `mask` speaks of -> image; rows the mask leaves out and chunks
-// beyond `chunks` are zeros.  `base`, `st`, `mask`, `off` are uniform: a tile without holes costs no vector instruction but the loads.
+// Chunks beyond the head's channels (a head size that is not a multiple of 32) are zeroed once, by `images` images of ROWS rows, and
+// left alone by the loads, whose lanes for them stay idle.
+template <typename T, int DP, int ROWS> __device__ __forceinline__ void zero_pads(char *img, int images, int chunks, int wave) {
+  typedef Pieces<T, DP, ROWS> P;
+  if (chunks == P::I::NCH) return;
+  const uint4 zero = {0, 0, 0, 0};
+  for (int i = 0; i < images; ++i)
+#pragma unroll
+    for (int u = 0; u < P::NU; ++u)
+      if (P::any(u, wave) && P::chunk(u) >= chunks)
+        *reinterpret_cast<uint4 *>(img + (size_t)i * ROWS * P::I::RB + (u * 256 + (int)threadIdx.x) * 16) = zero;
+}
+
+// ROWS rows that lie `st` bytes apart, from row `off` of the 64 that `mask` speaks of -> image; rows the mask leaves out are zeros.
+// `base`, `st`, `mask`, `off` are uniform: a tile without holes costs no vector instruction but the loads.
 template <typename T, int DP, int ROWS> __device__ __forceinline__ void dma_segment(char *img, const char *base, unsigned st, uint64_t mask, int off, int chunks, int wave) {
   typedef Pieces<T, DP, ROWS> P;
   base += (size_t)((unsigned)off * st);
   mask >>= off;
   const uint64_t need = ROWS >= 64 ? ~0ull : (1ull << ROWS) - 1;
-  if ((mask & need) == need && chunks == DP / P::I::VE && P::I::NCH == DP / P::I::VE) {
+  if ((mask & need) == need) {
 #pragma unroll
     for (int u = 0; u < P::NU; ++u)
-      if (P::any(u, wave)) dma16(base + ((unsigned)P::row(u) * st + (unsigned)P::chunk(u) * 16), P::dst(img, u, wave));
+      if (P::any(u, wave) && P::chunk(u) < chunks) dma16(base + ((unsigned)P::row(u) * st + (unsigned)P::chunk(u) * 16), P::dst(img, u, wave));
   } else {
     const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
 #pragma unroll
     for (int u = 0; u < P::NU; ++u)
-      if (P::any(u, wave)) {
+      if (P::any(u, wave) && P::chunk(u) < chunks) {
         const uint32_t half = P::RPU > 32 ? (P::row(u) < 32 ? (uint32_t)mask : (uint32_t)(mask >> 32)) : u * P::RPU < 32 ? (uint32_t)mask : (uint32_t)(mask >> 32);
-        const bool in = ((half >> (P::row(u) & 31)) & 1) && P::chunk(u) < chunks;
+        const bool in = (half >> (P::row(u) & 31)) & 1;
         const char *p = base + ((unsigned)P::row(u) * st + (unsigned)P::chunk(u) * 16);
         dma16(in ? p : zero, P::dst(img, u, wave));
       }
@@ -162,9 +175,9 @@ template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type 
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
-// ... for a contraction over the 32 tokens from t0 (a multiple of 32): tokens t0 + 4 g .. + 3 and t0 + 16 + 4 g .. + 3 of channel
-// d0 + lane % 16, g = lane / 16
-template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type col_frag(const char *img, int t0, int d0, int lane) {
+// ... for a contraction over the 16 KU tokens from t0 (a multiple of 16): tokens t0 + 4 g .. + 3 and t0 + 16 + 4 g .. + 3 (KU = 1: zeros) of
+// channel d0 + lane % 16, g = lane / 16
+template <typename T, int DP, int KU = 2> __device__ __forceinline__ typename Vec8<T>::type col_frag(const char *img, int t0, int d0, int lane) {
   typedef Img<T, DP> I;
   const int g = lane / 16, col = lane % 16;
   if constexpr (sizeof(T) == 2) {
@@ -172,7 +185,8 @@ template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type 
     const int row = 4 * g + col / 4, p = col % 4;
     const char *a = img + (t0 + row) * I::RB + (((d0 / 8 + p / 2) ^ I::swz(row)) << 4) + (p % 2) * 8;
     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)a);
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(a + 16 * I::RB));
+    s16x4 y = {0, 0, 0, 0};
+    if constexpr (KU == 2) y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(a + 16 * I::RB));
     const s16x8 both = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(typename Vec8<T>::type, both);
   } else {
@@ -182,16 +196,34 @@ template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type 
       const int row = 4 * g + e;
       const char *a = img + (t0 + row) * I::RB + (((d0 / 4 + col / 4) ^ I::swz(row)) << 4) + (col % 4) * 4;
       r[e] = *reinterpret_cast<const float *>(a);
-      r[4 + e] = *reinterpret_cast<const float *>(a + 16 * I::RB);
+      r[4 + e] = KU == 2 ? *reinterpret_cast<const float *>(a + 16 * I::RB) : 0.f;
     }
     return r;
   }
 }
 
 // ------------------------------------------------------------------------------------------ the blocks of one group
-// blocks[0 .. top) of one group -> list[]: the valid indices, ascending, each once (a repeated index counts once, an index outside
-// [0, nb) is no block).  Through a bit per block; returns their number.  Called by the whole workgroup.
+// blocks[0 .. top) of one group -> list[]: the valid indices, each once (an index outside [0, nb) is no block).  A list that is
+// ascending with its invalid entries last, as select_blocks writes it, is taken as it is; any other goes through a bit per block.
+// Returns their number.  Called by the whole workgroup.
 __device__ __forceinline__ int group_blocks(const int32_t *blocks, int top, int nb, uint32_t *bits, int *list, int *n_out) {
+  int good = 1, mine = 0;
+  for (int i0 = 0; i0 < top; i0 += 256) {
+    const int i = i0 + (int)threadIdx.x;
+    const int j = i < top ? blocks[i] : -1, before = i < top && i > 0 ? blocks[i - 1] : -1;
+    const bool valid = j >= 0 && j < nb;
+    if (valid) {
+      good &= i == 0 || (before >= 0 && before < j);
+      if (i < min(top, nb)) list[i] = j;
+      ++mine;
+    }
+  }
+  if (threadIdx.x == 0) *n_out = 0;
+  if (__syncthreads_and(good)) {
+    if (mine) atomicAdd(n_out, mine);
+    __syncthreads();
+    return *n_out;
+  }
   const int words = (nb + 31) / 32;
   for (int i = threadIdx.x; i < words; i += 256) bits[i] = 0;
   __syncthreads();
@@ -245,24 +277,33 @@ struct KeySource {
     const int key = min(key0 + (int)(threadIdx.x & 63), nk - 1);
     return SegmentLoad{i < n ? key0 : -1, *(const __attribute__((address_space(1))) float *)(vis + (int64_t)key * vis_step)};
   }
+  // segment 0, which has to be waited for: without a mask nothing is loaded
+  __device__ __forceinline__ Segment first() const {
+    if (vis_step) return finish(load(0));
+    Segment s{__builtin_amdgcn_readfirstlane(list[0] << lb), 0};
+    s.mask = s.there(nk);
+    return s;
+  }
   __device__ __forceinline__ Segment finish(const SegmentLoad &l) const {
     return Segment{l.key0, l.key0 < 0 ? 0ull : __ballot(l.seen > 0.5f && l.key0 + (int)(threadIdx.x & 63) < nk)};
   }
 };
 
 // One workgroup: M = 16 NQ WM query rows of one group (a row = one query token and one head of the key head's group), 4 waves as WM
-// row sets x WN key sets.  The group's keys pass as one stream in tiles of TK = 32 WN; every wave keeps its own running maximum, sum
-// and output for its 32 keys of each tile, joined at the end, so the only meeting of the waves in the loop is the hand-over of the tile.
-template <typename T, int DP, int NQ, int WM, int WN> struct FwdTile {
-  static constexpr int M = 16 * NQ * WM, TK = 32 * WN, NS = TK > 64 ? TK / 64 : 1;
+// row sets x WN key sets.  The group's keys pass as one stream in tiles of TK = 16 KU WN (up to a segment); every wave keeps its own
+// running maximum, sum and output for its 16 KU keys of each tile, joined at the end, so the only meeting of the waves in the loop is
+// the hand-over of the tile.
+template <typename T, int DP, int NQ, int WM, int WN, int KU> struct FwdTile {
+  static constexpr int M = 16 * NQ * WM, TK = 16 * KU * WN, LO = DP + 4;
   static constexpr size_t img = (size_t)TK * Img<T, DP>::RB, tiles = 4 * img;          // K and V, twice
-  static constexpr size_t join = (size_t)M * (DP + 4) * 4 + (size_t)WN * M * 8;
+  static constexpr size_t join = (size_t)WN * M * (LO + 2) * 4;                        // outputs, maxima and sums of the key sets
   static constexpr size_t body = tiles > join ? tiles : join;
 };
-template <typename T, int DP, int NQ, int WM, int WN, int OCC>
+template <typename T, int DP, int NQ, int WM, int WN, int KU, int OCC>
 __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
-  typedef FwdTile<T, DP, NQ, WM, WN> F;
-  constexpr int M = F::M, TK = F::TK, NS = F::NS, KC = DP / 32, DT = DP / 16;
+  typedef FwdTile<T, DP, NQ, WM, WN, KU> F;
+  constexpr int M = F::M, TK = F::TK, KC = DP / 32, DT = DP / 16;
+  static_assert(TK <= 64, "one segment per tile");
   typedef typename Vec8<T>::type frag;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int *list = reinterpret_cast<int *>(smem + F::body);
@@ -280,15 +321,6 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
   const int s = (int)(item % a.S);
   const int bh = (int)(item / a.S), hk = bh % a.Hkv, b = bh / a.Hkv;
 
-  const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + s) * a.top, a.top, a.nb, bits, list, &n_list);
-  const int e0 = (int)((int64_t)n * split / a.splits), e1 = (int)((int64_t)n * (split + 1) / a.splits);
-  const KeySource keys{list + e0, a.vis ? a.vis + (int64_t)b * a.Nk : &g_one, a.vis != nullptr, (e1 - e0) << (a.lb - 6), a.lb, a.Nk};
-  const int nt = (keys.n * 64 + TK - 1) / TK;
-  const char *kb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h);
-  const char *vb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h);
-  const int chunks = a.D / Img<T, DP>::VE;
-  const unsigned kst = (unsigned)(a.sk.n * sizeof(T)), vst = (unsigned)(a.sv.n * sizeof(T));   // host: 128 rows stay below 2^31
-
   // row r of the group: token q_block * s + r / G, head hk * G + r % G
   auto row_of = [&](int m, int &token, int &head) {
     const int r = chunk * M + m;
@@ -297,36 +329,8 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     head = hk * a.G + (r - t * a.G);
     return r < a.rows && token < a.Nq;
   };
-  auto seg_load = [&](int t, SegmentLoad *r) {
-#pragma unroll
-    for (int i = 0; i < NS; ++i) r[i] = keys.load(t * TK / 64 + i);
-  };
-  auto issue = [&](int t, const Segment *sg) {
-    char *kd = smem + (t & 1) * 2 * F::img, *vd = kd + F::img;
-    constexpr int R = TK < 64 ? TK : 64;
-    const int off = TK < 64 ? (t * TK) & 63 : 0;                 // within the segment
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      // a hidden key's score is overwritten, so its row may be anything; its value row is multiplied by a probability of 0
-      dma_segment<T, DP, R>(kd + i * 64 * Img<T, DP>::RB, kb + (int64_t)sg[i].key0 * a.sk.n * (int64_t)sizeof(T), kst, sg[i].there(a.Nk), off, chunks, wave);
-      dma_segment<T, DP, R>(vd + i * 64 * Img<T, DP>::RB, vb + (int64_t)sg[i].key0 * a.sv.n * (int64_t)sizeof(T), vst, sg[i].mask, off, chunks, wave);
-    }
-  };
-
-  Segment cur[NS] = {}, nxt[NS] = {};
-  SegmentLoad raw[NS] = {};
-  if (nt > 0) {
-    seg_load(0, raw);
-#pragma unroll
-    for (int i = 0; i < NS; ++i) cur[i] = keys.finish(raw[i]);
-    issue(0, cur);
-    seg_load(1, raw);
-  }
-
-  // the queries, as columns; a negative scale turns their sign, so that the largest product is the largest score
+  // the queries, as columns (asked for first, so that they arrive while the list is made)
   frag qf[NQ][KC];
-  const bool neg = a.c < 0.f;
-  const float sc2 = fmaxf(fabsf(a.c), 1e-30f);                   // not 0: -inf times it has to stay -inf
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     int token, head;
@@ -337,8 +341,39 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
       const int ch = c * 32 + g * 8;
       frag t = {};
       if (ok && ch < a.D) t = *reinterpret_cast<const frag *>(p + ch);
-      qf[i][c] = neg ? -t : t;
+      qf[i][c] = t;
     }
+  }
+  const int chunks = a.D / Img<T, DP>::VE;
+  zero_pads<T, DP, TK>(smem, 4, chunks, wave);
+  const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + s) * a.top, a.top, a.nb, bits, list, &n_list);
+  const int e0 = (int)((int64_t)n * split / a.splits), e1 = (int)((int64_t)n * (split + 1) / a.splits);
+  const KeySource keys{list + e0, a.vis ? a.vis + (int64_t)b * a.Nk : &g_one, a.vis != nullptr, (e1 - e0) << (a.lb - 6), a.lb, a.Nk};
+  const int nt = keys.n * 64 / TK;
+  const char *kb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h);
+  const char *vb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h);
+  const unsigned kst = (unsigned)(a.sk.n * sizeof(T)), vst = (unsigned)(a.sv.n * sizeof(T));   // host: 128 rows stay below 2^31
+  auto issue = [&](int t, const Segment &x) {
+    char *kd = smem + (t & 1) * 2 * F::img, *vd = kd + F::img;
+    const int off = (t * TK) & 63;                               // within the segment
+    // a hidden key's score is overwritten, so its row may be anything; its value row is multiplied by a probability of 0
+    dma_segment<T, DP, TK>(kd, kb + (int64_t)x.key0 * a.sk.n * (int64_t)sizeof(T), kst, x.there(a.Nk), off, chunks, wave);
+    dma_segment<T, DP, TK>(vd, vb + (int64_t)x.key0 * a.sv.n * (int64_t)sizeof(T), vst, x.mask, off, chunks, wave);
+  };
+  Segment cur = {}, nxt = {};
+  SegmentLoad raw = {};
+  if (nt > 0) {
+    cur = keys.first();
+    issue(0, cur);
+    raw = keys.load(TK / 64);
+  }
+  // a negative scale turns the queries' sign, so that the largest product is the largest score
+  const float sc2 = fmaxf(fabsf(a.c), 1e-30f);                   // not 0: -inf times it has to stay -inf
+  if (a.c < 0.f) {
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) qf[i][c] = -qf[i][c];
   }
   f32x4 o[NQ][DT];
   float m[NQ], l[NQ];                                            // maximum in log2 units, sum of exp2(score - maximum)
@@ -349,24 +384,23 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-#pragma unroll
-  for (int i = 0; i < NS; ++i) nxt[i] = keys.finish(raw[i]);
+  if (nt > 0) nxt = keys.finish(raw);
   for (int t = 0; t < nt; ++t) {
-    tile_barrier<0>();                                              // tile t is there, tile t - 1 has been read
+    tile_barrier<0>();                                           // tile t is there, tile t - 1 has been read
     if (t + 1 < nt) issue(t + 1, nxt);
-    seg_load(t + 2, raw);
+    raw = keys.load((t + 2) * TK / 64);
     const char *krows = smem + (t & 1) * 2 * F::img, *vrows = krows + F::img;
     // all fragments of a product are asked for before its first step, those of the second product before the softmax: an LDS read
     // takes longer than a product, and there are only a few waves to hide it behind
-    frag kf[2][KC];
+    frag kf[KU][KC];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < KU; ++u)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) kf[u][c] = row_frag<T, DP>(krows, wn * 32 + u * 16 + col, c * 32 + g * 8);
+      for (int c = 0; c < KC; ++c) kf[u][c] = row_frag<T, DP>(krows, (wn * KU + u) * 16 + col, c * 32 + g * 8);
     __builtin_amdgcn_sched_barrier(0);
-    f32x4 sc[2][NQ];
+    f32x4 sc[KU][NQ];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < KU; ++u) {
 #pragma unroll
       for (int i = 0; i < NQ; ++i) sc[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -377,13 +411,12 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     constexpr int AH = sizeof(T) == 2 ? DT : DT / 2;             // fp32 fragments are twice as large, and their products 16 times as long
     frag vf[AH];
 #pragma unroll
-    for (int d = 0; d < AH; ++d) vf[d] = col_frag<T, DP>(vrows, wn * 32, d * 16, lane);
+    for (int d = 0; d < AH; ++d) vf[d] = col_frag<T, DP, KU>(vrows, wn * KU * 16, d * 16, lane);
     __builtin_amdgcn_sched_barrier(0);
-    const uint64_t mask = cur[wn * 32 / 64 % NS].mask;
-    if (mask != ~0ull) {
-      const unsigned seen = (unsigned)(mask >> ((TK < 64 ? (t * TK) & 63 : wn * 32 & 63) + g * 4));
+    if (cur.mask != ~0ull) {
+      const unsigned seen = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * KU * 16 + g * 4));
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < KU; ++u)
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
 #pragma unroll
@@ -396,7 +429,7 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     for (int i = 0; i < NQ; ++i) {
       float mx = max2(sc[0][i][0], sc[0][i][1]);
 #pragma unroll
-      for (int e = 2; e < 8; ++e) mx = max2(mx, sc[e / 4][i][e % 4]);
+      for (int e = 2; e < 4 * KU; ++e) mx = max2(mx, sc[e / 4][i][e % 4]);
       mx = quarter_max(mx);
       const float mn = max2(m[i], mx * sc2);
       const float ms = mn == kNegInf ? 0.f : mn;                 // nothing seen yet: exp2(-inf - 0) = 0
@@ -405,13 +438,15 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
       m[i] = mn;
       float sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i][e], sc2, -ms));
-          sum += p;
-          pf[i][u * 4 + e] = (T)p;
+      for (int e = 0; e < 8; ++e) {
+        if (e >= 4 * KU) {
+          pf[i][e] = (T)0.f;
+          continue;
         }
+        const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / 4 % KU][i][e % 4], sc2, -ms));
+        sum += p;
+        pf[i][e] = (T)p;
+      }
       l[i] = fmaf(l[i], f[i], sum);
     }
     if (__any(grew)) {                                           // no maximum moved in most tiles behind the first ones
@@ -422,67 +457,50 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const frag v = d < AH ? vf[d % AH] : col_frag<T, DP>(vrows, wn * 32, d * 16, lane);
+      const frag v = d < AH ? vf[d % AH] : col_frag<T, DP, KU>(vrows, wn * KU * 16, d * 16, lane);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) o[i][d] = mma(v, pf[i], o[i][d]);
     }
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      cur[i] = nxt[i];
-      nxt[i] = keys.finish(raw[i]);
-    }
+    cur = nxt;
+    nxt = keys.finish(raw);
   }
 
-  // join the key sets: common maximum, then the outputs added up in LDS in wave order
-  float *jo = reinterpret_cast<float *>(smem);                   // [M][DP + 4]
-  float *jm = jo + M * (DP + 4), *jl = jm + WN * M;              // [WN][M] each
+  // join the key sets: every wave leaves its output, maximum and sum, and a thread adds them up under the common maximum
+  float *jo = reinterpret_cast<float *>(smem);                   // [WN][M][LO]
+  float *jm = jo + WN * M * F::LO, *jl = jm + WN * M;            // [WN][M] each
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
+    const int r = wn * M + (wm * NQ + i) * 16 + col;
     l[i] += __shfl_xor(l[i], 16, 64);
     l[i] += __shfl_xor(l[i], 32, 64);
     if (g == 0) {
-      jm[wn * M + (wm * NQ + i) * 16 + col] = m[i];
-      jl[wn * M + (wm * NQ + i) * 16 + col] = l[i];
+      jm[r] = m[i];
+      jl[r] = l[i];
     }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(jo + r * F::LO + d * 16 + g * 4) = o[i][d];
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WN; ++w) {
-    if (wn == w) {
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        const int r = (wm * NQ + i) * 16 + col;
-        float mx = kNegInf;
-#pragma unroll
-        for (int x = 0; x < WN; ++x) mx = fmaxf(mx, jm[x * M + r]);
-        const float f = mx == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[i] - mx);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          f32x4 *p = reinterpret_cast<f32x4 *>(jo + r * (DP + 4) + d * 16 + g * 4);
-          const f32x4 x = o[i][d] * f;
-          *p = w == 0 ? x : *p + x;
-        }
-      }
-    }
-    __syncthreads();
-  }
   // write out: rows of D channels, 4 per thread
   float *pm = a.splits > 1 ? a.part + ((int64_t)work * a.splits + split) * M * (a.D + 2) : nullptr;
-  const int per = a.D / 4;
-  for (int id = tid; id < M * per; id += 256) {
-    const int r = id / per, ch = (id - r * per) * 4;
+  for (int id = tid; id < M * (a.D / 4); id += 256) {
+    const int r = (int)a.by_d4.div((unsigned)id), ch = (id - r * (a.D / 4)) * 4;
     int token, head;
     if (!row_of(r, token, head)) continue;
     float mx = kNegInf, sum = 0.f;
 #pragma unroll
     for (int x = 0; x < WN; ++x) mx = fmaxf(mx, jm[x * M + r]);
+    f32x4 x4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < WN; ++x) sum += mx == kNegInf ? 0.f : jl[x * M + r] * __builtin_amdgcn_exp2f(jm[x * M + r] - mx);
-    const f32x4 x = *reinterpret_cast<const f32x4 *>(jo + r * (DP + 4) + ch);
+    for (int x = 0; x < WN; ++x) {
+      const float f = mx == kNegInf ? 0.f : __builtin_amdgcn_exp2f(jm[x * M + r] - mx);
+      sum += mx == kNegInf ? 0.f : jl[x * M + r] * f;
+      x4 += *reinterpret_cast<const f32x4 *>(jo + (x * M + r) * F::LO + ch) * f;
+    }
     if (pm) {
-      *reinterpret_cast<f32x4 *>(pm + (int64_t)r * a.D + ch) = x;
+      *reinterpret_cast<f32x4 *>(pm + (int64_t)r * a.D + ch) = x4;
       if (ch == 0) {
         pm[(int64_t)M * a.D + r] = mx;
         pm[(int64_t)M * a.D + M + r] = sum;
@@ -492,7 +510,7 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // nothing seen: zero; NaN stays NaN
     typename Vec4<T>::type y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
+    for (int e = 0; e < 4; ++e) y[e] = (T)(x4[e] * inv);
     *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.out) + (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch) = y;
     if (ch == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx + __builtin_log2f(sum)) * kLn2;
   }
@@ -645,12 +663,13 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   item /= a.chunks;
   const int s = (int)(item % a.S);
   const int bh = (int)(item / a.S), hk = bh % a.Hkv, b = bh / a.Hkv;
+  const int chunks = a.D / Img<T, DP>::VE;
+  zero_pads<T, DP, TK>(smem, 4, chunks, wave);
   const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + s) * a.top, a.top, a.nb, bits, list, &n_list);
   const KeySource keys{list, a.vis ? a.vis + (int64_t)b * a.Nk : &g_one, a.vis != nullptr, n << (a.lb - 6), a.lb, a.Nk};
   const int nt = keys.n * 64 / TK;
   const char *kb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h);
   const char *vb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h);
-  const int chunks = a.D / Img<T, DP>::VE;
   const unsigned kst = (unsigned)(a.sk.n * sizeof(T)), vst = (unsigned)(a.sv.n * sizeof(T));
   auto row_of = [&](int m, int &token, int &head) {
     const int r = chunk * M + m;
@@ -668,7 +687,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   Segment cur = {}, nxt = {};
   SegmentLoad raw = {};
   if (nt > 0) {
-    cur = keys.finish(keys.load(0));
+    cur = keys.first();
     issue(0, cur);
     raw = keys.load(TK / 64);
   }
@@ -706,7 +725,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   for (int i = 0; i < NQ; ++i)
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  nxt = keys.finish(raw);
+  if (nt > 0) nxt = keys.finish(raw);
   for (int t = 0; t < nt; ++t) {
     tile_barrier<0>();
     if (t + 1 < nt) issue(t + 1, nxt);
@@ -784,9 +803,8 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     }
     __syncthreads();
   }
-  const int per = a.D / 4;
-  for (int id = tid; id < M * per; id += 256) {
-    const int r = id / per, ch = (id - r * per) * 4;
+  for (int id = tid; id < M * (a.D / 4); id += 256) {
+    const int r = (int)a.by_d4.div((unsigned)id), ch = (id - r * (a.D / 4)) * 4;
     int token, head;
     if (!row_of(r, token, head)) continue;
     const f32x4 x = *reinterpret_cast<const f32x4 *>(jo + r * (DP + 4) + ch) * (sizeof(T) == 2 && PScale<T>::bits > 0.f ? 1.f : a.scale);
@@ -861,6 +879,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
   f32x4 gk[DT], gv[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) gk[d] = gv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  zero_pads<T, DP, TR>(smem, 2 * NB, chunks, wave);
 
   for (int w0 = 0; w0 < a.words; w0 += kWindow) {
     __syncthreads();                                             // the last window's list has been read
@@ -920,9 +939,12 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
 #pragma unroll
         for (int u = 0; u < P::NU; ++u)
           if (P::any(u, wave)) {
-            const bool in = x[u].x != ~0u && P::chunk(u) < chunks;
-            dma16(in ? qb + ((uint64_t)x[u].x + P::chunk(u)) * 16 : zero, P::dst(qd, u, wave));
-            dma16(in ? db + ((uint64_t)x[u].y + P::chunk(u)) * 16 : zero, P::dst(dd, u, wave));
+            const bool in = x[u].x != ~0u;
+            const char *p = in ? qb + ((uint64_t)x[u].x + P::chunk(u)) * 16 : zero, *q = in ? db + ((uint64_t)x[u].y + P::chunk(u)) * 16 : zero;
+            if (P::chunk(u) < chunks) {
+              dma16(p, P::dst(qd, u, wave));
+              dma16(q, P::dst(dd, u, wave));
+            }
           }
       };
 #pragma unroll
@@ -1033,12 +1055,13 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------ host
-// Tile shapes.  16-bit: 64 rows x 64 keys as 2 x 2 waves of 32 x 32 (every LDS fragment feeds two products); groups of up to 16 rows (one
-// token of a few heads) take 16 rows x 128 keys, the four waves sharing out the keys.  fp32, whose products take 16 times as long
-// per fragment: 64 rows x 32 keys as 4 x 1 waves of 16 x 32, few rows (up to 32) x 64 keys.
-constexpr int few_rows(bool f32) { return f32 ? 32 : 16; }
-static int fwd_rows(const AttnArgs &a, bool f32) { return a.rows <= few_rows(f32) ? few_rows(f32) : 64; }
-static int fwd_keys(const AttnArgs &a, bool f32) { return a.rows <= few_rows(f32) ? (f32 ? 64 : 128) : (f32 ? 32 : 64); }
+// Tile shapes.  16-bit: 64 rows x 64 keys as 2 x 2 waves of 32 x 32 (every LDS fragment feeds two products); fp32, whose products take 16
+// times as long per fragment: 64 rows x 32 keys as 4 x 1 waves of 16 x 32.  Groups of up to 16 rows (one token of a few heads) take
+// 16 rows x 64 keys, the four waves sharing out the keys by 16: half of the second product's slots stay empty there, but such
+// calls wait for memory, and two workgroups fit a CU (against 128 keys a tile, 32 a wave: TBD).
+constexpr int kFewRows = 16;
+static int fwd_rows(const AttnArgs &a) { return a.rows <= kFewRows ? 16 : 64; }
+static int fwd_keys(const AttnArgs &a, bool f32) { return a.rows > kFewRows && f32 ? 32 : 64; }
 
 static size_t list_bytes(const AttnArgs &a) { return (size_t)a.cap * 4 + (size_t)(a.nb + 31) / 32 * 4; }
 
@@ -1050,14 +1073,9 @@ template <typename K> static int launch(K kernel, size_t lds, int64_t blocks, co
 }
 template <typename T, int DP> static int launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t s) {
   const char *what = "block_attention";
-  const bool few = a.rows <= few_rows(sizeof(T) == 4);
-  if constexpr (sizeof(T) == 4) {
-    if (few) return launch(attend_fwd_kernel<T, DP, 1, 2, 2, 1>, FwdTile<T, DP, 1, 2, 2>::body + list_bytes(a), blocks, a, s, what);
-    return launch(attend_fwd_kernel<T, DP, 1, 4, 1, 2>, FwdTile<T, DP, 1, 4, 1>::body + list_bytes(a), blocks, a, s, what);
-  } else {
-    if (few) return launch(attend_fwd_kernel<T, DP, 1, 1, 4, 1>, FwdTile<T, DP, 1, 1, 4>::body + list_bytes(a), blocks, a, s, what);
-    return launch(attend_fwd_kernel<T, DP, 2, 2, 2, 2>, FwdTile<T, DP, 2, 2, 2>::body + list_bytes(a), blocks, a, s, what);
-  }
+  if (a.rows <= kFewRows) return launch(attend_fwd_kernel<T, DP, 1, 1, 4, 1, 2>, FwdTile<T, DP, 1, 1, 4, 1>::body + list_bytes(a), blocks, a, s, what);
+  if constexpr (sizeof(T) == 4) return launch(attend_fwd_kernel<T, DP, 1, 4, 1, 2, 2>, FwdTile<T, DP, 1, 4, 1, 2>::body + list_bytes(a), blocks, a, s, what);
+  else return launch(attend_fwd_kernel<T, DP, 2, 2, 2, 2, 2>, FwdTile<T, DP, 2, 2, 2, 2>::body + list_bytes(a), blocks, a, s, what);
 }
 template <typename T, int DP> static int launch_dq(AttnArgs a, hipStream_t s) {
   const char *what = "block_attention backward (queries)";
@@ -1118,6 +1136,7 @@ static int attn_setup(AttnArgs &a, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq
   a.words = (int)cdiv(a.S, 32);
   a.by_g = make_fastdiv((uint32_t)a.G);
   a.by_rows = make_fastdiv((uint32_t)a.rows);
+  a.by_d4 = make_fastdiv((uint32_t)(a.D / 4));
   a.scale = (float)scale;
   a.c = (float)(scale * 1.4426950408889634074);
   a.chunks = 1;
@@ -1129,13 +1148,13 @@ static int attn_setup(AttnArgs &a, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq
 struct FwdPlan { int chunks, splits; int64_t works; size_t part; };
 static FwdPlan fwd_plan(const AttnArgs &a, bool f32) {
   FwdPlan p;
-  p.chunks = (int)cdiv(a.rows, fwd_rows(a, f32));
+  p.chunks = (int)cdiv(a.rows, fwd_rows(a));
   p.works = (int64_t)a.B * a.Hkv * a.S * p.chunks;
   const int64_t tiles = cdiv((int64_t)a.cap << a.lb, fwd_keys(a, f32));
   int64_t n = cdiv(2 * kNumCU, p.works > 0 ? p.works : 1);
   if (n > tiles / 2) n = tiles / 2;
   p.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-  p.part = p.splits > 1 ? round_up((size_t)p.works * p.splits * fwd_rows(a, f32) * (a.D + 2) * 4, 256) : 0;
+  p.part = p.splits > 1 ? round_up((size_t)p.works * p.splits * fwd_rows(a) * (a.D + 2) * 4, 256) : 0;
   return p;
 }
 static bool rows16(const void *p, const Str &s, int dtype) {
@@ -1187,7 +1206,7 @@ extern "C" int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn
   const hipStream_t s = (hipStream_t)stream;
   const int r = dtype == TCL_DT_F32 ? fwd_by_dim<float>(a, blocks_n, s) : dtype == TCL_DT_BF16 ? fwd_by_dim<__bf16>(a, blocks_n, s) : fwd_by_dim<_Float16>(a, blocks_n, s);
   if (r != TCL_OK || a.splits == 1) return r;
-  const int M = fwd_rows(a, f32);
+  const int M = fwd_rows(a);
   TCL_REQUIRE(plan.works * M < (1LL << 31), TCL_ERR_SHAPE, "block_attention: too many rows for one call");
   const dim3 grid((unsigned)(plan.works * M));
   if (dtype == TCL_DT_F32) hipLaunchKernelGGL((attend_join_kernel<float>), grid, dim3(256), 0, s, a, M);
