@@ -3,10 +3,10 @@
 //   out_q = sum_n softmax_n(scale <q, k_n>) v_n   over the visible keys n of the blocks chosen for q's group
 //   (0, and lse = -inf, where nothing is visible).
 //
-// All products run on the matrix pipe in one shape, 16 x 16 with 32 k-elements per step (one v_mfma_f32_16x16x32 for 16-bit
-// operands, eight v_mfma_f32_16x16x4_f32 for fp32): lane l holds row (column) l % 16 of an operand and 8 k-elements of the quarter
-// l / 16; the result has column l % 16 and rows 4 (l / 16) .. + 3.  The order of the k-elements is free as long as both operands
-// share it, and that is what keeps the probabilities in registers: S^T = K Q^T leaves a lane 4 + 4 probabilities of ITS query (two
+// All products run on the matrix pipe, 16 x 16 with 32 k-elements per step (one v_mfma_f32_16x16x32 for 16-bit operands, eight
+// v_mfma_f32_16x16x4_f32 for fp32): lane l holds row (column) l % 16 of an operand and 8 k-elements of the quarter l / 16; the result
+// has column l % 16 and rows 4 (l / 16) .. + 3 (32 x 32 with 16 k-elements where a wave's tile allows: half the instructions, and one
+// softmax row per lane instead of two).  The order of the k-elements is free as long as both operands share it, and that is what keeps the probabilities in registers: S^T = K Q^T leaves a lane 4 + 4 probabilities of ITS query (two
 // 16-key tiles), which are, as they are, the second operand of O^T = V^T P^T once V^T is read in the same key order: for 16-bit
 // types with the transposing LDS read, for fp32 element by element.  So every tensor has ONE image in LDS, rows as they lie in
 // memory, for contractions over channels and over tokens alike.
@@ -28,6 +28,8 @@ typedef float f32x8 __attribute__((ext_vector_type(8), aligned(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
 template <typename T> struct Vec8;
 template <> struct Vec8<float> { typedef f32x8 type; };
 template <> struct Vec8<__bf16> { typedef bf16x8 type; };
@@ -41,6 +43,25 @@ __device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
   for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
   return c;
 }
+
+// the same 32 x 32 with 16 k-elements: lane l holds row (column) l % 32 and 8 k-elements of the half l / 32, and gets column l % 32, rows
+// 8 j + 4 (l / 32) .. + 3
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// The two shapes: S x S products of KS k-elements, AE results per lane.  Result e of a lane in quarter (half) q = lane / S is row
+// row(e) + 4 q of the tile.
+template <int S> struct Shape;
+template <> struct Shape<16> {
+  typedef f32x4 acc;
+  static constexpr int KS = 32, AE = 4;
+  static constexpr int row(int e) { return e; }
+};
+template <> struct Shape<32> {
+  typedef f32x16 acc;
+  static constexpr int KS = 16, AE = 16;
+  static constexpr int row(int e) { return e / 4 * 8 + e % 4; }
+};
 
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kPosInf = __builtin_inff();
@@ -87,6 +108,7 @@ template <typename T, int DP> struct Img {
 
 typedef __attribute__((address_space(3))) void *lds_vptr;
 typedef const __attribute__((address_space(1))) void *glb_cvptr;
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -96,21 +118,24 @@ static __device__ __attribute__((aligned(16))) const uint32_t g_zero_chunk[4] = 
 __device__ __forceinline__ void dma16(const char *src, char *lds) {   // lds: of the wave's first lane
   __builtin_amdgcn_global_load_lds((glb_cvptr)src, (lds_vptr)lds, 16, 0, 0);
 }
-// maximum without the quieting instructions of fmaxf (a NaN may come out as the other operand, as it may there)
-__device__ __forceinline__ float max2(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, kPosInf); }
-// maximum over lanes l, l ^ 16, l ^ 32, l ^ 48: the swaps leave rows (halves) of both halves in both operands
-__device__ __forceinline__ float quarter_max(float x) {
-  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-  const unsigned u = __float_as_uint(x);
-  const u32x2 a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const float y = max2(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const unsigned w = __float_as_uint(y);
+// Maxima that hand on a NaN (one instruction for three operands; fmaxf, which does not, takes two for two): a row that sees a NaN is NaN
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// maximum over the lanes that hold the same column of an S x S result: the swaps leave rows (halves) of both halves in both operands
+template <int S> __device__ __forceinline__ float column_max(float x) {
+  if constexpr (S == 16) {
+    const unsigned u = __float_as_uint(x);
+    const u32x2 a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = max2(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+  const unsigned w = __float_as_uint(x);
   const u32x2 b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
   return max2(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 // all but the last N LDS-DMAs of this wave have landed and every LDS read of it has been served; then the workgroup meets
+// (by the builtin: a wait in inline assembly is unknown to the compiler, which then waits again, for the tile that is on its way)
 template <int N> __device__ __forceinline__ void tile_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);   // vmcnt(N) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -175,28 +200,32 @@ template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type 
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
-// ... for a contraction over the 16 KU tokens from t0 (a multiple of 16): tokens t0 + 4 g .. + 3 and t0 + 16 + 4 g .. + 3 (KU = 1: zeros) of
-// channel d0 + lane % 16, g = lane / 16
-template <typename T, int DP, int KU = 2> __device__ __forceinline__ typename Vec8<T>::type col_frag(const char *img, int t0, int d0, int lane) {
+// ... for a contraction over tokens, in the order in which a lane holds the results of an S x S product: channel d0 + lane % S, and
+//   S = 16: of the 32 tokens from t0, tokens t0 + 4 q .. + 3 and t0 + 16 + 4 q .. + 3 (HALF: 16 tokens, the second four are zeros)
+//   S = 32: of the 16 tokens from t0, tokens t0 + 4 q .. + 3 and t0 + 8 + 4 q .. + 3
+// with q = lane / S; t0 is a multiple of 16.
+template <typename T, int DP, int S = 16, bool HALF = false> __device__ __forceinline__ typename Vec8<T>::type col_frag(const char *img, int t0, int d0, int lane) {
   typedef Img<T, DP> I;
-  const int g = lane / 16, col = lane % 16;
+  const int q = lane / S, col = lane % 16;
+  constexpr int SECOND = S == 16 ? 16 : 8;
   if constexpr (sizeof(T) == 2) {
-    // transposing read: lane 4 q + p of a group of 16 points at row q, elements 4 p .. + 3 of a 4 x 16 block and gets column lane % 16 of it
-    const int row = 4 * g + col / 4, p = col % 4;
-    const char *a = img + (t0 + row) * I::RB + (((d0 / 8 + p / 2) ^ I::swz(row)) << 4) + (p % 2) * 8;
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)a);
+    // transposing read: lane 4 r + p of a group of 16 points at row r, elements 4 p .. + 3 of a 4 x 16 block and gets column lane % 16 of it
+    const int row = 4 * q + col / 4, p = col % 4, ch = (d0 + (S == 32 ? lane / 16 % 2 * 16 : 0)) / 8 + p / 2;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(img + (t0 + row) * I::RB + ((ch ^ I::swz(row)) << 4) + (p % 2) * 8));
     s16x4 y = {0, 0, 0, 0};
-    if constexpr (KU == 2) y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(a + 16 * I::RB));
+    if constexpr (!HALF)
+      y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(img + (t0 + row + SECOND) * I::RB + ((ch ^ I::swz(row + SECOND)) << 4) + (p % 2) * 8));
     const s16x8 both = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(typename Vec8<T>::type, both);
   } else {
+    static_assert(S == 16, "fp32 products are 16 x 16");
     f32x8 r;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int row = 4 * g + e;
+      const int row = 4 * q + e;
       const char *a = img + (t0 + row) * I::RB + (((d0 / 4 + col / 4) ^ I::swz(row)) << 4) + (col % 4) * 4;
       r[e] = *reinterpret_cast<const float *>(a);
-      r[4 + e] = KU == 2 ? *reinterpret_cast<const float *>(a + 16 * I::RB) : 0.f;
+      r[4 + e] = HALF ? 0.f : *reinterpret_cast<const float *>(a + 16 * I::RB);
     }
     return r;
   }
@@ -289,28 +318,30 @@ struct KeySource {
   }
 };
 
-// One workgroup: M = 16 NQ WM query rows of one group (a row = one query token and one head of the key head's group), 4 waves as WM
-// row sets x WN key sets.  The group's keys pass as one stream in tiles of TK = 16 KU WN (up to a segment); every wave keeps its own
-// running maximum, sum and output for its 16 KU keys of each tile, joined at the end, so the only meeting of the waves in the loop is
+// One workgroup: M = S WM query rows of one group (a row = one query token and one head of the key head's group), 4 waves as WM row
+// sets x WN key sets.  The group's keys pass as one stream in tiles of TK = S KU WN (up to a segment); every wave keeps its own
+// running maximum, sum and output for its S KU keys of each tile, joined at the end, so the only meeting of the waves in the loop is
 // the hand-over of the tile.
-template <typename T, int DP, int NQ, int WM, int WN, int KU> struct FwdTile {
-  static constexpr int M = 16 * NQ * WM, TK = 16 * KU * WN, LO = DP + 4;
+template <typename T, int DP, int S, int WM, int WN, int KU> struct FwdTile {
+  static constexpr int M = S * WM, TK = S * KU * WN, LO = DP + 4;
   static constexpr size_t img = (size_t)TK * Img<T, DP>::RB, tiles = 4 * img;          // K and V, twice
   static constexpr size_t join = (size_t)WN * M * (LO + 2) * 4;                        // outputs, maxima and sums of the key sets
   static constexpr size_t body = tiles > join ? tiles : join;
 };
-template <typename T, int DP, int NQ, int WM, int WN, int KU, int OCC>
-__global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
-  typedef FwdTile<T, DP, NQ, WM, WN, KU> F;
-  constexpr int M = F::M, TK = F::TK, KC = DP / 32, DT = DP / 16;
+template <typename T, int DP, int S, int WM, int WN, int KU>
+__global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
+  typedef FwdTile<T, DP, S, WM, WN, KU> F;
+  typedef Shape<S> H;
+  constexpr int M = F::M, TK = F::TK, KC = DP / H::KS, DT = DP / S, E = H::AE * KU, PF = (E + 7) / 8;   // E: scores per lane
   static_assert(TK <= 64, "one segment per tile");
+  typedef typename H::acc acc;
   typedef typename Vec8<T>::type frag;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int *list = reinterpret_cast<int *>(smem + F::body);
   uint32_t *bits = reinterpret_cast<uint32_t *>(list + a.cap);
   __shared__ int n_list;
 
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % 16, g = lane / 16;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % S, g = lane / S;
   const int wm = wave / WN, wn = wave % WN;
   unsigned item = xcd_remap(blockIdx.x, gridDim.x);
   const int split = (int)(item % a.splits);
@@ -318,35 +349,34 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
   const unsigned work = item;
   const int chunk = (int)(item % a.chunks);
   item /= a.chunks;
-  const int s = (int)(item % a.S);
+  const int gr = (int)(item % a.S);
   const int bh = (int)(item / a.S), hk = bh % a.Hkv, b = bh / a.Hkv;
 
   // row r of the group: token q_block * s + r / G, head hk * G + r % G
   auto row_of = [&](int m, int &token, int &head) {
     const int r = chunk * M + m;
     const int t = (int)a.by_g.div((unsigned)r);
-    token = s * a.q_block + t;
+    token = gr * a.q_block + t;
     head = hk * a.G + (r - t * a.G);
     return r < a.rows && token < a.Nq;
   };
   // the queries, as columns (asked for first, so that they arrive while the list is made)
-  frag qf[NQ][KC];
-#pragma unroll
-  for (int i = 0; i < NQ; ++i) {
+  frag qf[KC];
+  {
     int token, head;
-    const bool ok = row_of((wm * NQ + i) * 16 + col, token, head);
+    const bool ok = row_of(wm * S + col, token, head);
     const T *p = reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sq.b + (int64_t)token * a.sq.n + (int64_t)head * a.sq.h;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      const int ch = c * 32 + g * 8;
+      const int ch = c * H::KS + g * 8;
       frag t = {};
       if (ok && ch < a.D) t = *reinterpret_cast<const frag *>(p + ch);
-      qf[i][c] = t;
+      qf[c] = t;
     }
   }
   const int chunks = a.D / Img<T, DP>::VE;
   zero_pads<T, DP, TK>(smem, 4, chunks, wave);
-  const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + s) * a.top, a.top, a.nb, bits, list, &n_list);
+  const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + gr) * a.top, a.top, a.nb, bits, list, &n_list);
   const int e0 = (int)((int64_t)n * split / a.splits), e1 = (int)((int64_t)n * (split + 1) / a.splits);
   const KeySource keys{list + e0, a.vis ? a.vis + (int64_t)b * a.Nk : &g_one, a.vis != nullptr, (e1 - e0) << (a.lb - 6), a.lb, a.Nk};
   const int nt = keys.n * 64 / TK;
@@ -371,19 +401,12 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
   const float sc2 = fmaxf(fabsf(a.c), 1e-30f);                   // not 0: -inf times it has to stay -inf
   if (a.c < 0.f) {
 #pragma unroll
-    for (int i = 0; i < NQ; ++i)
-#pragma unroll
-      for (int c = 0; c < KC; ++c) qf[i][c] = -qf[i][c];
+    for (int c = 0; c < KC; ++c) qf[c] = -qf[c];
   }
-  f32x4 o[NQ][DT];
-  float m[NQ], l[NQ];                                            // maximum in log2 units, sum of exp2(score - maximum)
+  acc o[DT];
+  float m = kNegInf, l = 0.f;                                    // maximum in log2 units, sum of exp2(score - maximum)
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    m[i] = kNegInf;
-    l[i] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < DT; ++d) o[d] = acc(0.f);
   if (nt > 0) nxt = keys.finish(raw);
   for (int t = 0; t < nt; ++t) {
     tile_barrier<0>();                                           // tile t is there, tile t - 1 has been read
@@ -396,71 +419,58 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
 #pragma unroll
     for (int u = 0; u < KU; ++u)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) kf[u][c] = row_frag<T, DP>(krows, (wn * KU + u) * 16 + col, c * 32 + g * 8);
+      for (int c = 0; c < KC; ++c) kf[u][c] = row_frag<T, DP>(krows, (wn * KU + u) * S + col, c * H::KS + g * 8);
     __builtin_amdgcn_sched_barrier(0);
-    f32x4 sc[KU][NQ];
+    acc sc[KU];
 #pragma unroll
     for (int u = 0; u < KU; ++u) {
+      sc[u] = acc(0.f);
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) sc[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) sc[u][i] = mma(kf[u][c], qf[i][c], sc[u][i]);
+      for (int c = 0; c < KC; ++c) sc[u] = mma(kf[u][c], qf[c], sc[u]);
     }
-    constexpr int AH = sizeof(T) == 2 ? DT : DT / 2;             // fp32 fragments are twice as large, and their products 16 times as long
+    constexpr int NV = DT * PF, AH = sizeof(T) == 2 ? NV : NV / 2;   // fp32 fragments are twice as large, and their products 16 times as long
     frag vf[AH];
+    auto v_frag = [&](int i) { return col_frag<T, DP, S, E < 8>(vrows, wn * KU * S + i % PF * 16, i / PF * S, lane); };
 #pragma unroll
-    for (int d = 0; d < AH; ++d) vf[d] = col_frag<T, DP, KU>(vrows, wn * KU * 16, d * 16, lane);
+    for (int i = 0; i < AH; ++i) vf[i] = v_frag(i);
     __builtin_amdgcn_sched_barrier(0);
-    if (cur.mask != ~0ull) {
-      const unsigned seen = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * KU * 16 + g * 4));
+    // this wave's keys of the mask
+    const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * KU * S)) | (S * KU < 32 ? ~0u << (S * KU % 32) : 0u);
+    if (part != ~0u) {
+      const unsigned seen = part >> (g * 4);
 #pragma unroll
       for (int u = 0; u < KU; ++u)
 #pragma unroll
-        for (int i = 0; i < NQ; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[u][i][e] = (seen >> (u * 16 + e)) & 1 ? sc[u][i][e] : kNegInf;
+        for (int e = 0; e < H::AE; ++e) sc[u][e] = (seen >> (u * S + H::row(e))) & 1 ? sc[u][e] : kNegInf;
     }
-    frag pf[NQ];
-    bool grew = false;
-    float f[NQ];
+    float mx = max2(sc[0][0], sc[0][1]);
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      float mx = max2(sc[0][i][0], sc[0][i][1]);
+    for (int e = 2; e < E; ++e) mx = max2(mx, sc[e / H::AE][e % H::AE]);
+    mx = column_max<S>(mx);
+    const float mn = max2(m, mx * sc2);
+    const float ms = mn == kNegInf ? 0.f : mn;                   // nothing seen yet: exp2(-inf - 0) = 0
+    const float f = __builtin_amdgcn_exp2f(m - ms);              // exactly 1 while the maximum stays
+    const bool grew = mn > m;
+    m = mn;
+    float sum = 0.f;
+    frag pf[PF];
 #pragma unroll
-      for (int e = 2; e < 4 * KU; ++e) mx = max2(mx, sc[e / 4][i][e % 4]);
-      mx = quarter_max(mx);
-      const float mn = max2(m[i], mx * sc2);
-      const float ms = mn == kNegInf ? 0.f : mn;                 // nothing seen yet: exp2(-inf - 0) = 0
-      f[i] = __builtin_amdgcn_exp2f(m[i] - ms);                  // exactly 1 while the maximum stays
-      grew |= mn > m[i];
-      m[i] = mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (e >= 4 * KU) {
-          pf[i][e] = (T)0.f;
-          continue;
-        }
-        const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / 4 % KU][i][e % 4], sc2, -ms));
-        sum += p;
-        pf[i][e] = (T)p;
+    for (int e = 0; e < 8 * PF; ++e) {
+      if (e >= E) {
+        pf[e / 8][e % 8] = (T)0.f;
+        continue;
       }
-      l[i] = fmaf(l[i], f[i], sum);
+      const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / H::AE % KU][e % H::AE], sc2, -ms));
+      sum += p;
+      pf[e / 8][e % 8] = (T)p;
     }
+    l = fmaf(l, f, sum);
     if (__any(grew)) {                                           // no maximum moved in most tiles behind the first ones
 #pragma unroll
-      for (int i = 0; i < NQ; ++i)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[i][d] *= f[i];
+      for (int d = 0; d < DT; ++d) o[d] *= f;
     }
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const frag v = d < AH ? vf[d % AH] : col_frag<T, DP, KU>(vrows, wn * KU * 16, d * 16, lane);
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) o[i][d] = mma(v, pf[i], o[i][d]);
-    }
+    for (int i = 0; i < NV; ++i) o[i / PF] = mma(i < AH ? vf[i % AH] : v_frag(i), pf[i % PF], o[i / PF]);
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
     cur = nxt;
     nxt = keys.finish(raw);
@@ -470,17 +480,19 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
   float *jo = reinterpret_cast<float *>(smem);                   // [WN][M][LO]
   float *jm = jo + WN * M * F::LO, *jl = jm + WN * M;            // [WN][M] each
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    const int r = wn * M + (wm * NQ + i) * 16 + col;
-    l[i] += __shfl_xor(l[i], 16, 64);
-    l[i] += __shfl_xor(l[i], 32, 64);
+  {
+    const int r = wn * M + wm * S + col;
+    if (S == 16) l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
     if (g == 0) {
-      jm[r] = m[i];
-      jl[r] = l[i];
+      jm[r] = m;
+      jl[r] = l;
     }
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(jo + r * F::LO + d * 16 + g * 4) = o[i][d];
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < H::AE; e += 4)
+        *reinterpret_cast<f32x4 *>(jo + r * F::LO + d * S + H::row(e) + g * 4) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
   }
   __syncthreads();
   // write out: rows of D channels, 4 per thread
@@ -491,7 +503,7 @@ __global__ __launch_bounds__(256, OCC) void attend_fwd_kernel(AttnArgs a) {
     if (!row_of(r, token, head)) continue;
     float mx = kNegInf, sum = 0.f;
 #pragma unroll
-    for (int x = 0; x < WN; ++x) mx = fmaxf(mx, jm[x * M + r]);
+    for (int x = 0; x < WN; ++x) mx = max2(mx, jm[x * M + r]);
     f32x4 x4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < WN; ++x) {
@@ -838,7 +850,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
   constexpr int M = F::M, TR = F::TR, NB = F::NB, KC = DP / 32, DT = DP / 16, PER = 2 * P::NU;
   typedef typename Vec8<T>::type frag;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  uint2 *tab = reinterpret_cast<uint2 *>(smem + F::body);                              // [kBatch], x = ~0: no row
+  u32x2 *tab = reinterpret_cast<u32x2 *>(smem + F::body);                              // [kBatch], x = ~0: no row
   float *lse2 = reinterpret_cast<float *>(tab + kBatch), *delta = lse2 + kBatch;       // [kBatch] each
   int *list = reinterpret_cast<int *>(delta + kBatch);                                 // [32 kWindow]
   __shared__ int n_list;
@@ -906,7 +918,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
 #pragma unroll
       for (int u = 0; u < kBatch / 256; ++u) {
         const int r = u * 256 + tid;
-        uint2 where = {~0u, ~0u};
+        u32x2 where = {~0u, ~0u};
         float ls = kPosInf, de = 0.f;                            // exp2(x - inf) = 0
         if (r < in_batch) {
           const unsigned e = a.by_rows.div(r0 + r), rr = r0 + r - e * (unsigned)a.rows;
@@ -928,7 +940,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
         delta[r] = de;
       }
       __syncthreads();
-      uint2 x[P::NU];                                            // where the rows of the next tile lie, read a tile before they are asked for
+      u32x2 x[P::NU];                                            // where the rows of the next tile lie, read a tile before they are asked for
       auto locate = [&](int t) {
 #pragma unroll
         for (int u = 0; u < P::NU; ++u) x[u] = tab[min(t, kBatch / TR - 1) * TR + (P::whole ? P::row(u) : min(P::row(u), TR - 1))];
@@ -1073,9 +1085,9 @@ template <typename K> static int launch(K kernel, size_t lds, int64_t blocks, co
 }
 template <typename T, int DP> static int launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t s) {
   const char *what = "block_attention";
-  if (a.rows <= kFewRows) return launch(attend_fwd_kernel<T, DP, 1, 1, 4, 1, 2>, FwdTile<T, DP, 1, 1, 4, 1>::body + list_bytes(a), blocks, a, s, what);
-  if constexpr (sizeof(T) == 4) return launch(attend_fwd_kernel<T, DP, 1, 4, 1, 2, 2>, FwdTile<T, DP, 1, 4, 1, 2>::body + list_bytes(a), blocks, a, s, what);
-  else return launch(attend_fwd_kernel<T, DP, 2, 2, 2, 2, 2>, FwdTile<T, DP, 2, 2, 2, 2>::body + list_bytes(a), blocks, a, s, what);
+  if (a.rows <= kFewRows) return launch(attend_fwd_kernel<T, DP, 16, 1, 4, 1>, FwdTile<T, DP, 16, 1, 4, 1>::body + list_bytes(a), blocks, a, s, what);
+  if constexpr (sizeof(T) == 4) return launch(attend_fwd_kernel<T, DP, 16, 4, 1, 2>, FwdTile<T, DP, 16, 4, 1, 2>::body + list_bytes(a), blocks, a, s, what);
+  else return launch(attend_fwd_kernel<T, DP, 32, 2, 2, 1>, FwdTile<T, DP, 32, 2, 2, 1>::body + list_bytes(a), blocks, a, s, what);
 }
 template <typename T, int DP> static int launch_dq(AttnArgs a, hipStream_t s) {
   const char *what = "block_attention backward (queries)";
