@@ -410,8 +410,6 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
   if (nt > 0) nxt = keys.finish(raw);
   for (int t = 0; t < nt; ++t) {
     tile_barrier<0>();                                           // tile t is there, tile t - 1 has been read
-    if (t + 1 < nt) issue(t + 1, nxt);
-    raw = keys.load((t + 2) * TK / 64);
     const char *krows = smem + (t & 1) * 2 * F::img, *vrows = krows + F::img;
     // all fragments of a product are asked for before its first step, those of the second product before the softmax: an LDS read
     // takes longer than a product, and there are only a few waves to hide it behind
@@ -434,6 +432,10 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < AH; ++i) vf[i] = v_frag(i);
     __builtin_amdgcn_sched_barrier(0);
+    // The next tile sets out once this one's fragments have been asked for: a transposing read behind it would be held back until it
+    // has landed (the compiler cannot tell the two halves of the LDS apart).
+    if (t + 1 < nt) issue(t + 1, nxt);
+    raw = keys.load((t + 2) * TK / 64);
     // this wave's keys of the mask
     const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * KU * S)) | (S * KU < 32 ? ~0u << (S * KU % 32) : 0u);
     if (part != ~0u) {
@@ -651,16 +653,18 @@ __global__ __launch_bounds__(1024) void attend_order_kernel(AttnArgs a) {
   for (int j = threadIdx.x; j < a.nb; j += 1024) order[atomicAdd(&start[cls(cnt[j])], 1u)] = j;
 }
 
-template <typename T, int DP, int NQ, int WM, int WN> struct DqTile {
-  static constexpr int M = 16 * NQ * WM, TK = 32 * WN;
-  static constexpr size_t img = (size_t)TK * Img<T, DP>::RB, tiles = 4 * img;
-  static constexpr size_t join = (size_t)M * (DP + 4) * 4;
+template <typename T, int DP, int S, int WM, int WN> struct DqTile {
+  static constexpr int KU = 32 / S, M = S * WM, TK = 32 * WN, LO = DP + 4;             // 32 keys a wave
+  static constexpr size_t img = (size_t)TK * Img<T, DP>::RB, tiles = 4 * img;          // K and V, twice
+  static constexpr size_t join = (size_t)WN * M * LO * 4;
   static constexpr size_t body = tiles > join ? tiles : join;
 };
-template <typename T, int DP, int NQ, int WM, int WN, int OCC>
+template <typename T, int DP, int S, int WM, int WN, int OCC>
 __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
-  typedef DqTile<T, DP, NQ, WM, WN> F;
-  constexpr int M = F::M, TK = F::TK, KC = DP / 32, DT = DP / 16;
+  typedef DqTile<T, DP, S, WM, WN> F;
+  typedef Shape<S> H;
+  typedef typename H::acc acc;
+  constexpr int M = F::M, TK = F::TK, KU = F::KU, KC = DP / H::KS, DT = DP / S, PF = 2 * KU * H::AE / 16;
   static_assert(TK <= 64, "one segment per tile");
   typedef typename Vec8<T>::type frag;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -668,28 +672,53 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   uint32_t *bits = reinterpret_cast<uint32_t *>(list + a.cap);
   __shared__ int n_list;
 
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % 16, g = lane / 16;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % S, g = lane / S;
   const int wm = wave / WN, wn = wave % WN;
   unsigned item = xcd_remap(blockIdx.x, gridDim.x);
   const int chunk = (int)(item % a.chunks);
   item /= a.chunks;
-  const int s = (int)(item % a.S);
+  const int gr = (int)(item % a.S);
   const int bh = (int)(item / a.S), hk = bh % a.Hkv, b = bh / a.Hkv;
+  auto row_of = [&](int m, int &token, int &head) {
+    const int r = chunk * M + m;
+    const int t = (int)a.by_g.div((unsigned)r);
+    token = gr * a.q_block + t;
+    head = hk * a.G + (r - t * a.G);
+    return r < a.rows && token < a.Nq;
+  };
+  frag qf[KC], df[KC];
+  float lse2 = kPosInf, delta = 0.f;                             // exp2(x - inf) = 0: no row, or a row that sees nothing
+  {
+    int token, head;
+    const bool ok = row_of(wm * S + col, token, head);
+    const T *p = reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sq.b + (int64_t)token * a.sq.n + (int64_t)head * a.sq.h;
+    const T *d = reinterpret_cast<const T *>(a.dout) + (int64_t)b * a.sdo.b + (int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h;
+    if (ok) {
+      const int64_t at = ((int64_t)b * a.Hq + head) * a.Nq + token;
+      const float x = a.lse[at];
+      if (x != kNegInf) lse2 = x * kLog2e;
+      delta = a.delta[at];
+    }
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int ch = c * H::KS + g * 8;
+      frag t = {}, u = {};
+      if (ok && ch < a.D) {
+        t = *reinterpret_cast<const frag *>(p + ch);
+        u = *reinterpret_cast<const frag *>(d + ch);
+      }
+      qf[c] = t;
+      df[c] = u;
+    }
+  }
   const int chunks = a.D / Img<T, DP>::VE;
   zero_pads<T, DP, TK>(smem, 4, chunks, wave);
-  const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + s) * a.top, a.top, a.nb, bits, list, &n_list);
+  const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + gr) * a.top, a.top, a.nb, bits, list, &n_list);
   const KeySource keys{list, a.vis ? a.vis + (int64_t)b * a.Nk : &g_one, a.vis != nullptr, n << (a.lb - 6), a.lb, a.Nk};
   const int nt = keys.n * 64 / TK;
   const char *kb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h);
   const char *vb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h);
   const unsigned kst = (unsigned)(a.sk.n * sizeof(T)), vst = (unsigned)(a.sv.n * sizeof(T));
-  auto row_of = [&](int m, int &token, int &head) {
-    const int r = chunk * M + m;
-    const int t = (int)a.by_g.div((unsigned)r);
-    token = s * a.q_block + t;
-    head = hk * a.G + (r - t * a.G);
-    return r < a.rows && token < a.Nq;
-  };
   auto issue = [&](int t, const Segment &x) {
     char *kd = smem + (t & 1) * 2 * F::img, *vd = kd + F::img;
     const int off = (t * TK) & 63;
@@ -703,123 +732,80 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     issue(0, cur);
     raw = keys.load(TK / 64);
   }
-
-  frag qf[NQ][KC], df[NQ][KC];
-  float lse2[NQ], delta[NQ];
+  acc o[DT];
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    int token, head;
-    const bool ok = row_of((wm * NQ + i) * 16 + col, token, head);
-    const T *p = reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sq.b + (int64_t)token * a.sq.n + (int64_t)head * a.sq.h;
-    const T *d = reinterpret_cast<const T *>(a.dout) + (int64_t)b * a.sdo.b + (int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h;
-    lse2[i] = kPosInf;                                           // exp2(x - inf) = 0: no row, or a row that sees nothing
-    delta[i] = 0.f;
-    if (ok) {
-      const int64_t at = ((int64_t)b * a.Hq + head) * a.Nq + token;
-      const float x = a.lse[at];
-      lse2[i] = x == kNegInf ? kPosInf : x * kLog2e;
-      delta[i] = a.delta[at];
-    }
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      const int ch = c * 32 + g * 8;
-      frag t = {}, u = {};
-      if (ok && ch < a.D) {
-        t = *reinterpret_cast<const frag *>(p + ch);
-        u = *reinterpret_cast<const frag *>(d + ch);
-      }
-      qf[i][c] = t;
-      df[i][c] = u;
-    }
-  }
-  f32x4 o[NQ][DT];
-#pragma unroll
-  for (int i = 0; i < NQ; ++i)
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < DT; ++d) o[d] = acc(0.f);
   if (nt > 0) nxt = keys.finish(raw);
   for (int t = 0; t < nt; ++t) {
     tile_barrier<0>();
-    if (t + 1 < nt) issue(t + 1, nxt);
-    raw = keys.load((t + 2) * TK / 64);
     const char *krows = smem + (t & 1) * 2 * F::img, *vrows = krows + F::img;
-    f32x4 sc[2][NQ], dp[2][NQ];
-    frag kf[KC], vf[KC];
+    acc sc[KU], dp[KU];
 #pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      kf[c] = row_frag<T, DP>(krows, wn * 32 + col, c * 32 + g * 8);
-      vf[c] = row_frag<T, DP>(vrows, wn * 32 + col, c * 32 + g * 8);
-    }
+    for (int u = 0; u < KU; ++u) sc[u] = dp[u] = acc(0.f);
+    // the fragments of a quarter of the products (S = 32: half of them) at a time, always one batch ahead
+    constexpr int NB = 2, CB = KU * KC / NB;                     // (u, c) pairs of a batch
+    frag kf[NB][CB], vf[NB][CB];
+    auto rows = [&](int x) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+      for (int i = 0; i < CB; ++i) {
+        const int u = (x * CB + i) / KC, c = (x * CB + i) % KC;
+        kf[x][i] = row_frag<T, DP>(krows, wn * 32 + u * S + col, c * H::KS + g * 8);
+        vf[x][i] = row_frag<T, DP>(vrows, wn * 32 + u * S + col, c * H::KS + g * 8);
+      }
+    };
+    rows(0);
+#pragma unroll
+    for (int x = 0; x < NB; ++x) {
       __builtin_amdgcn_sched_barrier(0);
+      if (x + 1 < NB) rows(x + 1);
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) sc[u][i] = dp[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          sc[u][i] = mma(kf[c], qf[i][c], sc[u][i]);
-          dp[u][i] = mma(vf[c], df[i][c], dp[u][i]);
-        }
-        if (u == 0) {                                            // the other 16 keys' fragments take the place of the used ones
-          kf[c] = row_frag<T, DP>(krows, wn * 32 + 16 + col, c * 32 + g * 8);
-          vf[c] = row_frag<T, DP>(vrows, wn * 32 + 16 + col, c * 32 + g * 8);
-        }
+      for (int i = 0; i < CB; ++i) {
+        const int u = (x * CB + i) / KC, c = (x * CB + i) % KC;
+        sc[u] = mma(kf[x][i], qf[c], sc[u]);
+        dp[u] = mma(vf[x][i], df[c], dp[u]);
       }
     }
-    constexpr int AH = DT / 2;
+    constexpr int NV = DT * PF, AH = sizeof(T) == 2 ? NV : NV / 2;
     frag ka[AH];
+    auto k_frag = [&](int i) { return col_frag<T, DP, S>(krows, wn * 32 + i % PF * 16, i / PF * S, lane); };
 #pragma unroll
-    for (int d = 0; d < AH; ++d) ka[d] = col_frag<T, DP>(krows, wn * 32, d * 16, lane);
+    for (int i = 0; i < AH; ++i) ka[i] = k_frag(i);
     __builtin_amdgcn_sched_barrier(0);
-    frag gf[NQ];
-    const unsigned seen = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32 + g * 4));
+    if (t + 1 < nt) issue(t + 1, nxt);                           // behind the transposing reads, as in the forward
+    raw = keys.load((t + 2) * TK / 64);
+    frag gf[PF];
+    const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32)), seen = part >> (g * 4);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < NQ; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i][e], a.c, -lse2[i]));
-          p = (seen >> (u * 16 + e)) & 1 ? p : 0.f;              // an unseen key's products are those of zeros
-          float ds = p * (dp[u][i][e] - delta[i]);
-          if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= a.scale;   // fp16: small score gradients; else the scale comes last
-          gf[i][u * 4 + e] = (T)ds;
-        }
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const frag k = ka[d % AH];
-      if (d + AH < DT) ka[d % AH] = col_frag<T, DP>(krows, wn * 32, (d + AH) * 16, lane);
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) o[i][d] = mma(k, gf[i], o[i][d]);
+    for (int e = 0; e < KU * H::AE; ++e) {
+      const int u = e / H::AE, x = e % H::AE;
+      float p = __builtin_amdgcn_exp2f(fmaf(sc[u][x], a.c, -lse2));
+      p = (seen >> (u * S + H::row(x))) & 1 ? p : 0.f;           // an unseen key's products are those of zeros
+      float ds = p * (dp[u][x] - delta);
+      if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= a.scale;   // fp16: small score gradients; else the scale comes last
+      gf[e / 8][e % 8] = (T)ds;
     }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) o[i / PF] = mma(i < AH ? ka[i % AH] : k_frag(i), gf[i % PF], o[i / PF]);
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
     cur = nxt;
     nxt = keys.finish(raw);
   }
-  float *jo = reinterpret_cast<float *>(smem);
+  float *jo = reinterpret_cast<float *>(smem);                   // [WN][M][LO]
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < WN; ++w) {
-    if (wn == w) {
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        const int r = (wm * NQ + i) * 16 + col;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          f32x4 *p = reinterpret_cast<f32x4 *>(jo + r * (DP + 4) + d * 16 + g * 4);
-          *p = w == 0 ? o[i][d] : *p + o[i][d];
-        }
-      }
-    }
-    __syncthreads();
-  }
+    for (int e = 0; e < H::AE; e += 4)
+      *reinterpret_cast<f32x4 *>(jo + (wn * M + wm * S + col) * F::LO + d * S + H::row(e) + g * 4) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+  __syncthreads();
   for (int id = tid; id < M * (a.D / 4); id += 256) {
     const int r = (int)a.by_d4.div((unsigned)id), ch = (id - r * (a.D / 4)) * 4;
     int token, head;
     if (!row_of(r, token, head)) continue;
-    const f32x4 x = *reinterpret_cast<const f32x4 *>(jo + r * (DP + 4) + ch) * (sizeof(T) == 2 && PScale<T>::bits > 0.f ? 1.f : a.scale);
+    f32x4 x = *reinterpret_cast<const f32x4 *>(jo + r * F::LO + ch);
+#pragma unroll
+    for (int w = 1; w < WN; ++w) x += *reinterpret_cast<const f32x4 *>(jo + (w * M + r) * F::LO + ch);
+    x *= sizeof(T) == 2 && PScale<T>::bits > 0.f ? 1.f : a.scale;
     typename Vec4<T>::type y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
@@ -983,8 +969,6 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
         if (NB == 4 && t + 2 < nt) tile_barrier<NB == 4 ? 2 * PER : 0>();
         else if (NB == 4 && t + 1 < nt) tile_barrier<NB == 4 ? PER : 0>();
         else tile_barrier<0>();
-        if (t + NB - 1 < nt) issue(t + NB - 1);
-        locate(t + NB);
         const char *qrows = smem + (t % NB) * 2 * F::img, *drows = qrows + F::img;
         constexpr bool ahead = sizeof(T) == 2 || DP <= 64;        // all fragments before the first product (fp32: registers for 64 channels)
         frag qf[2][KC], df[2][KC];
@@ -1039,6 +1023,9 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
           if (d + AH < DT) {
             da[d % AH] = col_frag<T, DP>(drows, 0, (d + AH) * 16, lane);
             qa[d % AH] = col_frag<T, DP>(qrows, 0, (d + AH) * 16, lane);
+          } else if (d + AH == DT) {                             // behind the transposing reads, as in the forward
+            if (t + NB - 1 < nt) issue(t + NB - 1);
+            locate(t + NB);
           }
           gv[d] = mma(x, pf, gv[d]);
           gk[d] = mma(y, gf, gk[d]);
@@ -1094,9 +1081,9 @@ template <typename T, int DP> static int launch_dq(AttnArgs a, hipStream_t s) {
   const bool few = a.rows <= 32;
   a.chunks = (int)cdiv(a.rows, few ? 32 : 64);
   const int64_t blocks = (int64_t)a.B * a.Hkv * a.S * a.chunks;
-  if (few) return launch(attend_dq_kernel<T, DP, 1, 2, 2, 1>, DqTile<T, DP, 1, 2, 2>::body + list_bytes(a), blocks, a, s, what);
-  if constexpr (sizeof(T) == 4) return launch(attend_dq_kernel<T, DP, 1, 4, 1, 1>, DqTile<T, DP, 1, 4, 1>::body + list_bytes(a), blocks, a, s, what);
-  else return launch(attend_dq_kernel<T, DP, 2, 2, 2, 2>, DqTile<T, DP, 2, 2, 2>::body + list_bytes(a), blocks, a, s, what);
+  if (few) return launch(attend_dq_kernel<T, DP, 16, 2, 2, 1>, DqTile<T, DP, 16, 2, 2>::body + list_bytes(a), blocks, a, s, what);
+  if constexpr (sizeof(T) == 4) return launch(attend_dq_kernel<T, DP, 16, 4, 1, 1>, DqTile<T, DP, 16, 4, 1>::body + list_bytes(a), blocks, a, s, what);
+  else return launch(attend_dq_kernel<T, DP, 32, 2, 2, 2>, DqTile<T, DP, 32, 2, 2>::body + list_bytes(a), blocks, a, s, what);
 }
 template <typename T, int DP> static int launch_dkv(const AttnArgs &a, hipStream_t s) {
   const char *what = "block_attention backward (keys)";
