@@ -290,7 +290,9 @@ __device__ __forceinline__ int group_blocks(const int32_t *blocks, int top, int 
 struct Segment {
   int key0;                                                      // first key, or -1: none
   uint64_t mask;                                                 // bit r: key0 + r exists and is seen
-  __device__ __forceinline__ uint64_t there(int nk) const { return key0 < 0 ? 0ull : key0 + 64 <= nk ? ~0ull : (1ull << (nk - key0)) - 1; }
+  __device__ __forceinline__ uint64_t there(int nk) const {      // bit r: key0 + r exists (a block of 128 may end in its first segment)
+    return key0 < 0 || key0 >= nk ? 0ull : key0 + 64 <= nk ? ~0ull : (1ull << (nk - key0)) - 1;
+  }
 };
 // The raw parts of a segment are asked for a tile before they are needed.  The load is unconditional (clamped): a load behind a
 // condition would be waited for where the paths meet, and with it the tile that is on its way.

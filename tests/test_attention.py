@@ -357,6 +357,9 @@ ATTEND = [  # b, nq, nk, hq, hk, d, block, q_block, top, masked, layout, lists
     (1, 40, 640, 8, 1, 32, 64, 1, 4, False, "dense", "ascending"),             # every token with blocks of its own
     (1, 70, 190, 24, 1, 16, 64, 1, 2, True, "dense", "mixed"),
     (2, 64, 64, 1, 1, 64, 64, 128, 4, False, "dense", "ascending"),            # more choices than blocks, groups beyond the end
+    (2, 70, 20, 2, 1, 64, 128, 16, 3, False, "dense", "ascending"),            # the last block of 128 ends in its first half
+    (1, 1, 150, 8, 2, 128, 128, 1, 2, True, "heads_first", "mixed"),
+    (1, 65, 300, 1, 1, 32, 128, 64, 3, True, "dense", "ascending"),
 ]
 
 
