@@ -29,6 +29,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Vec8;
 template <> struct Vec8<float> { typedef f32x8 type; };
@@ -41,6 +44,17 @@ __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __built
 __device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+// 16 k-elements, 4 per lane (element 4 (l / 16) + e)
+__device__ __forceinline__ f32x4 mma4(bf16x4 a, bf16x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma4(f16x4 a, f16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma4(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
   return c;
 }
 
@@ -109,7 +123,6 @@ template <typename T, int DP> struct Img {
 typedef __attribute__((address_space(3))) void *lds_vptr;
 typedef const __attribute__((address_space(1))) void *glb_cvptr;
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -201,33 +214,40 @@ template <typename T, int DP> __device__ __forceinline__ typename Vec8<T>::type 
   }
 }
 // ... for a contraction over tokens, in the order in which a lane holds the results of an S x S product: channel d0 + lane % S, and
-//   S = 16: of the 32 tokens from t0, tokens t0 + 4 q .. + 3 and t0 + 16 + 4 q .. + 3 (HALF: 16 tokens, the second four are zeros)
+//   S = 16: of the 32 tokens from t0, tokens t0 + 4 q .. + 3 and t0 + 16 + 4 q .. + 3
 //   S = 32: of the 16 tokens from t0, tokens t0 + 4 q .. + 3 and t0 + 8 + 4 q .. + 3
-// with q = lane / S; t0 is a multiple of 16.
-template <typename T, int DP, int S = 16, bool HALF = false> __device__ __forceinline__ typename Vec8<T>::type col_frag(const char *img, int t0, int d0, int lane) {
+// with q = lane / S; t0 is a multiple of 16.  col_frag4: the first four alone.
+template <typename T, int DP, int S = 16> __device__ __forceinline__ typename Vec4<T>::type col_frag4(const char *img, int d0, int lane) {
   typedef Img<T, DP> I;
   const int q = lane / S, col = lane % 16;
-  constexpr int SECOND = S == 16 ? 16 : 8;
   if constexpr (sizeof(T) == 2) {
     // transposing read: lane 4 r + p of a group of 16 points at row r, elements 4 p .. + 3 of a 4 x 16 block and gets column lane % 16 of it
     const int row = 4 * q + col / 4, p = col % 4, ch = (d0 + (S == 32 ? lane / 16 % 2 * 16 : 0)) / 8 + p / 2;
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(img + (t0 + row) * I::RB + ((ch ^ I::swz(row)) << 4) + (p % 2) * 8));
-    s16x4 y = {0, 0, 0, 0};
-    if constexpr (!HALF)
-      y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(img + (t0 + row + SECOND) * I::RB + ((ch ^ I::swz(row + SECOND)) << 4) + (p % 2) * 8));
-    const s16x8 both = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_bit_cast(typename Vec8<T>::type, both);
+    return __builtin_bit_cast(typename Vec4<T>::type, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(img + row * I::RB + ((ch ^ I::swz(row)) << 4) + (p % 2) * 8)));
   } else {
     static_assert(S == 16, "fp32 products are 16 x 16");
-    f32x8 r;
+    f32x4 r;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int row = 4 * q + e;
-      const char *a = img + (t0 + row) * I::RB + (((d0 / 4 + col / 4) ^ I::swz(row)) << 4) + (col % 4) * 4;
-      r[e] = *reinterpret_cast<const float *>(a);
-      r[4 + e] = HALF ? 0.f : *reinterpret_cast<const float *>(a + 16 * I::RB);
+      r[e] = *reinterpret_cast<const float *>(img + row * I::RB + (((d0 / 4 + col / 4) ^ I::swz(row)) << 4) + (col % 4) * 4);
     }
     return r;
+  }
+}
+template <typename T, int DP, int S = 16> __device__ __forceinline__ typename Vec8<T>::type col_frag(const char *img, int t0, int d0, int lane) {
+  typedef Img<T, DP> I;
+  if constexpr (sizeof(T) == 2) {
+    const int q = lane / S, col = lane % 16;
+    constexpr int SECOND = S == 16 ? 16 : 8;
+    const int row = 4 * q + col / 4, p = col % 4, ch = (d0 + (S == 32 ? lane / 16 % 2 * 16 : 0)) / 8 + p / 2;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(img + (t0 + row) * I::RB + ((ch ^ I::swz(row)) << 4) + (p % 2) * 8));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(img + (t0 + row + SECOND) * I::RB + ((ch ^ I::swz(row + SECOND)) << 4) + (p % 2) * 8));
+    const s16x8 both = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(typename Vec8<T>::type, both);
+  } else {
+    const f32x4 x = col_frag4<T, DP, S>(img + t0 * I::RB, d0, lane), y = col_frag4<T, DP, S>(img + (t0 + 16) * I::RB, d0, lane);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
 
@@ -320,6 +340,63 @@ struct KeySource {
   }
 };
 
+// Joins the WN key sets of a workgroup's M = S WM rows and writes them: every wave leaves its output, maximum and sum, and a thread adds
+// them up under the common maximum.  `o`, `m`, `l` as the forward's loops leave them; `part`: where a split's partial rows go, or null.
+template <typename T, int DP, int S, int WM, int WN, typename Rows>
+__device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const typename Shape<S>::acc (&o)[DP / S], float m, float l, const Rows &row_of, float *pm, int b, int wm, int wn) {
+  typedef Shape<S> H;
+  constexpr int M = S * WM, LO = DP + 4, DT = DP / S;
+  const int tid = threadIdx.x, lane = tid % 64, col = lane % S, g = lane / S;
+  float *jo = reinterpret_cast<float *>(smem);                   // [WN][M][LO]
+  float *jm = jo + WN * M * LO, *jl = jm + WN * M;            // [WN][M] each
+  __syncthreads();
+  {
+    const int r = wn * M + wm * S + col;
+    if (S == 16) l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (g == 0) {
+      jm[r] = m;
+      jl[r] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < H::AE; e += 4)
+        *reinterpret_cast<f32x4 *>(jo + r * LO + d * S + H::row(e) + g * 4) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+  }
+  __syncthreads();
+  // write out: rows of D channels, 4 per thread
+  for (int id = tid; id < M * (a.D / 4); id += 256) {
+    const int r = (int)a.by_d4.div((unsigned)id), ch = (id - r * (a.D / 4)) * 4;
+    int token, head;
+    if (!row_of(r, token, head)) continue;
+    float mx = kNegInf, sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < WN; ++x) mx = max2(mx, jm[x * M + r]);
+    f32x4 x4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < WN; ++x) {
+      const float f = mx == kNegInf ? 0.f : __builtin_amdgcn_exp2f(jm[x * M + r] - mx);
+      sum += mx == kNegInf ? 0.f : jl[x * M + r] * f;
+      x4 += *reinterpret_cast<const f32x4 *>(jo + (x * M + r) * LO + ch) * f;
+    }
+    if (pm) {
+      *reinterpret_cast<f32x4 *>(pm + (int64_t)r * a.D + ch) = x4;
+      if (ch == 0) {
+        pm[(int64_t)M * a.D + r] = mx;
+        pm[(int64_t)M * a.D + M + r] = sum;
+      }
+      continue;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // nothing seen: zero; NaN stays NaN
+    typename Vec4<T>::type y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)(x4[e] * inv);
+    *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.out) + (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch) = y;
+    if (ch == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx + __builtin_log2f(sum)) * kLn2;
+  }
+}
+
 // One workgroup: M = S WM query rows of one group (a row = one query token and one head of the key head's group), 4 waves as WM row
 // sets x WN key sets.  The group's keys pass as one stream in tiles of TK = S KU WN (up to a segment); every wave keeps its own
 // running maximum, sum and output for its S KU keys of each tile, joined at the end, so the only meeting of the waves in the loop is
@@ -334,8 +411,8 @@ template <typename T, int DP, int S, int WM, int WN, int KU>
 __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
   typedef FwdTile<T, DP, S, WM, WN, KU> F;
   typedef Shape<S> H;
-  constexpr int M = F::M, TK = F::TK, KC = DP / H::KS, DT = DP / S, E = H::AE * KU, PF = (E + 7) / 8;   // E: scores per lane
-  static_assert(TK <= 64, "one segment per tile");
+  constexpr int M = F::M, TK = F::TK, KC = DP / H::KS, DT = DP / S, E = H::AE * KU, PF = E / 8;   // E: scores per lane
+  static_assert(TK <= 64 && S * KU == 32, "one segment per tile, 32 keys a wave");
   typedef typename H::acc acc;
   typedef typename Vec8<T>::type frag;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -430,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     }
     constexpr int NV = DT * PF, AH = sizeof(T) == 2 ? NV : NV / 2;   // fp32 fragments are twice as large, and their products 16 times as long
     frag vf[AH];
-    auto v_frag = [&](int i) { return col_frag<T, DP, S, E < 8>(vrows, wn * KU * S + i % PF * 16, i / PF * S, lane); };
+    auto v_frag = [&](int i) { return col_frag<T, DP, S>(vrows, wn * 32 + i % PF * 16, i / PF * S, lane); };
 #pragma unroll
     for (int i = 0; i < AH; ++i) vf[i] = v_frag(i);
     __builtin_amdgcn_sched_barrier(0);
@@ -439,7 +516,7 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     if (t + 1 < nt) issue(t + 1, nxt);
     raw = keys.load((t + 2) * TK / 64);
     // this wave's keys of the mask
-    const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * KU * S)) | (S * KU < 32 ? ~0u << (S * KU % 32) : 0u);
+    const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32));
     if (part != ~0u) {
       const unsigned seen = part >> (g * 4);
 #pragma unroll
@@ -459,12 +536,8 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     float sum = 0.f;
     frag pf[PF];
 #pragma unroll
-    for (int e = 0; e < 8 * PF; ++e) {
-      if (e >= E) {
-        pf[e / 8][e % 8] = (T)0.f;
-        continue;
-      }
-      const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / H::AE % KU][e % H::AE], sc2, -ms));
+    for (int e = 0; e < E; ++e) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / H::AE][e % H::AE], sc2, -ms));
       sum += p;
       pf[e / 8][e % 8] = (T)p;
     }
@@ -480,60 +553,153 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     nxt = keys.finish(raw);
   }
 
-  // join the key sets: every wave leaves its output, maximum and sum, and a thread adds them up under the common maximum
-  float *jo = reinterpret_cast<float *>(smem);                   // [WN][M][LO]
-  float *jm = jo + WN * M * F::LO, *jl = jm + WN * M;            // [WN][M] each
-  __syncthreads();
-  {
-    const int r = wn * M + wm * S + col;
-    if (S == 16) l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (g == 0) {
-      jm[r] = m;
-      jl[r] = l;
-    }
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int e = 0; e < H::AE; e += 4)
-        *reinterpret_cast<f32x4 *>(jo + r * F::LO + d * S + H::row(e) + g * 4) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
-  }
-  __syncthreads();
-  // write out: rows of D channels, 4 per thread
-  float *pm = a.splits > 1 ? a.part + ((int64_t)work * a.splits + split) * M * (a.D + 2) : nullptr;
-  for (int id = tid; id < M * (a.D / 4); id += 256) {
-    const int r = (int)a.by_d4.div((unsigned)id), ch = (id - r * (a.D / 4)) * 4;
-    int token, head;
-    if (!row_of(r, token, head)) continue;
-    float mx = kNegInf, sum = 0.f;
-#pragma unroll
-    for (int x = 0; x < WN; ++x) mx = max2(mx, jm[x * M + r]);
-    f32x4 x4 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int x = 0; x < WN; ++x) {
-      const float f = mx == kNegInf ? 0.f : __builtin_amdgcn_exp2f(jm[x * M + r] - mx);
-      sum += mx == kNegInf ? 0.f : jl[x * M + r] * f;
-      x4 += *reinterpret_cast<const f32x4 *>(jo + (x * M + r) * F::LO + ch) * f;
-    }
-    if (pm) {
-      *reinterpret_cast<f32x4 *>(pm + (int64_t)r * a.D + ch) = x4;
-      if (ch == 0) {
-        pm[(int64_t)M * a.D + r] = mx;
-        pm[(int64_t)M * a.D + M + r] = sum;
-      }
-      continue;
-    }
-    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // nothing seen: zero; NaN stays NaN
-    typename Vec4<T>::type y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (T)(x4[e] * inv);
-    *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.out) + (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch) = y;
-    if (ch == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx + __builtin_log2f(sum)) * kLn2;
-  }
+  join_sets<T, DP, S, WM, WN>(a, smem, o, m, l, row_of, a.splits > 1 ? a.part + ((int64_t)work * a.splits + split) * M * (a.D + 2) : nullptr, b, wm, wn);
 }
 
-// Joins the splits (at most 64) of a row: one workgroup per row.  Lane x of every wave holds split x's factor; the waves take the
-// splits in turn, a lane two channels of them, and are added up in wave order.
+// Few rows (a group of up to 16: one token of some heads): one workgroup holds all of them, and no element of a key is used twice.  The four
+// waves take 16 keys of a segment each and go their own ways: keys come to registers in the operand's order, values pass through 16 rows
+// of LDS of the wave's own (for the transposing read alone), one segment ahead, and no wave waits for another before the join.  What counts is
+// the number of loads in flight, so registers are kept to four workgroups per CU; two or three segments ahead at two or three
+// workgroups are slower (1,590 tokens x 2 key heads, each with 12 blocks of 64 keys of 72 bf16 channels: 69 us; two ahead 78, three ahead
+// 82; the tiles shared through LDS that the larger groups use: 109).  That is 10 TB/s of keys and values, out of the caches; the
+// vector instructions of the softmax take about half the time.  A single token of 4 items against 64 blocks of 128 (34 MB): 14 us, 5 of them
+// the launch and the list, and 4 for the join.
+template <typename T, int DP> struct FewTile {
+  static constexpr size_t img = (size_t)16 * Img<T, DP>::RB, tiles = 4 * img, join = (size_t)4 * 16 * (DP + 6) * 4;
+  static constexpr size_t body = tiles > join ? tiles : join;
+};
+template <typename T, int DP, int OCC>
+__global__ __launch_bounds__(256, OCC) void attend_few_kernel(AttnArgs a) {
+  typedef FewTile<T, DP> F;
+  typedef Img<T, DP> I;
+  constexpr int KC = DP / 32, DT = DP / 16;
+  typedef typename Vec8<T>::type frag;
+  typedef typename Vec4<T>::type frag4;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  int *list = reinterpret_cast<int *>(smem + F::body);
+  uint32_t *bits = reinterpret_cast<uint32_t *>(list + a.cap);
+  __shared__ int n_list;
+
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, col = lane % 16, g = lane / 16;
+  unsigned item = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = (int)(item % a.splits);
+  const unsigned work = item / a.splits;
+  const int gr = (int)(work % a.S), bh = (int)(work / a.S), hk = bh % a.Hkv, b = bh / a.Hkv;
+  auto row_of = [&](int r, int &token, int &head) {
+    const int t = (int)a.by_g.div((unsigned)r);
+    token = gr * a.q_block + t;
+    head = hk * a.G + (r - t * a.G);
+    return r < a.rows && token < a.Nq;
+  };
+  frag qf[KC];
+  {
+    int token, head;
+    const bool ok = row_of(col, token, head);
+    const T *p = reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sq.b + (int64_t)token * a.sq.n + (int64_t)head * a.sq.h;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int ch = c * 32 + g * 8;
+      frag t = {};
+      if (ok && ch < a.D) t = *reinterpret_cast<const frag *>(p + ch);
+      qf[c] = a.c < 0.f ? -t : t;                                // a negative scale turns the queries' sign, as in the other forward
+    }
+  }
+  const int n = group_blocks(a.blocks + ((int64_t)bh * a.S + gr) * a.top, a.top, a.nb, bits, list, &n_list);
+  const int e0 = (int)((int64_t)n * split / a.splits), e1 = (int)((int64_t)n * (split + 1) / a.splits);
+  const int per = a.lb - 6, nt = (e1 - e0) << per;
+  const char *kb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + (int64_t)b * a.sk.b + (int64_t)hk * a.sk.h);
+  const char *vb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + (int64_t)b * a.sv.b + (int64_t)hk * a.sv.h);
+  const float *vis = a.vis ? a.vis + (int64_t)b * a.Nk : &g_one;
+  const int vis_step = a.vis != nullptr;
+  const int64_t kst = a.sk.n * (int64_t)sizeof(T), vst = a.sv.n * (int64_t)sizeof(T);
+  // channels from D on are read as the last ones (a product's are zeroed, an output's not written)
+  const unsigned ch0 = (unsigned)(g * 8 * sizeof(T)), ch1 = (unsigned)(min((KC - 1) * 32 + g * 8, a.D - 8) * sizeof(T));
+  char *img = smem + wave * F::img;
+
+  frag kf[KC], vf[KC];
+  float see = 0.f;
+  int left = 0;                                                  // keys from this wave's first one on
+  auto key_of = [&](int i) { return (list[e0 + (i >> per)] << a.lb) + ((i & ((1 << per) - 1)) << 6) + wave * 16; };
+  // A key behind the last one is read as the last (a wave that has none: as the head's first); its score is overwritten.
+  auto load = [&](int key0) {
+    left = a.Nk - key0;
+    const bool live = left > 0;
+    const int first = live ? key0 : 0;
+    const unsigned row = live ? (unsigned)min(col, left - 1) : 0u;
+    const char *kp = kb + first * kst, *vp = vb + first * vst;
+    const unsigned kr = row * (unsigned)kst, vr = row * (unsigned)vst;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) kf[c] = *(const __attribute__((address_space(1))) frag *)(kp + (kr + (c + 1 < KC ? c * 32 * (unsigned)sizeof(T) + ch0 : ch1)));
+#pragma unroll
+    for (int c = 0; c < KC; ++c) vf[c] = *(const __attribute__((address_space(1))) frag *)(vp + (vr + (c + 1 < KC ? c * 32 * (unsigned)sizeof(T) + ch0 : ch1)));
+    see = *(const __attribute__((address_space(1))) float *)(vis + first * vis_step + row * (unsigned)vis_step);
+  };
+  const float sc2 = fmaxf(fabsf(a.c), 1e-30f);                   // not 0: -inf times it has to stay -inf
+  f32x4 o[DT];
+  float m = kNegInf, l = 0.f;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (nt > 0) load(__builtin_amdgcn_readfirstlane(key_of(0)));
+  for (int t = 0; t < nt; ++t) {
+    const int next = key_of(min(t + 1, nt - 1));
+    const bool in = col < left && see > 0.5f;
+    const unsigned part = (unsigned)__ballot(in);                // the four quarters say the same
+    f32x4 sc = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (part != 0) {
+      if (a.D < DP && (KC - 1) * 32 + g * 8 >= a.D) kf[KC - 1] = frag{};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) sc = mma(kf[c], qf[c], sc);
+      if (part != ~0u) {                                         // a hidden value is multiplied by a probability of 0: it has to be a number
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          typedef unsigned words __attribute__((ext_vector_type(sizeof(frag) / 4)));
+          words w = __builtin_bit_cast(words, vf[c]);
+#pragma unroll
+          for (int e = 0; e < (int)sizeof(frag) / 4; ++e) w[e] = in ? w[e] : 0u;
+          vf[c] = __builtin_bit_cast(frag, w);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[e] = (part >> (g * 4 + e)) & 1 ? sc[e] : kNegInf;
+      }
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        char *row = img + col * I::RB;
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<frag *>(row + (((c * 4 + g) ^ I::swz(col)) << 4)) = vf[c];
+        else {
+          *reinterpret_cast<f32x4 *>(row + (((c * 8 + g * 2) ^ I::swz(col)) << 4)) = __builtin_shufflevector(vf[c], vf[c], 0, 1, 2, 3);
+          *reinterpret_cast<f32x4 *>(row + (((c * 8 + g * 2 + 1) ^ I::swz(col)) << 4)) = __builtin_shufflevector(vf[c], vf[c], 4, 5, 6, 7);
+        }
+      }
+    }
+    if (t + 1 < nt) load(__builtin_amdgcn_readfirstlane(next));
+    if (part == 0) continue;
+    frag4 vt[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vt[d] = col_frag4<T, DP>(img, d * 16, lane);
+    const float mx = column_max<16>(max2(max2(sc[0], sc[1]), max2(sc[2], sc[3])));
+    const float mn = max2(m, mx * sc2);
+    const float ms = mn == kNegInf ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - ms);
+    const bool grew = mn > m;
+    m = mn;
+    f32x4 p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], sc2, -ms));
+    l = fmaf(l, f, (p[0] + p[1]) + (p[2] + p[3]));
+    if (__any(grew)) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
+    const frag4 pf = __builtin_convertvector(p, frag4);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = mma4(vt[d], pf, o[d]);
+  }
+  join_sets<T, DP, 16, 1, 4>(a, smem, o, m, l, row_of, a.splits > 1 ? a.part + ((int64_t)work * a.splits + split) * 16 * (a.D + 2) : nullptr, b, 0, wave);
+}
+// Joins the splits (at most kMaxSplits) of a row: one workgroup per row.  Lane x of every wave holds split x's factor; the waves take
+// the splits in turn, a lane two channels of them, and are added up in wave order.  Everything is asked for at once: the time is that
+// of one trip to memory.
+constexpr int kMaxSplits = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
   __shared__ float2 sums[4][64];
@@ -549,16 +715,19 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
   const int x = min(lane, a.splits - 1);
   const float m = lane < a.splits ? p[x * step + (int64_t)M * a.D + r] : kNegInf;
   const float l = p[x * step + (int64_t)M * a.D + M + r];
+  const int ch = min(lane * 2, a.D - 2);
+  float2 v[kMaxSplits / 4];
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 4; ++i) v[i] = *reinterpret_cast<const float2 *>(p + min(i * 4 + wave, a.splits - 1) * step + (int64_t)r * a.D + ch);
   const float mx = wave_max(m);
   const float w = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mx);
   const float sum = wave_sum(m == kNegInf ? 0.f : l * w);
-  const int ch = min(lane * 2, a.D - 2);
   float2 o = {0.f, 0.f};
-  for (int i = wave; i < a.splits; i += 4) {
-    const float2 v = *reinterpret_cast<const float2 *>(p + i * step + (int64_t)r * a.D + ch);
-    const float f = __shfl(w, i, 64);
-    o.x += f == 0.f ? 0.f : v.x * f;
-    o.y += f == 0.f ? 0.f : v.y * f;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 4; ++i) {                     // a split that is not there has a factor of 0
+    const float f = __shfl(w, i * 4 + wave, 64);
+    o.x += f == 0.f ? 0.f : v[i].x * f;
+    o.y += f == 0.f ? 0.f : v[i].y * f;
   }
   sums[wave][lane] = o;
   __syncthreads();
@@ -1057,9 +1226,8 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------------------------------ host
 // Tile shapes.  16-bit: 64 rows x 64 keys as 2 x 2 waves of 32 x 32 (every LDS fragment feeds two products); fp32, whose products take 16
-// times as long per fragment: 64 rows x 32 keys as 4 x 1 waves of 16 x 32.  Groups of up to 16 rows (one token of a few heads) take
-// 16 rows x 64 keys, the four waves sharing out the keys by 16: half of the second product's slots stay empty there, but such
-// calls wait for memory, and two workgroups fit a CU (against 128 keys a tile, 32 a wave: TBD).
+// times as long per fragment: 64 rows x 32 keys as 4 x 1 waves of 16 x 32.  Groups of up to 16 rows (one token of a few heads) have a
+// kernel of their own: half of the second product's k-elements stay empty there, but such calls wait for memory.
 constexpr int kFewRows = 16;
 static int fwd_rows(const AttnArgs &a) { return a.rows <= kFewRows ? 16 : 64; }
 static int fwd_keys(const AttnArgs &a, bool f32) { return a.rows > kFewRows && f32 ? 32 : 64; }
@@ -1074,7 +1242,7 @@ template <typename K> static int launch(K kernel, size_t lds, int64_t blocks, co
 }
 template <typename T, int DP> static int launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t s) {
   const char *what = "block_attention";
-  if (a.rows <= kFewRows) return launch(attend_fwd_kernel<T, DP, 16, 1, 4, 1>, FwdTile<T, DP, 16, 1, 4, 1>::body + list_bytes(a), blocks, a, s, what);
+  if (a.rows <= kFewRows) return launch(attend_few_kernel<T, DP, (sizeof(T) == 4 && DP > 64 ? 2 : 4)>, FewTile<T, DP>::body + list_bytes(a), blocks, a, s, what);
   if constexpr (sizeof(T) == 4) return launch(attend_fwd_kernel<T, DP, 16, 4, 1, 2>, FwdTile<T, DP, 16, 4, 1, 2>::body + list_bytes(a), blocks, a, s, what);
   else return launch(attend_fwd_kernel<T, DP, 32, 2, 2, 1>, FwdTile<T, DP, 32, 2, 2, 1>::body + list_bytes(a), blocks, a, s, what);
 }
@@ -1154,7 +1322,7 @@ static FwdPlan fwd_plan(const AttnArgs &a, bool f32) {
   const int64_t tiles = cdiv((int64_t)a.cap << a.lb, fwd_keys(a, f32));
   int64_t n = cdiv(2 * kNumCU, p.works > 0 ? p.works : 1);
   if (n > tiles / 2) n = tiles / 2;
-  p.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  p.splits = (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
   p.part = p.splits > 1 ? round_up((size_t)p.works * p.splits * fwd_rows(a) * (a.D + 2) * 4, 256) : 0;
   return p;
 }
