@@ -612,8 +612,8 @@ class ResizeFlowFn(torch.autograd.Function):
 # ----------------------------------------------------------------------------------------------- frame attention
 # Token tensors (B, N, H, D) in fp32, bf16 or fp16; the kernels read them through (batch, token, head) strides, so views of
 # (B, H, N, D) tensors and slices of a cache need no copy as long as channels are dense and rows start on 16 bytes.
+# Their autograd nodes call no operation that autocast would change, so they do without its wrappers (10 us a step).
 _DT = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
-_plain_fwd = torch.amp.custom_fwd(device_type="cuda")
 
 
 def _tokens_device(what, *tensors):
@@ -689,7 +689,6 @@ def _rotate(x, positions, sections, base, interleaved, inverse):
 
 class RotatePositionsFn(torch.autograd.Function):
     @staticmethod
-    @_plain_fwd
     def forward(ctx, x, positions, sections, base, interleaved):
         ctx.meta = (sections, base, interleaved)
         ctx.save_for_backward(positions)
@@ -697,7 +696,6 @@ class RotatePositionsFn(torch.autograd.Function):
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    @_bwd
     def backward(ctx, g):
         positions, = ctx.saved_tensors
         return _rotate(g, positions, *ctx.meta, True), None, None, None, None
@@ -794,7 +792,6 @@ class BlockAttentionFn(torch.autograd.Function):
     statistic."""
 
     @staticmethod
-    @_plain_fwd
     def forward(ctx, q, k, v, blocks, visible, block, q_block, scale):
         qc, kc, vc = _rows16(q), _rows16(k), _rows16(v)
         out, lse = _attend(qc, kc, vc, blocks, visible, block, q_block, scale, True)
@@ -805,7 +802,6 @@ class BlockAttentionFn(torch.autograd.Function):
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    @_bwd
     def backward(ctx, g_out, _g_lse):
         q, k, v, blocks, visible, out, lse = ctx.saved_tensors
         block, q_block, scale = ctx.meta
