@@ -144,6 +144,27 @@ template <int S> __device__ __forceinline__ float column_max(float x) {
   const u32x2 b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
   return max2(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+// Bit `row` + 4 (lane / S) of a uniform mask.  S = 32: as a lane mask that the scalar unit makes, which leaves one vector instruction per
+// masked score of three (four bits instead of two would cost the scalar unit more than that: fp32 backward 138 -> 144 us).
+template <int S> __device__ __forceinline__ bool key_seen(unsigned part, int row) {
+  if constexpr (S == 32) {
+    const unsigned lo = (unsigned)((int)(part << (31 - row)) >> 31), hi = (unsigned)((int)(part << (27 - row)) >> 31);
+    return __builtin_amdgcn_inverse_ballot_w64((uint64_t)hi << 32 | lo);
+  } else return (part >> (threadIdx.x % 64 / 16 * 4 + row)) & 1;
+}
+// The running maximum need not be the maximum: any reference r with the scores at most 8 above it (in log2 units) keeps exp2(score - r) <= 256
+// far from every type's limits, and it costs no accuracy, since all sums are of floating-point numbers.  So the sums and outputs so far are
+// scaled only where a score passes the reference by more (64 tiles of random scores, 32 rows a wave: in 1 or 2 tiles instead of about 45).
+// A NaN becomes the reference, and with it the whole row.
+template <int S, typename O> __device__ __forceinline__ void raise_reference(float mx, float &m, float &l, O &o) {
+  if (__any(!(mx <= m + 8.f))) {
+    const float mn = max2(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.f : mn));
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int d = 0; d < (int)(sizeof(O) / sizeof(o[0])); ++d) o[d] *= f;
+  }
+}
 // all but the last N LDS-DMAs of this wave have landed and every LDS read of it has been served; then the workgroup meets
 // (by the builtin: a wait in inline assembly is unknown to the compiler, which then waits again, for the tile that is on its way)
 template <int N> __device__ __forceinline__ void tile_barrier() {
@@ -483,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     for (int c = 0; c < KC; ++c) qf[c] = -qf[c];
   }
   acc o[DT];
-  float m = kNegInf, l = 0.f;                                    // maximum in log2 units, sum of exp2(score - maximum)
+  float m = kNegInf, l = 0.f;                                    // reference in log2 units, sum of exp2(score - reference)
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = acc(0.f);
   if (nt > 0) nxt = keys.finish(raw);
@@ -518,21 +539,17 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     // this wave's keys of the mask
     const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32));
     if (part != ~0u) {
-      const unsigned seen = part >> (g * 4);
 #pragma unroll
       for (int u = 0; u < KU; ++u)
 #pragma unroll
-        for (int e = 0; e < H::AE; ++e) sc[u][e] = (seen >> (u * S + H::row(e))) & 1 ? sc[u][e] : kNegInf;
+        for (int e = 0; e < H::AE; ++e) sc[u][e] = key_seen<S>(part, u * S + H::row(e)) ? sc[u][e] : kNegInf;
     }
     float mx = max2(sc[0][0], sc[0][1]);
 #pragma unroll
     for (int e = 2; e < E; ++e) mx = max2(mx, sc[e / H::AE][e % H::AE]);
     mx = column_max<S>(mx);
-    const float mn = max2(m, mx * sc2);
-    const float ms = mn == kNegInf ? 0.f : mn;                   // nothing seen yet: exp2(-inf - 0) = 0
-    const float f = __builtin_amdgcn_exp2f(m - ms);              // exactly 1 while the maximum stays
-    const bool grew = mn > m;
-    m = mn;
+    raise_reference<S>(mx * sc2, m, l, o);
+    const float ms = m == kNegInf ? 0.f : m;                     // nothing seen yet: exp2(-inf - 0) = 0
     float sum = 0.f;
     frag pf[PF];
 #pragma unroll
@@ -541,11 +558,7 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
       sum += p;
       pf[e / 8][e % 8] = (T)p;
     }
-    l = fmaf(l, f, sum);
-    if (__any(grew)) {                                           // no maximum moved in most tiles behind the first ones
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= f;
-    }
+    l += sum;
 #pragma unroll
     for (int i = 0; i < NV; ++i) o[i / PF] = mma(i < AH ? vf[i % AH] : v_frag(i), pf[i % PF], o[i / PF]);
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
@@ -659,7 +672,7 @@ __global__ __launch_bounds__(256, OCC) void attend_few_kernel(AttnArgs a) {
           vf[c] = __builtin_bit_cast(frag, w);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[e] = (part >> (g * 4 + e)) & 1 ? sc[e] : kNegInf;
+        for (int e = 0; e < 4; ++e) sc[e] = key_seen<16>(part, e) ? sc[e] : kNegInf;
       }
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
@@ -677,19 +690,12 @@ __global__ __launch_bounds__(256, OCC) void attend_few_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) vt[d] = col_frag4<T, DP>(img, d * 16, lane);
     const float mx = column_max<16>(max2(max2(sc[0], sc[1]), max2(sc[2], sc[3])));
-    const float mn = max2(m, mx * sc2);
-    const float ms = mn == kNegInf ? 0.f : mn;
-    const float f = __builtin_amdgcn_exp2f(m - ms);
-    const bool grew = mn > m;
-    m = mn;
+    raise_reference<16>(mx * sc2, m, l, o);
+    const float ms = m == kNegInf ? 0.f : m;
     f32x4 p;
 #pragma unroll
     for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], sc2, -ms));
-    l = fmaf(l, f, (p[0] + p[1]) + (p[2] + p[3]));
-    if (__any(grew)) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= f;
-    }
+    l += (p[0] + p[1]) + (p[2] + p[3]);
     const frag4 pf = __builtin_convertvector(p, frag4);
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = mma4(vt[d], pf, o[d]);
@@ -903,6 +909,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     issue(0, cur);
     raw = keys.load(TK / 64);
   }
+  const float c2 = a.c == 0.f ? 1e-30f : a.c, hidden = c2 < 0.f ? kPosInf : kNegInf;   // their product has to be -inf
   acc o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = acc(0.f);
@@ -945,12 +952,15 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     if (t + 1 < nt) issue(t + 1, nxt);                           // behind the transposing reads, as in the forward
     raw = keys.load((t + 2) * TK / 64);
     frag gf[PF];
-    const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32)), seen = part >> (g * 4);
+    const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32));
+    if (part != ~0u) {                                           // an unseen key's products are those of zeros: its probability has to become 0
+#pragma unroll
+      for (int e = 0; e < KU * H::AE; ++e) sc[e / H::AE][e % H::AE] = key_seen<S>(part, e / H::AE * S + H::row(e % H::AE)) ? sc[e / H::AE][e % H::AE] : hidden;
+    }
 #pragma unroll
     for (int e = 0; e < KU * H::AE; ++e) {
       const int u = e / H::AE, x = e % H::AE;
-      float p = __builtin_amdgcn_exp2f(fmaf(sc[u][x], a.c, -lse2));
-      p = (seen >> (u * S + H::row(x))) & 1 ? p : 0.f;           // an unseen key's products are those of zeros
+      const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][x], c2, -lse2));
       float ds = p * (dp[u][x] - delta);
       if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= a.scale;   // fp16: small score gradients; else the scale comes last
       gf[e / 8][e % 8] = (T)ds;
