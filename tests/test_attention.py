@@ -393,6 +393,38 @@ def test_block_attention(case, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [1.0, -0.7, 0.0])
+@pytest.mark.parametrize("q_block", [1, 64])
+def test_scores_that_rise_and_scales(q_block, scale, dtype):
+    """Scores that climb by 60 along the keys, in small and large steps (a running maximum that moves all the time), and scales of any
+    sign.  A negative scale is that of the turned queries."""
+    g = torch.Generator().manual_seed(23)
+    b, nq, nk, hq, hk, d = 1, 64, 700, 2, 1, 64
+    u = rnd(g, d)
+    u = u / u.norm()
+    steps = torch.rand(nk, generator=g) * (torch.rand(nk, generator=g) < 0.1)
+    ramp = steps.cumsum(0) / steps.sum() * 60 * (1 if scale >= 0 else -1)
+    q = (u + rnd(g, b, nq, hq, d, scale=0.02)).to(dtype)
+    k = (ramp[:, None, None] * u + rnd(g, b, nk, hk, d, scale=0.1)).to(dtype)
+    v, do = rnd(g, b, nk, hk, d, dtype=dtype), rnd(g, b, nq, hq, d, dtype=dtype)
+    vis = (torch.rand(b, nk, generator=g) < 0.8).float()
+    groups = -(-nq // q_block)
+    blocks = torch.arange(11).int().expand(b, hk, groups, 11).contiguous()
+    reach = ref_reach(blocks, nq, nk, 64, q_block, vis, b, hk)
+    sign = -1 if scale < 0 else 1
+    r = ref_attention(sign * q, k, v, reach, abs(scale), do)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    out, lse = A.block_attention(*leaves, blocks.to(DEV), vis.to(DEV), 64, q_block, scale=scale, return_lse=True)
+    inside(out, r["out"], r["out_tol"], "out")
+    inside(lse, r["lse"], r["lse_tol"], "lse")
+    dq, dk, dv = torch.autograd.grad(out, leaves, do.to(DEV))
+    inside(dq, sign * r["dq"], r["dq_tol"], "dq")
+    inside(dk, r["dk"], r["dk_tol"], "dk")
+    inside(dv, r["dv"], r["dv_tol"], "dv")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_gradients_against_differences(dtype):
     """Central differences of the 64-bit plain form along random directions."""
     g = torch.Generator().manual_seed(5)
