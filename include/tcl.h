@@ -290,24 +290,27 @@ int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, c
 
 /*   out = softmax(scale q k^T) v over the visible keys of the blocks chosen for the query's group; a query that sees no key gets 0 and
  *   lse = -inf.  visible as in tcl_block_means; blocks (B,Hkv,S,top_k) int32: an index outside [0, nb) is no block, a repeated one
- *   counts once, order does not matter.  lse (B,Hq,Nq) fp32, natural logarithm, nullable (the backward pass needs it).
+ *   counts once, order does not matter.  lse (B,Hq,Nq) fp32, natural logarithm, nullable (the backward pass needs it).  out_lo (16-bit
+ *   types, nullable): laid out like out, what its rounding took from it, for the backward pass.
  *   Limits: top_k <= 2048, nb <= 65,536, q_block * G <= 2^20 (q_block beyond Nq counts as Nq).
  *   Contents of invisible keys do not matter (NaN and infinities included).  A workspace of 0 bytes may be NULL. */
 size_t tcl_block_attention_fwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block,
                                                int64_t q_block);
 int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh,
                             const void *v, int64_t v_sb, int64_t v_sn, int64_t v_sh, const float *visible, const int32_t *blocks,
-                            void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, float *lse,
+                            void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, void *out_lo, float *lse,
                             int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block, int64_t q_block,
                             double scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);
-/*   grad_out like out -> g_q, g_k, g_v (each nullable); out and lse are the forward's.  Every row of the gradients is written (zero
+/*   grad_out like out -> g_q, g_k, g_v (each nullable); out, out_lo (nullable: gradients of rows with few keys are
+ *   less exact) and lse are the forward's.  Every row of the gradients is written (zero
  *   for keys that no group sees), except in an empty attention (B, Nq or Nk of 0), where nothing is.  No atomics on values:
  *   the same inputs give the same bits. */
 size_t tcl_block_attention_bwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block,
                                                int64_t q_block);
 int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64_t g_sn, int64_t g_sh, const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
                             const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_sn, int64_t v_sh,
-                            const float *visible, const int32_t *blocks, const void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, const float *lse,
+                            const float *visible, const int32_t *blocks, const void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, const void *out_lo,
+                            const float *lse,
                             void *g_q, int64_t gq_sb, int64_t gq_sn, int64_t gq_sh, void *g_k, int64_t gk_sb, int64_t gk_sn, int64_t gk_sh,
                             void *g_v, int64_t gv_sb, int64_t gv_sn, int64_t gv_sh,
                             int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block, int64_t q_block,

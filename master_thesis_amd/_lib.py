@@ -57,9 +57,9 @@ SIGNATURES = {
     "tcl_select_blocks_workspace_bytes": (_SZ, [_I64] * 7),
     "tcl_select_blocks": (_INT, [_P] + [_I64] * 3 + [_P] * 3 + [_I64] * 8 + [_INT, _P, _SZ, _P]),
     "tcl_block_attention_fwd_workspace_bytes": (_SZ, [_I64] * 9),
-    "tcl_block_attention_fwd": (_INT, ([_P] + [_I64] * 3) * 3 + [_P] * 2 + [_P] + [_I64] * 3 + [_P] + [_I64] * 9 + [_c.c_double, _INT, _P, _SZ, _P]),
+    "tcl_block_attention_fwd": (_INT, ([_P] + [_I64] * 3) * 3 + [_P] * 2 + [_P] + [_I64] * 3 + [_P] * 2 + [_I64] * 9 + [_c.c_double, _INT, _P, _SZ, _P]),
     "tcl_block_attention_bwd_workspace_bytes": (_SZ, [_I64] * 9),
-    "tcl_block_attention_bwd": (_INT, ([_P] + [_I64] * 3) * 4 + [_P] * 2 + [_P] + [_I64] * 3 + [_P] + ([_P] + [_I64] * 3) * 3 + [_I64] * 9
+    "tcl_block_attention_bwd": (_INT, ([_P] + [_I64] * 3) * 4 + [_P] * 2 + [_P] + [_I64] * 3 + [_P] * 2 + ([_P] + [_I64] * 3) * 3 + [_I64] * 9
                                 + [_c.c_double, _INT, _P, _SZ, _P]),
 }
 

@@ -92,7 +92,7 @@ struct AttnArgs {
   const void *q, *k, *v, *dout;
   const float *vis;
   const int32_t *blocks;
-  void *out, *dq, *dk, *dv;
+  void *out, *lo, *dq, *dk, *dv;   // lo: what rounding took from out, laid out like it
   float *lse;                      // (B, Hq, Nq), natural logarithm
   float *delta;                    // (B, Hq, Nq)
   uint32_t *inv;                   // (B, Hkv, nb, words): which groups chose the block
@@ -410,10 +410,15 @@ __device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const t
       continue;
     }
     const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // nothing seen: zero; NaN stays NaN
-    typename Vec4<T>::type y;
+    const int64_t at = (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch;
+    typename Vec4<T>::type y, lo;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (T)(x4[e] * inv);
-    *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.out) + (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch) = y;
+    for (int e = 0; e < 4; ++e) {
+      y[e] = (T)(x4[e] * inv);
+      lo[e] = (T)(x4[e] * inv - (float)y[e]);
+    }
+    *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.out) + at) = y;
+    if (sizeof(T) == 2 && a.lo) *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.lo) + at) = lo;
     if (ch == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx + __builtin_log2f(sum)) * kLn2;
   }
 }
@@ -745,9 +750,15 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
   }
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
   if (lane * 2 < a.D) {
-    T *y = reinterpret_cast<T *>(a.out) + (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch;
-    y[0] = (T)(o.x * inv);
-    y[1] = (T)(o.y * inv);
+    const int64_t at = (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch;
+    T *y = reinterpret_cast<T *>(a.out) + at, *lo = reinterpret_cast<T *>(a.lo) + at;
+    const T y0 = (T)(o.x * inv), y1 = (T)(o.y * inv);
+    y[0] = y0;
+    y[1] = y1;
+    if (sizeof(T) == 2 && a.lo) {
+      lo[0] = (T)(o.x * inv - (float)y0);
+      lo[1] = (T)(o.y * inv - (float)y1);
+    }
   }
   if (lane == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx + __builtin_log2f(sum)) * kLn2;
 }
@@ -761,7 +772,10 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
 template <typename T> struct PScale { static constexpr float bits = 0.f, inv = 1.f; };
 template <> struct PScale<_Float16> { static constexpr float bits = 10.f, inv = 0x1p-10f; };
 
-// delta of every row: 16 lanes per row, 8 channels each; and the plan of the key / value gradients (inv, chosen) is cleared
+// delta of every row: 16 lanes per row, 8 channels each.  The output is taken as it was before its rounding (out + lo): delta is
+// subtracted from products of its own size, and with few keys a rounded output's error is the largest of the gradient (2 to 16
+// keys: error of dq and dk 1.6 to 2.9 times that of their own rounding, 1.4 to 1.5 so; the smaller part of it is left, that of the
+// score gradients as operands).  And the plan of the key / value gradients (inv, chosen) is cleared
 template <typename T>
 __global__ __launch_bounds__(256) void attend_delta_kernel(AttnArgs a) {
   const int64_t id = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
@@ -776,8 +790,10 @@ __global__ __launch_bounds__(256) void attend_delta_kernel(AttnArgs a) {
     typedef typename Vec8<T>::type frag;
     const frag x = *reinterpret_cast<const frag *>(reinterpret_cast<const T *>(a.dout) + (int64_t)b * a.sdo.b + (int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h + ch);
     const frag y = *reinterpret_cast<const frag *>(reinterpret_cast<const T *>(a.out) + (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch);
+    frag z = {};
+    if (sizeof(T) == 2 && a.lo) z = *reinterpret_cast<const frag *>(reinterpret_cast<const T *>(a.lo) + (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf((float)x[e], (float)y[e], sum);
+    for (int e = 0; e < 8; ++e) sum = fmaf((float)x[e], (float)y[e] + (float)z[e], sum);
   }
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -951,7 +967,10 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     if (t + 1 < nt) issue(t + 1, nxt);                           // behind the transposing reads, as in the forward
     raw = keys.load((t + 2) * TK / 64);
-    frag gf[PF];
+    // 16-bit heads of up to 64 channels: what rounding takes from a score gradient is multiplied too.  Alone it makes an error of 1.4
+    // times that of the result's own rounding, but with few channels, whose keys lie along the sum, of 1.5 to 1.6.
+    constexpr bool TWO = sizeof(T) == 2 && DP <= 64;
+    frag gf[PF], gl[TWO ? PF : 1];
     const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32));
     if (part != ~0u) {                                           // an unseen key's products are those of zeros: its probability has to become 0
 #pragma unroll
@@ -964,9 +983,14 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
       float ds = p * (dp[u][x] - delta);
       if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= a.scale;   // fp16: small score gradients; else the scale comes last
       gf[e / 8][e % 8] = (T)ds;
+      if constexpr (TWO) gl[e / 8][e % 8] = (T)(ds - (float)gf[e / 8][e % 8]);
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) o[i / PF] = mma(i < AH ? ka[i % AH] : k_frag(i), gf[i % PF], o[i / PF]);
+    for (int i = 0; i < NV; ++i) {
+      const frag k = i < AH ? ka[i % AH] : k_frag(i);
+      o[i / PF] = mma(k, gf[i % PF], o[i / PF]);
+      if constexpr (TWO) o[i / PF] = mma(k, gl[i % PF], o[i / PF]);
+    }
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
     cur = nxt;
     nxt = keys.finish(raw);
@@ -1362,7 +1386,7 @@ extern "C" size_t tcl_block_attention_fwd_workspace_bytes(int64_t B, int64_t Nq,
 
 extern "C" int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh,
                                        const void *v, int64_t v_sb, int64_t v_sn, int64_t v_sh, const float *visible, const int32_t *blocks,
-                                       void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, float *lse,
+                                       void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, void *out_lo, float *lse,
                                        int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block, int64_t q_block,
                                        double scale, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   AttnArgs a{};
@@ -1370,9 +1394,9 @@ extern "C" int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn
   if (rc != TCL_OK) return rc;
   if (B == 0 || Nq == 0) return TCL_OK;
   TCL_REQUIRE(q && out && blocks && (Nk == 0 || (k && v)), TCL_ERR_ARG, "block_attention: null pointer");
-  a.q = q; a.k = k; a.v = v; a.vis = visible; a.blocks = blocks; a.out = out; a.lse = lse;
+  a.q = q; a.k = k; a.v = v; a.vis = visible; a.blocks = blocks; a.out = out; a.lo = out_lo; a.lse = lse;
   a.sq = Str{q_sb, q_sn, q_sh}; a.sk = Str{k_sb, k_sn, k_sh}; a.sv = Str{v_sb, v_sn, v_sh}; a.so = Str{o_sb, o_sn, o_sh};
-  TCL_REQUIRE(rows16(q, a.sq, dtype) && (Nk == 0 || (rows16(k, a.sk, dtype) && rows16(v, a.sv, dtype))) && rows16(out, a.so, dtype), TCL_ERR_ARG,
+  TCL_REQUIRE(rows16(q, a.sq, dtype) && (Nk == 0 || (rows16(k, a.sk, dtype) && rows16(v, a.sv, dtype))) && rows16(out, a.so, dtype) && aligned(out_lo, 16), TCL_ERR_ARG,
               "block_attention: rows must start on 16 bytes");
   TCL_REQUIRE(near_rows(a.sk) && near_rows(a.sv), TCL_ERR_UNSUPPORTED, "block_attention: keys lie more than 2^22 elements apart");
   const bool f32 = dtype == TCL_DT_F32;
@@ -1403,7 +1427,8 @@ extern "C" size_t tcl_block_attention_bwd_workspace_bytes(int64_t B, int64_t Nq,
 
 extern "C" int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64_t g_sn, int64_t g_sh, const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
                                        const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_sn, int64_t v_sh,
-                                       const float *visible, const int32_t *blocks, const void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, const float *lse,
+                                       const float *visible, const int32_t *blocks, const void *out, int64_t o_sb, int64_t o_sn, int64_t o_sh, const void *out_lo,
+                                       const float *lse,
                                        void *g_q, int64_t gq_sb, int64_t gq_sn, int64_t gq_sh, void *g_k, int64_t gk_sb, int64_t gk_sn, int64_t gk_sh,
                                        void *g_v, int64_t gv_sb, int64_t gv_sn, int64_t gv_sh,
                                        int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block, int64_t q_block,
@@ -1413,11 +1438,11 @@ extern "C" int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64
   if (rc != TCL_OK) return rc;
   if (B == 0 || Nq == 0 || Nk == 0) return TCL_OK;             // the caller zeroes gradients of an empty attention
   TCL_REQUIRE(grad_out && q && k && v && out && blocks && lse, TCL_ERR_ARG, "block_attention backward: null pointer");
-  a.q = q; a.k = k; a.v = v; a.dout = grad_out; a.vis = visible; a.blocks = blocks; a.out = const_cast<void *>(out); a.lse = const_cast<float *>(lse);
+  a.q = q; a.k = k; a.v = v; a.dout = grad_out; a.vis = visible; a.blocks = blocks; a.out = const_cast<void *>(out); a.lo = const_cast<void *>(out_lo); a.lse = const_cast<float *>(lse);
   a.dq = g_q; a.dk = g_k; a.dv = g_v;
   a.sq = Str{q_sb, q_sn, q_sh}; a.sk = Str{k_sb, k_sn, k_sh}; a.sv = Str{v_sb, v_sn, v_sh}; a.so = Str{o_sb, o_sn, o_sh}; a.sdo = Str{g_sb, g_sn, g_sh};
   a.sdq = Str{gq_sb, gq_sn, gq_sh}; a.sdk = Str{gk_sb, gk_sn, gk_sh}; a.sdv = Str{gv_sb, gv_sn, gv_sh};
-  TCL_REQUIRE(rows16(q, a.sq, dtype) && rows16(k, a.sk, dtype) && rows16(v, a.sv, dtype) && rows16(out, a.so, dtype) && rows16(grad_out, a.sdo, dtype) &&
+  TCL_REQUIRE(rows16(q, a.sq, dtype) && rows16(k, a.sk, dtype) && rows16(v, a.sv, dtype) && rows16(out, a.so, dtype) && rows16(grad_out, a.sdo, dtype) && aligned(out_lo, 16) &&
               (!g_q || rows16(g_q, a.sdq, dtype)) && (!g_k || rows16(g_k, a.sdk, dtype)) && (!g_v || rows16(g_v, a.sdv, dtype)), TCL_ERR_ARG,
               "block_attention backward: rows must start on 16 bytes");
   TCL_REQUIRE(near_rows(a.sk) && near_rows(a.sv), TCL_ERR_UNSUPPORTED, "block_attention backward: keys lie more than 2^22 elements apart");

@@ -146,13 +146,13 @@ def test_c_entries_refuse_without_gpu():
     assert means(n=0) == 0 and means(d=12) == 5 and means(d=136) == 5 and means(block=96) == 5 and means(k=off) == 2 and means(st=12) == 2
     sel = lambda nb=4, top=1, d=8, hk=1, ws=one, wsb=1 << 20: lib.tcl_select_blocks(one, 16, 8, 8, one, one, one, 1, 2, 2, hk, d, nb, top, 1, 0, ws, wsb, None)   # noqa: E731
     assert sel(nb=16385) == 5 and sel(top=0) == 1 and sel(hk=3) == 1 and sel(d=9) == 5 and sel(nb=600, wsb=8) == 3 and sel(nb=600, ws=None) == 3
-    fwd = lambda q=one, nk=64, d=8, top=1, block=64, qb=1, hk=1, wsb=0, dt=0, b=1: lib.tcl_block_attention_fwd(   # noqa: E731
-        q, 16, 8, 8, one, 512, 8, 8, one, 512, 8, 8, None, one, one, 16, 8, 8, None, b, 2, nk, 2, hk, d, top, block, qb, 1.0, dt, one, wsb, None)
+    fwd = lambda q=one, nk=64, d=8, top=1, block=64, qb=1, hk=1, wsb=0, dt=0, b=1, lo=None: lib.tcl_block_attention_fwd(   # noqa: E731
+        q, 16, 8, 8, one, 512, 8, 8, one, 512, 8, 8, None, one, one, 16, 8, 8, lo, None, b, 2, nk, 2, hk, d, top, block, qb, 1.0, dt, one, wsb, None)
     assert fwd(b=0) == 0
     assert fwd(d=4) == 5 and fwd(d=136) == 5 and fwd(top=2049) == 5 and fwd(block=32) == 5 and fwd(nk=64 * 65537) == 5 and fwd(dt=9) == 5
-    assert fwd(hk=3) == 1 and fwd(qb=0) == 1 and fwd(q=off) == 2 and fwd(q=None) == 2 and fwd(nk=1 << 16, top=100) == 3
+    assert fwd(hk=3) == 1 and fwd(qb=0) == 1 and fwd(q=off) == 2 and fwd(lo=off) == 2 and fwd(q=None) == 2 and fwd(nk=1 << 16, top=100) == 3
     need = lib.tcl_block_attention_bwd_workspace_bytes(1, 2, 64, 2, 1, 8, 1, 64, 1)
-    bwd = lambda wsb, go=one: lib.tcl_block_attention_bwd(go, 16, 8, 8, one, 16, 8, 8, one, 512, 8, 8, one, 512, 8, 8, None, one, one, 16, 8, 8, one,   # noqa: E731
+    bwd = lambda wsb, go=one: lib.tcl_block_attention_bwd(go, 16, 8, 8, one, 16, 8, 8, one, 512, 8, 8, one, 512, 8, 8, None, one, one, 16, 8, 8, None, one,   # noqa: E731
                                                           None, 0, 0, 0, None, 0, 0, 0, None, 0, 0, 0, 1, 2, 64, 2, 1, 8, 1, 64, 1, 1.0, 0, one, wsb, None)
     assert bwd(need - 1) == 3 and bwd(need, go=None) == 2
     assert lib.tcl_block_attention_fwd_workspace_bytes(1, 1, 1 << 20, 8, 1, 128, 64, 128, 1) > 256     # few rows, many keys: split
@@ -421,6 +421,35 @@ def test_scores_that_rise_and_scales(q_block, scale, dtype):
     inside(dq, sign * r["dq"], r["dq_tol"], "dq")
     inside(dk, r["dk"], r["dk_tol"], "dk")
     inside(dv, r["dv"], r["dv_tol"], "dv")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nk,d", [(2, 128), (3, 64), (5, 128), (16, 128), (200, 32)])
+def test_gradients_of_few_keys(nk, d, dtype):
+    """With few keys, rowsum(dout o out) nearly cancels against its terms: the roundings that are allowed are those of the
+    probabilities and the score gradients as operands and that of the result, NOT that of the forward's output.  A rounding is off by at most
+    h of its value, by h / sqrt(3) of it or less in the square mean, and the roundings are independent: the squares of the errors
+    of a whole tensor add up to the sum of the variances."""
+    g = torch.Generator().manual_seed(nk + d)
+    nq, h = 512, half(dtype)
+    q, k, v, do = rnd(g, 1, nq, 1, d, dtype=dtype, scale=1.5), rnd(g, 1, nk, 1, d, dtype=dtype), rnd(g, 1, nk, 1, d, dtype=dtype), rnd(g, 1, nq, 1, d, dtype=dtype)
+    top = -(-nk // 64)
+    blocks = torch.arange(top).int().expand(1, 1, nq // 64, top).contiguous()
+    leaves = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(A.block_attention(*leaves, blocks.to(DEV)), leaves, do.to(DEV))
+    Q, K, V, G = (t[0, :, 0].double() for t in (q, k, v, do))
+    c = d ** -0.5
+    P = torch.softmax(Q @ K.T * c, -1)
+    dP = G @ V.T
+    dS = P * (dP - (P * dP).sum(-1, keepdim=True)) * c
+    of_delta = (P * dP).square().sum(-1, keepdim=True) * c * c
+    for name, x, want, var in (("dq", got[0], dS @ K, dS.square() @ K.square() + of_delta * (P @ K).square()),
+                               ("dk", got[1], dS.T @ Q, dS.square().T @ Q.square() + (P.square() * of_delta).T @ Q.square()),
+                               ("dv", got[2], P.T @ G, P.square().T @ G.square())):
+        bound = (h / 3 ** 0.5) * (want.square() + var).sum().sqrt().item()
+        err = (x[0, :, 0].double().cpu() - want).norm().item()
+        assert err <= bound, (name, err, bound)
 
 
 @pytest.mark.gpu
