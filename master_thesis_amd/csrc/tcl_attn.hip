@@ -772,6 +772,15 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
 template <typename T> struct PScale { static constexpr float bits = 0.f, inv = 1.f; };
 template <> struct PScale<_Float16> { static constexpr float bits = 10.f, inv = 0x1p-10f; };
 
+// TWO: what rounding takes from a 16-bit operand (a score gradient; for dV a probability) is multiplied too.  Rounded once, it makes an error
+// of 1.4 times that of the result's own rounding; where the terms are few or lie along the sum (fewer than 64 channels) up to 1.6.  There
+// two parts are taken: in calls so small that it costs nothing (up to 2^20 scores: a few microseconds of a call of 150), and for heads of
+// fewer than 64 channels.
+template <typename T> static bool two_parts(const AttnArgs &a) {
+  const int64_t keys = (int64_t)a.cap << a.lb;
+  return sizeof(T) == 2 && (a.D < 64 || (int64_t)a.B * a.Nq * a.Hq * (keys < a.Nk ? keys : a.Nk) <= 1 << 20);
+}
+
 // delta of every row: 16 lanes per row, 8 channels each.  The output is taken as it was before its rounding (out + lo): delta is
 // subtracted from products of its own size, and with few keys a rounded output's error is the largest of the gradient (2 to 16
 // keys: error of dq and dk 1.6 to 2.9 times that of their own rounding, 1.4 to 1.5 so; the smaller part of it is left, that of the
@@ -852,7 +861,7 @@ template <typename T, int DP, int S, int WM, int WN> struct DqTile {
   static constexpr size_t join = (size_t)WN * M * LO * 4;
   static constexpr size_t body = tiles > join ? tiles : join;
 };
-template <typename T, int DP, int S, int WM, int WN, int OCC>
+template <typename T, int DP, int S, int WM, int WN, int OCC, bool TWO>
 __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   typedef DqTile<T, DP, S, WM, WN> F;
   typedef Shape<S> H;
@@ -967,9 +976,6 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     if (t + 1 < nt) issue(t + 1, nxt);                           // behind the transposing reads, as in the forward
     raw = keys.load((t + 2) * TK / 64);
-    // 16-bit heads of up to 64 channels: what rounding takes from a score gradient is multiplied too.  Alone it makes an error of 1.4
-    // times that of the result's own rounding, but with few channels, whose keys lie along the sum, of 1.5 to 1.6.
-    constexpr bool TWO = sizeof(T) == 2 && DP <= 64;
     frag gf[PF], gl[TWO ? PF : 1];
     const unsigned part = (unsigned)(cur.mask >> (((t * TK) & 63) + wn * 32));
     if (part != ~0u) {                                           // an unseen key's products are those of zeros: its probability has to become 0
@@ -1034,7 +1040,7 @@ template <typename T, int DP> struct DkvTile {
   // behind the tiles: where a row lies in q and dout (in 16 bytes), lse and delta, the list of groups
   static constexpr size_t bytes = body + kBatch * 16 + 32 * kWindow * 4;
 };
-template <typename T, int DP>
+template <typename T, int DP, bool TWO>
 __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
   typedef DkvTile<T, DP> F;
   typedef Pieces<T, DP, F::TR> P;
@@ -1211,7 +1217,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
           qa[d] = col_frag<T, DP>(qrows, 0, d * 16, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
-        frag pf, gf;
+        frag pf, gf, pl, gl;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -1221,6 +1227,10 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
             if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= each;
             pf[u * 4 + e] = (T)p;
             gf[u * 4 + e] = (T)ds;
+            if constexpr (TWO) {
+              pl[u * 4 + e] = (T)(p - (float)pf[u * 4 + e]);
+              gl[u * 4 + e] = (T)(ds - (float)gf[u * 4 + e]);
+            }
           }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -1234,6 +1244,10 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
           }
           gv[d] = mma(x, pf, gv[d]);
           gk[d] = mma(y, gf, gk[d]);
+          if constexpr (TWO) {
+            gv[d] = mma(x, pl, gv[d]);
+            gk[d] = mma(y, gl, gk[d]);
+          }
         }
       }
     }
@@ -1280,19 +1294,19 @@ template <typename T, int DP> static int launch_fwd(const AttnArgs &a, int64_t b
   if constexpr (sizeof(T) == 4) return launch(attend_fwd_kernel<T, DP, 16, 4, 1, 2>, FwdTile<T, DP, 16, 4, 1, 2>::body + list_bytes(a), blocks, a, s, what);
   else return launch(attend_fwd_kernel<T, DP, 32, 2, 2, 1>, FwdTile<T, DP, 32, 2, 2, 1>::body + list_bytes(a), blocks, a, s, what);
 }
-template <typename T, int DP> static int launch_dq(AttnArgs a, hipStream_t s) {
+template <typename T, int DP, bool TWO> static int launch_dq(AttnArgs a, hipStream_t s) {
   const char *what = "block_attention backward (queries)";
   const bool few = a.rows <= 32;
   a.chunks = (int)cdiv(a.rows, few ? 32 : 64);
   const int64_t blocks = (int64_t)a.B * a.Hkv * a.S * a.chunks;
-  if (few) return launch(attend_dq_kernel<T, DP, 16, 2, 2, 1>, DqTile<T, DP, 16, 2, 2>::body + list_bytes(a), blocks, a, s, what);
-  if constexpr (sizeof(T) == 4) return launch(attend_dq_kernel<T, DP, 16, 4, 1, 1>, DqTile<T, DP, 16, 4, 1>::body + list_bytes(a), blocks, a, s, what);
-  else return launch(attend_dq_kernel<T, DP, 32, 2, 2, 2>, DqTile<T, DP, 32, 2, 2>::body + list_bytes(a), blocks, a, s, what);
+  if (few) return launch(attend_dq_kernel<T, DP, 16, 2, 2, 1, TWO>, DqTile<T, DP, 16, 2, 2>::body + list_bytes(a), blocks, a, s, what);
+  if constexpr (sizeof(T) == 4) return launch(attend_dq_kernel<T, DP, 16, 4, 1, 1, TWO>, DqTile<T, DP, 16, 4, 1>::body + list_bytes(a), blocks, a, s, what);
+  else return launch(attend_dq_kernel<T, DP, 32, 2, 2, 2, TWO>, DqTile<T, DP, 32, 2, 2>::body + list_bytes(a), blocks, a, s, what);
 }
-template <typename T, int DP> static int launch_dkv(const AttnArgs &a, hipStream_t s) {
+template <typename T, int DP, bool TWO> static int launch_dkv(const AttnArgs &a, hipStream_t s) {
   const char *what = "block_attention backward (keys)";
   const int64_t blocks = ((int64_t)a.nb << (a.lb - 6)) * a.B * a.Hkv;
-  return launch(attend_dkv_kernel<T, DP>, DkvTile<T, DP>::bytes, blocks, a, s, what);
+  return launch(attend_dkv_kernel<T, DP, TWO>, DkvTile<T, DP>::bytes, blocks, a, s, what);
 }
 
 // head sizes are padded to a multiple of 32 in LDS and registers
@@ -1308,13 +1322,14 @@ template <typename T> static int fwd_by_dim(const AttnArgs &a, int64_t blocks, h
   TCL_BY_DIM(T, CALL)
 #undef CALL
 }
+// a head of up to 32 channels is always taken in two parts, fp32 never
 template <typename T> static int dq_by_dim(const AttnArgs &a, hipStream_t s) {
-#define CALL(T, DP) (launch_dq<T, DP>(a, s))
+#define CALL(T, DP) (DP == 32 || two_parts<T>(a) ? launch_dq<T, DP, sizeof(T) == 2>(a, s) : launch_dq<T, DP, sizeof(T) == 2 && DP == 32>(a, s))
   TCL_BY_DIM(T, CALL)
 #undef CALL
 }
 template <typename T> static int dkv_by_dim(const AttnArgs &a, hipStream_t s) {
-#define CALL(T, DP) (launch_dkv<T, DP>(a, s))
+#define CALL(T, DP) (DP == 32 || two_parts<T>(a) ? launch_dkv<T, DP, sizeof(T) == 2>(a, s) : launch_dkv<T, DP, sizeof(T) == 2 && DP == 32>(a, s))
   TCL_BY_DIM(T, CALL)
 #undef CALL
 }

@@ -360,6 +360,9 @@ ATTEND = [  # b, nq, nk, hq, hk, d, block, q_block, top, masked, layout, lists
     (2, 70, 20, 2, 1, 64, 128, 16, 3, False, "dense", "ascending"),            # the last block of 128 ends in its first half
     (1, 1, 150, 8, 2, 128, 128, 1, 2, True, "heads_first", "mixed"),
     (1, 65, 300, 1, 1, 32, 128, 64, 3, True, "dense", "ascending"),
+    (1, 600, 530, 4, 2, 128, 64, 64, 9, True, "dense", "ascending"),           # more than 2^20 scores: operands of the gradients in one part
+    (1, 1100, 500, 2, 1, 64, 64, 16, 8, False, "heads_first", "mixed"),
+    (2, 300, 1000, 2, 2, 96, 128, 100, 8, True, "cache", "mixed"),
 ]
 
 
