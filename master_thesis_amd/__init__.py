@@ -10,6 +10,7 @@ The sub-modules mirror the reference's module and function names for this path:
     master_thesis_amd.models.thesis_alignment <- models/thesis_alignment.py (the alignment network around the HIP cost volume)
     master_thesis_amd.models.cpn_original <- models/cpn_original.py (CM_Module; CPNOriginal around the HIP warp + matching)
     master_thesis_amd.utils.movement      <- utils/movement.py (on the device)
+    master_thesis_amd.utils.attention     (no counterpart there: attention of a target's tokens over many reference frames)
     master_thesis_amd.runners / schedulers <- the static step functions and sequence schedulers of the three runners
 
 `install_dropin()` registers them under the reference's own names (`utils.correlation`, `utils.flow`, and the

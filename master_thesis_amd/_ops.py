@@ -5,6 +5,7 @@ it, outputs and workspaces come from torch's caching allocator, and the call is 
 stream of the tensor's device.  There is no CPU path: a CPU tensor raises.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -639,7 +640,7 @@ def _side(what, t, dev, dtypes, shape):
         raise TclError("%s must be %s (got %s)" % (what, " or ".join(str(d) for d in dtypes), t.dtype))
     if tuple(t.shape) != tuple(shape):
         raise ValueError("%s must be %s, got %s" % (what, tuple(shape), tuple(t.shape)))
-    return t.detach().contiguous()
+    return t if t.is_contiguous() and not t.requires_grad else t.detach().contiguous()
 
 
 def _visible(visible, dev, b, n):
@@ -770,6 +771,11 @@ def select_blocks(q, means, counts, top_k, q_block=64):
     return blocks
 
 
+@functools.lru_cache(maxsize=256)
+def _attend_bytes(*sizes):
+    return _lib.lib().tcl_block_attention_fwd_workspace_bytes(*sizes)
+
+
 def _attend(q, k, v, blocks, visible, block, q_block, scale, want_lse, want_lo=False):
     """-> out (B,Nq,Hq,D), lse (B,Hq,Nq) | None, what out's rounding took | None; q, k, v as _rows16 left them."""
     dev = q.device
@@ -779,7 +785,7 @@ def _attend(q, k, v, blocks, visible, block, q_block, scale, want_lse, want_lo=F
     out = torch.empty((b, nq, hq, d), dtype=q.dtype, device=dev)
     lse = torch.empty((b, hq, nq), dtype=torch.float32, device=dev) if want_lse else None
     lo = torch.empty_like(out) if want_lo and q.dtype != torch.float32 else None
-    nbytes = _lib.lib().tcl_block_attention_fwd_workspace_bytes(b, nq, nk, hq, hk, d, top, block, q_block)
+    nbytes = _attend_bytes(b, nq, nk, hq, hk, d, top, block, q_block)
     ws = _workspace(nbytes, dev) if nbytes else None      # only for few tokens, whose keys are split
     with _on(dev):
         _lib.call("tcl_block_attention_fwd", q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), _p(visible),
@@ -844,5 +850,5 @@ def block_attention(q, k, v, blocks, visible=None, block=64, q_block=64, scale=N
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = BlockAttentionFn.apply(q, k, v, bl, vis, block, q_block, scale)
     else:
-        out, lse, _ = _attend(_rows16(q.detach()), _rows16(k.detach()), _rows16(v.detach()), bl, vis, block, q_block, scale, return_lse)
+        out, lse, _ = _attend(_rows16(q), _rows16(k), _rows16(v), bl, vis, block, q_block, scale, return_lse)
     return (out, lse) if return_lse else out

@@ -24,7 +24,7 @@ struct MeansArgs {
 
 // One wave per (item, head, block).  A row takes D / VE lanes (16-byte loads), so 64 / (D / VE) rows are read per step, four steps in
 // flight; every lane sums its channels of its rows in 64 bits, the row groups are joined through LDS.
-// Bound: memory (K once).
+// Bound: memory (K once): 32 x 15,900 keys x 2 heads of 64 bf16 channels 24 us, 5.5 TB/s; one frame of 1,590 keys 5 us, a launch.
 template <typename T>
 __global__ __launch_bounds__(256) void block_means_kernel(MeansArgs a) {
   constexpr int VE = 16 / sizeof(T);
@@ -286,7 +286,8 @@ template <int R> __device__ __forceinline__ void choose(const uint64_t (&key)[R]
 // in LDS, and every wave chooses for four of the groups.  DIRECT: the groups' few queries are summed here; otherwise the sums come
 // from the workspace.  DS: slices of 16 channels.
 // Against scores written out and read back by a second kernel 330 -> 111 us (65,536 groups x 256 blocks, one wave per 16 groups with the keys
-// in registers), -> 89 us with the waves sharing the work as here.
+// in registers), -> 89 us with the waves sharing the work as here;
+// the products alone take 29 at the rate of a large 64-bit product, the comparisons the rest.
 template <typename T, bool DIRECT, int R, int DS>
 __global__ __launch_bounds__(256) void select_fused_kernel(SelectArgs a) {
   constexpr int LD = R * 64 + 16;
