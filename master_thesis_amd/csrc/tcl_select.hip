@@ -286,7 +286,8 @@ template <int R> __device__ __forceinline__ void choose(const uint64_t (&key)[R]
 // in LDS, and every wave chooses for four of the groups.  DIRECT: the groups' few queries are summed here; otherwise the sums come
 // from the workspace.  DS: slices of 16 channels.
 // Against scores written out and read back by a second kernel 330 -> 111 us (65,536 groups x 256 blocks, one wave per 16 groups with the keys
-// in registers), -> 89 us with the waves sharing the work as here;
+// in registers), -> 89 us with the waves sharing the products, -> 80 with
+// the sums of the queries shared out too; two or four choices of a wave side by side are slower (93, 96);
 // the products alone take 29 at the rate of a large 64-bit product, the comparisons the rest.
 template <typename T, bool DIRECT, int R, int DS>
 __global__ __launch_bounds__(256) void select_fused_kernel(SelectArgs a) {
@@ -304,19 +305,32 @@ __global__ __launch_bounds__(256) void select_fused_kernel(SelectArgs a) {
     typedef typename SelVec<T, 4>::type vec;
     const T *qp = reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sb + (int64_t)hk * a.G * a.sh;
     const int n0 = (int)((int64_t)s * a.q_block), n1 = (int)min((int64_t)a.N, (int64_t)n0 + a.q_block);
+    // a quarter of the channels per wave (summed by all four, the sums cost as much as the products); they meet where the keys come later
+    constexpr int LQ = DS * 16 + 2, MY = DS / 4;
+    double *lq = reinterpret_cast<double *>(lkey), sum[MY][4];
 #pragma unroll
-    for (int c = 0; c < DS; ++c)
+    for (int c = 0; c < MY; ++c)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q[c][e] = 0.0;
+      for (int e = 0; e < 4; ++e) sum[c][e] = 0.0;
     for (int n = n0; n < n1; ++n)
       for (int h = 0; h < a.G; ++h)
 #pragma unroll
-        for (int c = 0; c < DS; ++c) {
-          const int ch = c * 16 + g * 4;
+        for (int c = 0; c < MY; ++c) {
+          const int ch = (wave * MY + c) * 16 + g * 4;
           const vec t = *reinterpret_cast<const vec *>(qp + (int64_t)n * a.sn + (int64_t)h * a.sh + min(ch, a.D - 4));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) q[c][e] += ch < a.D ? (double)(float)t[e] : 0.0;
+          for (int e = 0; e < 4; ++e) sum[c][e] += ch < a.D ? (double)(float)t[e] : 0.0;
         }
+#pragma unroll
+    for (int c = 0; c < MY; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lq[r * LQ + (wave * MY + c) * 16 + g * 4 + e] = sum[c][e];
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < DS; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[c][e] = lq[r * LQ + c * 16 + g * 4 + e];
+    __syncthreads();
   } else {
 #pragma unroll
     for (int c = 0; c < DS; ++c) {
@@ -419,7 +433,9 @@ constexpr int kDirectRows = 8;          // groups of up to 8 query rows are summ
 static size_t pooled_bytes(int64_t B, int64_t Hkv, int64_t S, int64_t D) { return round_up((size_t)(B * Hkv * S * D) * sizeof(double), 256); }
 
 template <typename T, bool DIRECT, int R> static int launch_fused_r(const SelectArgs &a, dim3 wg, hipStream_t s) {
-  const size_t lds = (size_t)16 * (R * 64 + 16) * sizeof(uint64_t);
+  // a row's keys, or its queries' sum before them
+  const int keys = R * 64 + 16, sums = DIRECT ? (a.D <= 64 ? 4 : 8) * 16 + 2 : 0;
+  const size_t lds = (size_t)16 * (keys > sums ? keys : sums) * sizeof(uint64_t);
   const auto kernel = a.D <= 64 ? select_fused_kernel<T, DIRECT, R, 4> : select_fused_kernel<T, DIRECT, R, 8>;
   TCL_REQUIRE(lds_ready((const void *)kernel, lds), TCL_ERR_LAUNCH, "select_blocks: the device refuses %zu bytes of LDS", lds);
   hipLaunchKernelGGL(kernel, wg, dim3(256), lds, s, a);
