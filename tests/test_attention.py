@@ -285,7 +285,8 @@ def ref_select(q, means, counts, top, q_block):
 @pytest.mark.parametrize("b,n,h,hk,d,nb,top,q_block,dtype", [
     (1, 1, 1, 1, 8, 1, 1, 1, torch.float32), (2, 5, 2, 2, 64, 15, 4, 1, torch.bfloat16), (1, 130, 4, 2, 40, 64, 9, 64, torch.float16),
     (2, 70, 2, 1, 72, 65, 70, 16, torch.float32), (1, 33, 8, 1, 128, 300, 24, 1, torch.bfloat16), (1, 20, 1, 1, 96, 513, 31, 3, torch.float32),
-    (1, 3, 2, 1, 64, 1500, 64, 1, torch.float16), (1, 2, 1, 1, 32, 5000, 600, 2, torch.float32), (3, 200, 1, 1, 16, 257, 1, 1000, torch.float32)])
+    (1, 3, 2, 1, 64, 1500, 64, 1, torch.float16), (1, 2, 1, 1, 32, 5000, 600, 2, torch.float32), (3, 200, 1, 1, 16, 257, 1, 1000, torch.float32),
+    (1, 33, 4, 2, 128, 30, 5, 1, torch.float32), (2, 18, 8, 1, 96, 64, 12, 1, torch.float16)])
 def test_select_blocks(b, n, h, hk, d, nb, top, q_block, dtype):
     g = torch.Generator().manual_seed(nb * 7 + n)
     q, means = rnd(g, b, n, h, d, dtype=dtype), rnd(g, b, hk, nb, d, scale=0.2)
@@ -453,6 +454,49 @@ def test_gradients_of_few_keys(nk, d, dtype):
         bound = (h / 3 ** 0.5) * (want.square() + var).sum().sqrt().item()
         err = (x[0, :, 0].double().cpu() - want).norm().item()
         assert err <= bound, (name, err, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_block", [1, 64])
+def test_the_longest_list_of_blocks(q_block, dtype):
+    """2,048 chosen blocks of 2,100, the widest head: the most shared memory that a call can ask for."""
+    g = torch.Generator().manual_seed(2048 + q_block)
+    nq, nb, top, d = 40, 2100, 2048, 128
+    nk = nb * 64 - 5
+    (q, k, v), dev, blocks, vis = attention_case(g, 1, nq, nk, 1, 1, d, 64, q_block, top, dtype, True, "dense", "mixed")
+    do = rnd(g, 1, nq, 1, d, dtype=dtype)
+    r = ref_attention(q, k, v, ref_reach(blocks, nq, nk, 64, q_block, vis, 1, 1), d ** -0.5, do)
+    leaves = [t.detach().requires_grad_(True) for t in dev]
+    out = A.block_attention(*leaves, blocks.to(DEV), vis.to(DEV), 64, q_block)
+    inside(out, r["out"], r["out_tol"], "out")
+    for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, do.to(DEV))):
+        inside(got, r[name], r[name + "_tol"], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_some_inputs(dtype):
+    """Each input alone, keys that are the values, a cotangent without strides, the same graph twice: the bits of the whole step."""
+    g = torch.Generator().manual_seed(91)
+    (q, k, v), dev, blocks, vis = attention_case(g, 2, 90, 200, 4, 2, 40, 64, 32, 3, dtype, True)
+    bl, vd = blocks.to(DEV), vis.to(DEV)
+    leaves = [t.detach().requires_grad_(True) for t in dev]
+    out = A.block_attention(*leaves, bl, vd, 64, 32)
+    ones = torch.ones_like(out)
+    whole = torch.autograd.grad(out, leaves, ones, retain_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(whole, torch.autograd.grad(out.sum(), leaves, retain_graph=True)))
+    assert all(torch.equal(x, y) for x, y in zip(whole, torch.autograd.grad(out, leaves, ones)))
+    for i in range(3):
+        some = [t.detach().requires_grad_(j == i) for j, t in enumerate(dev)]
+        assert torch.equal(torch.autograd.grad(A.block_attention(*some, bl, vd, 64, 32), some[i], ones)[0], whole[i])
+    kv = torch.randn(2, 200, 2, 40, generator=g).to(dtype).to(DEV).requires_grad_(True)
+    both = [leaves[0], kv, kv.detach().clone().requires_grad_(True)]
+    _, dk, dv = torch.autograd.grad(A.block_attention(*both, bl, vd, 64, 32), both, ones)
+    assert torch.equal(torch.autograd.grad(A.block_attention(leaves[0], kv, kv, bl, vd, 64, 32), kv, ones)[0], dk + dv)
+    with pytest.raises(RuntimeError):
+        grad = torch.autograd.grad(A.block_attention(*leaves, bl, vd, 64, 32), leaves[0], ones, create_graph=True)[0]
+        torch.autograd.grad(grad.sum(), leaves[0])
 
 
 @pytest.mark.gpu
