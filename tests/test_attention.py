@@ -364,6 +364,8 @@ ATTEND = [  # b, nq, nk, hq, hk, d, block, q_block, top, masked, layout, lists
     (1, 600, 530, 4, 2, 128, 64, 64, 9, True, "dense", "ascending"),           # more than 2^20 scores: operands of the gradients in one part
     (1, 1100, 500, 2, 1, 64, 64, 16, 8, False, "heads_first", "mixed"),
     (2, 300, 1000, 2, 2, 96, 128, 100, 8, True, "cache", "mixed"),
+    (1, 3000, 100, 8, 1, 32, 64, 64, 2, True, "dense", "ascending"),           # few keys, many rows: their gradients are split
+    (2, 700, 70, 2, 2, 128, 128, 16, 1, False, "heads_first", "mixed"),
 ]
 
 
