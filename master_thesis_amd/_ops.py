@@ -613,7 +613,7 @@ class ResizeFlowFn(torch.autograd.Function):
 # ----------------------------------------------------------------------------------------------- frame attention
 # Token tensors (B, N, H, D) in fp32, bf16 or fp16; the kernels read them through (batch, token, head) strides, so views of
 # (B, H, N, D) tensors and slices of a cache need no copy as long as channels are dense and rows start on 16 bytes.
-# Their autograd nodes call no operation that autocast would change, so they do without its wrappers (10 us a step).
+# Their autograd nodes call no operation that autocast would change, so they do without its wrappers and their host time.
 _DT = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
 
