@@ -18,7 +18,8 @@
 //
 // Statistics (running maximum, sum, lse, rowsum(dout o out)) and all accumulators are fp32.  16-bit inputs: the probabilities and the
 // score gradients are rounded to the inputs' type as operands of the second product (half a step of it relative to each
-// term, the size of the rounding of the result itself); nothing else is rounded before the end.
+// term, the size of the rounding of the result itself; fp16, whose steps are absolute below 2^-14, after scaling: PScale, GradRange);
+// nothing else is rounded before the end.
 #include "tcl_common.h"
 
 namespace tcl {
@@ -777,6 +778,31 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
 template <typename T> struct PScale { static constexpr float bits = 0.f, inv = 1.f; };
 template <> struct PScale<_Float16> { static constexpr float bits = 10.f, inv = 0x1p-10f; };
 
+// fp16: a score gradient lies anywhere between the cotangent's size and that over the number of keys, and fp16 steps are absolute below 2^-14 (a
+// cotangent of 10^-3 and 4,096 keys, as they are: dq and dk off by 2 %).  So the gradients of a row (dq) or a key (dk) are multiplied by a power of
+// two of their own, which the sums are divided by at the end.  It starts high (a result of 2^-25 needs no term below 2^-60) and falls, like the
+// reference of a softmax, whenever one of the gradients passes 2^15; the largest of those is then just above 2^10, so what rounding takes from a term is half
+// a step of it or 2^-35 of the largest.  Nothing but the row's (key's) own terms decides it.
+template <typename T> struct GradRange { static constexpr bool on = false; };
+template <> struct GradRange<_Float16> { static constexpr bool on = true; static constexpr float start = 0x1p60f, limit = 0x1p15f; };
+// ds: a lane's gradients, times f; o: its column's sums, times f
+template <int S, typename V, int N, typename O, int DT> __device__ __forceinline__ void fit_range(V (&ds)[N], float &f, O (&o)[DT]) {
+  typedef GradRange<_Float16> R;
+  constexpr int E = sizeof(V) / 4;
+  float mx = 0.f;
+#pragma unroll
+  for (int e = 0; e < N * E; ++e) mx = fmaxf(mx, fabsf(ds[e / E][e % E]));
+  if (__any(mx > R::limit)) {
+    const float top = column_max<S>(mx);
+    const float g = top > R::limit && top < kPosInf ? __builtin_ldexpf(1.f, 11 - __builtin_amdgcn_frexp_expf(top)) : 1.f;
+    f *= g;
+#pragma unroll
+    for (int u = 0; u < N; ++u) ds[u] *= g;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] *= g;
+  }
+}
+
 // TWO: what rounding takes from a 16-bit operand (a score gradient; for dV a probability) is multiplied too.  Rounded once, it makes an error
 // of 1.4 times that of the result's own rounding; where the terms are few or lie along the sum (fewer than 64 channels) up to 1.6.  There
 // two parts are taken: in calls so small that it costs nothing (up to 2^20 scores: a few microseconds of a call of 150), and for heads of
@@ -942,6 +968,8 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   }
   const float c2 = a.c == 0.f ? 1e-30f : a.c, hidden = c2 < 0.f ? kPosInf : kNegInf;   // their product has to be -inf
   acc o[DT];
+  float range = 1.f;
+  if constexpr (GradRange<T>::on) range = GradRange<T>::start;
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = acc(0.f);
   if (nt > 0) nxt = keys.finish(raw);
@@ -992,8 +1020,13 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     for (int e = 0; e < KU * H::AE; ++e) {
       const int u = e / H::AE, x = e % H::AE;
       const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][x], c2, -lse2));
-      float ds = p * (dp[u][x] - delta);
-      if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= a.scale;   // fp16: small score gradients; else the scale comes last
+      sc[u][x] = p * (dp[u][x] - delta);
+      if constexpr (GradRange<T>::on) sc[u][x] *= range;
+    }
+    if constexpr (GradRange<T>::on) fit_range<S>(sc, range, o);
+#pragma unroll
+    for (int e = 0; e < KU * H::AE; ++e) {
+      const float ds = sc[e / H::AE][e % H::AE];
       gf[e / 8][e % 8] = (T)ds;
       if constexpr (TWO) gl[e / 8][e % 8] = (T)(ds - (float)gf[e / 8][e % 8]);
     }
@@ -1010,10 +1043,12 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   float *jo = reinterpret_cast<float *>(smem);                   // [WN][M][LO]
   __syncthreads();
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+  for (int d = 0; d < DT; ++d) {
+    if constexpr (GradRange<T>::on) o[d] *= 1.f / range;         // every key set has one of its own
 #pragma unroll
     for (int e = 0; e < H::AE; e += 4)
       *reinterpret_cast<f32x4 *>(jo + (wn * M + wm * S + col) * F::LO + d * S + H::row(e) + g * 4) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+  }
   __syncthreads();
   for (int id = tid; id < M * (a.D / 4); id += 256) {
     const int r = (int)a.by_d4.div((unsigned)id), ch = (id - r * (a.D / 4)) * 4;
@@ -1022,7 +1057,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     f32x4 x = *reinterpret_cast<const f32x4 *>(jo + r * F::LO + ch);
 #pragma unroll
     for (int w = 1; w < WN; ++w) x += *reinterpret_cast<const f32x4 *>(jo + (w * M + r) * F::LO + ch);
-    x *= sizeof(T) == 2 && PScale<T>::bits > 0.f ? 1.f : a.scale;
+    x *= a.scale;
     typename Vec4<T>::type y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
@@ -1091,9 +1126,8 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
   const char *qb = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.q) + (int64_t)b * a.sq.b);
   const char *db = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.dout) + (int64_t)b * a.sdo.b);
   const int chunks = a.D / P::I::VE;
-  // fp16: scale on each score gradient (they stay small); else once, on the sums
-  const float each = sizeof(T) == 2 && PScale<T>::bits > 0.f ? a.scale * PScale<T>::inv : 1.f;
-  const float k_scale = sizeof(T) == 2 && PScale<T>::bits > 0.f ? 1.f : a.scale;
+  float range = 1.f;                                             // of this lane's key; P's own factor is part of it
+  if constexpr (GradRange<T>::on) range = GradRange<T>::start * PScale<T>::inv;
   f32x4 gk[DT], gv[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) gk[d] = gv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1233,14 +1267,18 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][e], a.c, -ls[u][e]));
-            float ds = p * (dp[u][e] - de[u][e]);
-            if (sizeof(T) == 2 && PScale<T>::bits > 0.f) ds *= each;
+            dp[u][e] = p * (dp[u][e] - de[u][e]);
+            if constexpr (GradRange<T>::on) dp[u][e] *= range;
             pf[u * 4 + e] = (T)p;
-            gf[u * 4 + e] = (T)ds;
-            if constexpr (TWO) {
-              pl[u * 4 + e] = (T)(p - (float)pf[u * 4 + e]);
-              gl[u * 4 + e] = (T)(ds - (float)gf[u * 4 + e]);
-            }
+            if constexpr (TWO) pl[u * 4 + e] = (T)(p - (float)pf[u * 4 + e]);
+          }
+        if constexpr (GradRange<T>::on) fit_range<16>(dp, range, gk);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            gf[u * 4 + e] = (T)dp[u][e];
+            if constexpr (TWO) gl[u * 4 + e] = (T)(dp[u][e] - (float)gf[u * 4 + e]);
           }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -1264,6 +1302,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
   }
   // a lane holds 4 channels of its key per 16: the 4 quarters together write 32 (fp32: 64) bytes of 16 rows at a time
   if (key >= a.Nk) return;
+  const float k_scale = GradRange<T>::on ? a.scale * PScale<T>::inv / range : a.scale;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     T *out = reinterpret_cast<T *>(which ? a.dv : a.dk);

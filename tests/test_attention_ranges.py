@@ -1,0 +1,77 @@
+"""Frame attention where the numbers themselves are hard: small and large cotangents, long sums, probabilities that lie binades apart.
+
+Bounds are statistical, over whole tensors: a rounding is off by at most h of its value (half a step of the type), by h / sqrt(3) of it or less in the
+square mean, the roundings are independent, and what the rounding of the exact result costs is computed, not estimated."""
+import pytest
+import torch
+
+from master_thesis_amd.utils import attention as A
+from .test_attention import DEV, half, rnd
+
+
+def dense(q, k, v, do, scale):
+    """One head whose queries see every key -> P, dP - delta, dS, in the type of the inputs"""
+    p = torch.softmax(q @ k.T * scale, -1)
+    dp = do @ v.T
+    t = dp - (p * dp).sum(-1, keepdim=True)
+    return p, t, p * t * scale
+
+
+def gradients(q, k, v, do, q_block=64, scale=None):
+    """of block_attention, every block chosen: q, k, v, do (N, D) on the CPU -> dq, dk, dv (N, D) in 64 bits"""
+    top = -(-k.shape[0] // 64)
+    blocks = torch.arange(top, device=DEV).int().expand(1, 1, -(-q.shape[0] // q_block), top).contiguous()
+    leaves = [t.to(DEV)[None, :, None].requires_grad_(True) for t in (q, k, v)]
+    out = A.block_attention(*leaves, blocks, q_block=q_block, scale=scale)
+    return [t[0, :, 0].double() for t in torch.autograd.grad(out, leaves, do.to(DEV)[None, :, None])]
+
+
+def own_rounding(x, dtype):
+    return (x.to(dtype).double() - x).norm().item()
+
+
+def check(name, got, want, var, dtype):
+    """The error of the result's own rounding and that of one rounding of every operand (var: the squares of the terms, summed); a twentieth for the fp32 sums"""
+    own, h = own_rounding(want, dtype), half(dtype)
+    bound, err = 1.05 * (own ** 2 + h * h / 3 * var.sum().item()) ** 0.5, (got - want).norm().item()
+    size = want.norm().item()
+    assert err <= bound, "%s: error %.3g, own rounding %.3g, bound %.3g" % (name, err / size, own / size, bound / size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("nk,d,q_block", [(4096, 128, 64), (1024, 64, 64), (1024, 64, 1), (200, 24, 64)])
+def test_fp16_gradients_of_small_cotangents(nk, d, q_block, size):
+    """A cotangent of 10^-3 and thousands of keys: the score gradients lie far below 2^-14, the results do not."""
+    g = torch.Generator().manual_seed(nk + d)
+    dtype, nq = torch.float16, 512
+    q, k, v, do = rnd(g, nq, d, dtype=dtype, scale=1.5), rnd(g, nk, d, dtype=dtype), rnd(g, nk, d, dtype=dtype), rnd(g, nq, d, dtype=dtype, scale=size)
+    dq, dk, dv = gradients(q, k, v, do, q_block)
+    Q, K, V, G = (t.to(DEV).double() for t in (q, k, v, do))
+    p, _, ds = dense(Q, K, V, G, d ** -0.5)
+    check("dq", dq, ds @ K, ds.square() @ K.square(), dtype)
+    check("dk", dk, ds.T @ Q, ds.square().T @ Q.square(), dtype)
+    check("dv", dv, p.T @ G, p.square().T @ G.square(), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nk", [5, 700])
+def test_fp16_gradients_of_rows_of_all_sizes(nk):
+    """Rows whose cotangents lie 20 binades apart in one call, values so large that with few keys a score gradient passes fp16's largest number; the
+    keys (the queries) that it is multiplied by are small, and the results are ordinary numbers."""
+    g = torch.Generator().manual_seed(nk)
+    dtype, nq, d = torch.float16, 130, 64
+    sizes = torch.exp2(-20 * torch.rand(nq, 1, generator=g)) * 1000
+    v, do = rnd(g, nk, d, dtype=dtype, scale=1000), (rnd(g, nq, d) * sizes).to(dtype)
+    for big, small, which in ((100.0, 0.01, "dq"), (0.01, 100.0, "dk")):
+        q, k = rnd(g, nq, d, dtype=dtype, scale=big), rnd(g, nk, d, dtype=dtype, scale=small)
+        p, _, ds = dense(*(t.double() for t in (q, k, v, do)), d ** -0.5)
+        assert nk > 5 or ds.abs().max() > 2 ** 16
+        dq, dk, _ = gradients(q, k, v, do)
+        Q, K, ds = q.to(DEV).double(), k.to(DEV).double(), ds.to(DEV)
+        if which == "dq":                                                         # every row for itself
+            want, var = ds @ K, ds.square() @ K.square()
+            for i in range(nq):
+                check("dq %d" % i, dq[i], want[i], 15 * var[i], dtype)            # |sum of 5 errors|^2 <= 5 h^2 times the sum of squares
+        else:
+            check("dk", dk, ds.T @ Q, 15 * ds.square().T @ Q.square(), dtype)
