@@ -153,12 +153,18 @@ template <int S> __device__ __forceinline__ bool key_seen(unsigned part, int row
     return __builtin_amdgcn_inverse_ballot_w64((uint64_t)hi << 32 | lo);
   } else return (part >> (threadIdx.x % 64 / 16 * 4 + row)) & 1;
 }
-// The running maximum need not be the maximum: any reference r with the scores at most 8 above it (in log2 units) keeps exp2(score - r) <= 256
-// far from every type's limits, and it costs no accuracy, since all sums are of floating-point numbers.  So the sums and outputs so far are
-// scaled only where a score passes the reference by more (64 tiles of random scores, 32 rows a wave: in 1 or 2 tiles instead of about 45).
+// fp16 steps are absolute below 2^-14, so a probability is scaled up as an operand: in the forward, where those of a row are exp2(score - reference), by
+// 2^10 (unscaled, the tail of a long row is lost: 131,068 keys with 2^-25.2 of the largest each are 0.4 % of its weight and came out as zeros; scaled,
+// each loses 2^-35 of the largest at most), in the backward, where P <= 1, by 2^14.
+template <typename T> struct PScale { static constexpr float room = 8.f, fwd = 0.f, bits = 0.f, inv = 1.f; };
+template <> struct PScale<_Float16> { static constexpr float room = 4.f, fwd = 10.f, bits = 14.f, inv = 0x1p-14f; };
+
+// The running maximum need not be the maximum: any reference r with the scores at most `room` above it (in log2 units) keeps exp2(score - r) <= 256
+// (fp16: 16, scaled 2^14) far from every type's limits, and it costs no accuracy, since all sums are of floating-point numbers.  So the sums and outputs so
+// far are scaled only where a score passes the reference by more (64 tiles of random scores, 32 rows a wave: in 1 or 2 tiles instead of about 45).
 // A NaN becomes the reference, and with it the whole row.
-template <int S, typename O> __device__ __forceinline__ void raise_reference(float mx, float &m, float &l, O &o) {
-  if (__any(!(mx <= m + 8.f))) {
+template <int S, typename T, typename O> __device__ __forceinline__ void raise_reference(float mx, float &m, float &l, O &o) {
+  if (__any(!(mx <= m + PScale<T>::room))) {
     const float mn = max2(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.f : mn));
     m = mn;
     l *= f;
@@ -420,7 +426,7 @@ __device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const t
     }
     *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.out) + at) = y;
     if (sizeof(T) == 2 && a.lo) *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.lo) + at) = lo;
-    if (ch == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx + __builtin_log2f(sum)) * kLn2;
+    if (ch == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx - PScale<T>::fwd + __builtin_log2f(sum)) * kLn2;
   }
 }
 
@@ -515,7 +521,7 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     for (int c = 0; c < KC; ++c) qf[c] = -qf[c];
   }
   acc o[DT];
-  float m = kNegInf, l = 0.f;                                    // reference in log2 units, sum of exp2(score - reference)
+  float m = kNegInf, l = 0.f;                                    // reference in log2 units, sum of exp2(score - reference), scaled as P is
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = acc(0.f);
   if (nt > 0) nxt = keys.finish(raw);
@@ -559,8 +565,8 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 2; e < E; ++e) mx = max2(mx, sc[e / H::AE][e % H::AE]);
     mx = column_max<S>(mx);
-    raise_reference<S>(mx * sc2, m, l, o);
-    const float ms = m == kNegInf ? 0.f : m;                     // nothing seen yet: exp2(-inf - 0) = 0
+    raise_reference<S, T>(mx * sc2, m, l, o);
+    const float ms = (m == kNegInf ? 0.f : m) - PScale<T>::fwd;  // nothing seen yet: exp2(-inf - 0) = 0
     float sum = 0.f;
     frag pf[PF];
 #pragma unroll
@@ -701,8 +707,8 @@ __global__ __launch_bounds__(256, OCC) void attend_few_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) vt[d] = col_frag4<T, DP>(img, d * 16, lane);
     const float mx = column_max<16>(max2(max2(sc[0], sc[1]), max2(sc[2], sc[3])));
-    raise_reference<16>(mx * sc2, m, l, o);
-    const float ms = m == kNegInf ? 0.f : m;
+    raise_reference<16, T>(mx * sc2, m, l, o);
+    const float ms = (m == kNegInf ? 0.f : m) - PScale<T>::fwd;
     f32x4 p;
 #pragma unroll
     for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], sc2, -ms));
@@ -766,23 +772,20 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
       lo[1] = (T)(o.y * inv - (float)y1);
     }
   }
-  if (lane == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx + __builtin_log2f(sum)) * kLn2;
+  if (lane == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx - PScale<T>::fwd + __builtin_log2f(sum)) * kLn2;
 }
 
 // ------------------------------------------------------------------------------------------ backward
 // With P = exp(scale S - lse) and dP = dout V^T:  dV = P^T dout,  dS = scale P o (dP - delta),  delta = rowsum(dout o out),
 // dQ = dS K,  dK = dS^T Q.  dQ is summed per query tile (like the forward), dK and dV per key tile: two kernels that both recompute
 // S and dP, and no atomics, so a gradient does not depend on the order of the workgroups.
-//
-// fp16: P is scaled up by 2^10 as an operand (P <= 1; of 4096 equal keys each has 2^-12, and below 2^-14 fp16 loses bits).
-template <typename T> struct PScale { static constexpr float bits = 0.f, inv = 1.f; };
-template <> struct PScale<_Float16> { static constexpr float bits = 10.f, inv = 0x1p-10f; };
 
 // fp16: a score gradient lies anywhere between the cotangent's size and that over the number of keys, and fp16 steps are absolute below 2^-14 (a
 // cotangent of 10^-3 and 4,096 keys, as they are: dq and dk off by 2 %).  So the gradients of a row (dq) or a key (dk) are multiplied by a power of
 // two of their own, which the sums are divided by at the end.  It starts high (a result of 2^-25 needs no term below 2^-60) and falls, like the
 // reference of a softmax, whenever one of the gradients passes 2^15; the largest of those is then just above 2^10, so what rounding takes from a term is half
-// a step of it or 2^-35 of the largest.  Nothing but the row's (key's) own terms decides it.
+// a step of it or 2^-35 of the largest.  Nothing but the row's (key's) own terms decides it.  Measured: fp16 training step of 63,600 keys, dq 254 -> 267 us,
+// dk and dv 422 -> 428.
 template <typename T> struct GradRange { static constexpr bool on = false; };
 template <> struct GradRange<_Float16> { static constexpr bool on = true; static constexpr float start = 0x1p60f, limit = 0x1p15f; };
 // ds: a lane's gradients, times f; o: its column's sums, times f

@@ -75,3 +75,36 @@ def test_fp16_gradients_of_rows_of_all_sizes(nk):
                 check("dq %d" % i, dq[i], want[i], 15 * var[i], dtype)            # |sum of 5 errors|^2 <= 5 h^2 times the sum of squares
         else:
             check("dk", dk, ds.T @ Q, 15 * ds.square().T @ Q.square(), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q_block", [1, 64])
+def test_the_long_tail_of_a_row(q_block, dtype):
+    """131,068 equal keys about 25 binades below four others: together they carry 2^-10 of the weight, and all of the output.  (512 groups: no split of the
+    keys, in which the tail would be among its equals.)"""
+    nk, d, groups = 2048 * 64, 8, 512
+    q, k, v = torch.zeros(1, groups * q_block, 1, d, dtype=dtype), torch.zeros(1, nk, 1, d, dtype=dtype), torch.ones(1, nk, 1, d, dtype=dtype)
+    q[..., 0] = 1.0
+    k[0, [0, 16, 32, 48], 0, 0] = 17.47
+    v[0, [0, 16, 32, 48]] = 0
+    blocks = torch.arange(2048, device=DEV).int().expand(1, 1, groups, 2048).contiguous()
+    out, lse = A.block_attention(q.to(DEV), k.to(DEV), v.to(DEV), blocks, q_block=q_block, scale=1.0, return_lse=True)
+    s = k[0, :, 0, 0].double()
+    want = (torch.softmax(s, 0) * v[0, :, 0, 0].double()).sum().item()
+    # equal probabilities round alike (h), the result (h); a lane adds its equal ones up in 2^11 steps (2^-13)
+    assert (out.double() - want).abs().max().item() <= (2 * half(dtype) + 2.0 ** -12) * want
+    assert (lse.double() - torch.logsumexp(s, 0).item()).abs().max().item() <= 2.0 ** -13 + 32 * 2.0 ** -24
+
+
+@pytest.mark.gpu
+def test_fp16_value_gradient_of_an_unlikely_key():
+    """P = 1.4 2^-33 and a cotangent of 2^14: dv is 45 of fp16's smallest steps."""
+    q, k = torch.zeros(1, 1, 1, 8, dtype=torch.float16), torch.zeros(1, 2, 1, 8, dtype=torch.float16)
+    q[..., 0], k[0, 0, 0, 0] = 1.0, 22.54
+    v = torch.zeros_like(k).to(DEV).requires_grad_(True)
+    out = A.block_attention(q.to(DEV), k.to(DEV), v, torch.zeros(1, 1, 1, 1, dtype=torch.int32, device=DEV), scale=1.0)
+    dv, = torch.autograd.grad(out, v, torch.full_like(out, 2.0 ** 14))
+    want = torch.softmax(k[0, :, 0, 0].double(), 0) * 2.0 ** 14
+    # half a step each for the operand and the result; the score's rounding (33 log2 units)
+    assert (dv[0, 1, 0].double() - want[1].item()).abs().max().item() <= 2 * 2.0 ** -25 + 40 * 2.0 ** -24 * want[1].item()
