@@ -8,6 +8,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import TclError
@@ -632,6 +633,12 @@ def _tokens_device(what, *tensors):
     return dev
 
 
+def _no_tangents(what, *tensors):
+    """Forward-mode derivatives are refused here: calls that no backward pass will follow go past the autograd node, which would refuse them."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("%s has no forward-mode derivative" % what)
+
+
 def _side(what, t, dev, dtypes, shape):
     """A plan tensor (mask, block list, summary): on `dev`, of one of `dtypes`, of this shape; made dense."""
     if t.device != dev:
@@ -703,6 +710,7 @@ class RotatePositionsFn(torch.autograd.Function):
 
 
 def rotate_positions(x, positions, sections, base=10000.0, interleaved=False):
+    _no_tangents("rotate_positions", x, positions)
     dev = _tokens_device("rotate_positions", x)
     b, n, h, d = x.shape
     sections = tuple(int(s) for s in sections)
@@ -830,6 +838,7 @@ class BlockAttentionFn(torch.autograd.Function):
 
 
 def block_attention(q, k, v, blocks, visible=None, block=64, q_block=64, scale=None, return_lse=False):
+    _no_tangents("block_attention", q, k, v)
     if torch.is_autocast_enabled("cuda"):      # as torch's own attention: the operands of the products take the region's type
         q, k, v = (t.to(torch.get_autocast_dtype("cuda")) if t.is_floating_point() and t.is_cuda else t for t in (q, k, v))
     dev = _tokens_device("block_attention", q, k, v)

@@ -738,3 +738,36 @@ def test_long_cache_offsets_pass_31_bits():
     assert c[0, :nb - 4].abs().max() == 0 and int(c.sum()) == 300
     ref = tail[0, -(n % 128 or 128):, 0].double().mean(0)
     inside(m[0, 0, -1], ref, half(torch.float32) * ref.abs() + 1e-300, "means")
+
+
+# ------------------------------------------------------------------------------------------------ forward-mode derivatives
+def forward_mode_calls(dev):
+    x, pos, bl = torch.randn(1, 2, 1, 8, device=dev), torch.zeros(2, 1, device=dev), torch.zeros(1, 1, 1, 1, dtype=torch.int32, device=dev)
+    return x, [("rotate_positions", lambda d, x: A.rotate_positions(d, pos, (8,))), ("rotate_positions", lambda d, x: A.rotate_positions(x, d[:, :, 0, :1], (8,))),
+               ("block_attention", lambda d, x: A.block_attention(d, x, x, bl)), ("block_attention", lambda d, x: A.block_attention(x, d, x, bl)),
+               ("block_attention", lambda d, x: A.block_attention(x, x, d, bl))]
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent is never dropped: not with requires_grad, not without, not under no_grad, not by torch.func."""
+    from torch.autograd import forward_ad
+    x, calls = forward_mode_calls("cpu")
+    for what, call in calls:
+        for grad in (False, True):
+            with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                with pytest.raises(NotImplementedError, match=what):
+                    call(forward_ad.make_dual(x, torch.ones_like(x)), x)
+        with pytest.raises(NotImplementedError, match=what):
+            torch.func.jvp(lambda d: call(d, x), (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused_on_the_gpu():
+    from torch.autograd import forward_ad
+    x, calls = forward_mode_calls(DEV)
+    for what, call in calls:
+        with forward_ad.dual_level():
+            with pytest.raises(NotImplementedError, match=what):
+                call(forward_ad.make_dual(x, torch.ones_like(x)), x)
+            plain = call(x, x)                                                    # in a level, without a tangent: as ever
+        assert torch.equal(plain, call(x, x))
