@@ -1077,6 +1077,10 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
 // of four, three tiles ahead; where the rows lie is worked out for 512 of them at a time, not in the loop.
 constexpr int kWindow = 32;    // words of group bits taken at a time: up to 1024 groups in the list
 constexpr int kBatch = 512;    // rows located at a time
+// Rows after which an fp32 accumulator is added to the others: a serial sum of n random terms is off by about 0.4 sqrt(n / 2) 2^-24 of its size (measured:
+// 38 2^-24 for 16,000 rows, 10 so).  2,000 queries x 16 heads x 32 items, 512 keys of 2 heads of 64 channels: training step 5,262 -> 5,327 us.  16-bit
+// results have no use for it.
+constexpr unsigned kSerial = 512;
 
 template <typename T, int DP> struct DkvTile {
   static constexpr int M = 64, TR = 32, NB = sizeof(T) == 4 && DP > 64 ? 2 : 4;
@@ -1136,6 +1140,46 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
   for (int d = 0; d < DT; ++d) gk[d] = gv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   zero_pads<T, DP, TR>(smem, 2 * NB, chunks, wave);
 
+  // The sums to their rows (of a split: to its part).  A lane holds 4 channels of its key per 16: the 4 quarters together write 32 (fp32: 64) bytes of 16
+  // rows at a time.  fp32 sums go there every kSerial rows and are added to what lies there.
+  bool begun = false;
+  unsigned summed = 0;
+  auto put = [&]() {
+    if (key < a.Nk) {
+      const float k_scale = GradRange<T>::on ? a.scale * PScale<T>::inv / range : a.scale;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        T *out = reinterpret_cast<T *>(which ? a.dv : a.dk);
+        if (out == nullptr) continue;
+        const Str st = which ? a.sdv : a.sdk;
+        const float f = which ? PScale<T>::inv : k_scale;
+        float *part = a.splits > 1 ? a.part + ((((int64_t)which * a.splits + split) * a.B * a.Hkv + bh) * a.Nk + key) * a.D + g * 4 : nullptr;
+        T *row = out + (int64_t)b * st.b + (int64_t)key * st.n + (int64_t)hk * st.h + g * 4;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          if (d * 16 + g * 4 >= a.D) continue;
+          f32x4 y = seen ? (which ? gv[d] : gk[d]) * f : f32x4{0.f, 0.f, 0.f, 0.f};
+          if (part) {
+            f32x4 *to = reinterpret_cast<f32x4 *>(part + d * 16);
+            if (sizeof(T) == 4 && begun) y += *to;
+            *to = y;
+          } else {
+            typename Vec4<T>::type *to = reinterpret_cast<typename Vec4<T>::type *>(row + d * 16), z;
+            if constexpr (sizeof(T) == 4) {
+              if (begun) y += *to;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = (T)y[e];
+            *to = z;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) gk[d] = gv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    begun = true;
+    summed = 0;
+  };
   for (int w0 = 0; w0 < a.words; w0 += kWindow) {
     __syncthreads();                                             // the last window's list has been read
     if (tid < 64) {
@@ -1157,8 +1201,10 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
     const unsigned all = (unsigned)n_list * (unsigned)a.rows;    // < 2^31
     const unsigned total = (unsigned)((uint64_t)all * (split + 1) / a.splits);
     for (unsigned r0 = (unsigned)((uint64_t)all * split / a.splits); r0 < total; r0 += kBatch) {
+      if (sizeof(T) == 4 && summed >= kSerial) put();
       __syncthreads();                                           // the last batch's tables and tiles have been read
       const int in_batch = (int)min((unsigned)kBatch, total - r0), nt = (in_batch + TR - 1) / TR;
+      summed += in_batch;
 #pragma unroll
       for (int u = 0; u < kBatch / 256; ++u) {
         const int r = u * 256 + tid;
@@ -1303,32 +1349,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
       }
     }
   }
-  // a lane holds 4 channels of its key per 16: the 4 quarters together write 32 (fp32: 64) bytes of 16 rows at a time
-  if (key >= a.Nk) return;
-  const float k_scale = GradRange<T>::on ? a.scale * PScale<T>::inv / range : a.scale;
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    T *out = reinterpret_cast<T *>(which ? a.dv : a.dk);
-    if (out == nullptr) continue;
-    const Str st = which ? a.sdv : a.sdk;
-    const float f = which ? PScale<T>::inv : k_scale;
-    if (a.splits > 1) {
-      float *row = a.part + ((((int64_t)which * a.splits + split) * a.B * a.Hkv + bh) * a.Nk + key) * a.D + g * 4;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-        if (d * 16 + g * 4 < a.D) *reinterpret_cast<f32x4 *>(row + d * 16) = seen ? (which ? gv[d] : gk[d]) * f : f32x4{0.f, 0.f, 0.f, 0.f};
-      continue;
-    }
-    T *row = out + (int64_t)b * st.b + (int64_t)key * st.n + (int64_t)hk * st.h + g * 4;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      if (d * 16 + g * 4 >= a.D) continue;
-      typename Vec4<T>::type y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)(seen ? (which ? gv[d][e] : gk[d][e]) * f : 0.f);
-      *reinterpret_cast<typename Vec4<T>::type *>(row + d * 16) = y;
-    }
-  }
+  put();
 }
 
 // Adds the parts of split rows up, in the order of the rows: a thread has 4 channels of one key.
@@ -1384,7 +1405,7 @@ template <typename T, int DP, bool TWO> static int launch_dq(AttnArgs a, hipStre
   else return launch(attend_dq_kernel<T, DP, 32, 2, 2, 2, TWO>, DqTile<T, DP, 32, 2, 2>::body + list_bytes(a), blocks, a, s, what);
 }
 // Key tiles, and the splits of the rows each of them sums where there are too few tiles for the GPU: a batch of rows each at least.  The rows are
-// those of all groups (a key can be chosen by every one).  Sums of several thousand rows are the more exact for it.  A training step of 2,000
+// those of all groups (a key can be chosen by every one).  A training step of 2,000
 // queries x 16 heads against 200 keys of 2 heads of 64 fp32 channels 1,350 -> 141 us, bf16 350 -> 95 (the host's time).
 static int64_t dkv_tiles(const AttnArgs &a) { return ((int64_t)a.nb << (a.lb - 6)) * a.B * a.Hkv; }
 static int dkv_splits(const AttnArgs &a) {

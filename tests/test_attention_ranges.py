@@ -108,3 +108,34 @@ def test_fp16_value_gradient_of_an_unlikely_key():
     want = torch.softmax(k[0, :, 0, 0].double(), 0) * 2.0 ** 14
     # half a step each for the operand and the result; the score's rounding (33 log2 units)
     assert (dv[0, 1, 0].double() - want[1].item()).abs().max().item() <= 2 * 2.0 ** -25 + 40 * 2.0 ** -24 * want[1].item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,hk,nq,group,d,q_block", [(512, 1, 16000, 1, 8, 64), (128, 4, 2000, 8, 32, 64), (1, 1, 5000, 8, 128, 64), (1, 2, 4500, 8, 40, 1)])
+def test_fp32_key_gradients_are_not_one_serial_sum(b, hk, nq, group, d, q_block):
+    """Thousands of rows of every key, with key tiles enough for the whole GPU (no split of the rows) and with few.  A serial sum of n random terms has
+    an error of about 0.4 sqrt(n / 2) u of its size (the partial sums' roundings, u = 2^-24): 36 u for 16,000.  Sums of at most 1,024 terms: 9 u.  The
+    errors of the terms themselves are those of the same formulas in plain fp32 products, summed in blocks."""
+    u, nk = 2.0 ** -24, 64
+    g = torch.Generator(device=DEV).manual_seed(d)
+    q, k, v, do = (torch.randn(b, n, h, d, device=DEV, generator=g) for n, h in ((nq, hk * group), (nk, hk), (nk, hk), (nq, hk * group)))
+    visible = torch.ones(b, nk, device=DEV)
+    visible[:, 40:50] = 0
+    blocks = torch.zeros(b, hk, -(-nq // q_block), 1, dtype=torch.int32, device=DEV)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    _, dk, dv = torch.autograd.grad(A.block_attention(*leaves, blocks, visible, q_block=q_block), leaves, do)
+    assert dk[:, 40:50].abs().max() == 0 and dv[:, 40:50].abs().max() == 0
+    seen = visible[0] > 0
+    for i, j in ((0, 0), (b - 1, hk - 1)):
+        rows = [t[i, :, j * group:(j + 1) * group].detach().reshape(-1, d) for t in (q, do)]
+        keys = [t[i, seen, j].detach() for t in (k, v)]
+        exact, plain = [], []
+        for out, cast in ((exact, torch.float64), (plain, torch.float32)):
+            Q, G, K, V = (t.to(cast) for t in rows + keys)
+            p, _, ds = dense(Q, K, V, G, d ** -0.5)
+            for w, y in ((ds, Q), (p, G)):
+                out.append(sum(w[r:r + 512].T @ y[r:r + 512] for r in range(0, len(w), 512)))
+        for name, got, want, near in zip(("dk", "dv"), (dk, dv), exact, plain):
+            size = want.norm()
+            err, floor = ((x.double() - want).norm().item() / size.item() / u for x in (got[i, seen, j], near))
+            assert err <= 1.25 * (9.0 ** 2 + floor ** 2) ** 0.5, "%s: error %.1f u, that of the terms %.1f u" % (name, err, floor)
