@@ -64,6 +64,14 @@ __device__ __forceinline__ f32x4 mma4(f32x4 a, f32x4 b, f32x4 c) {
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
+// c + a b, where c is a long sum: fp32 products, whose k-elements go into an accumulator one after another, are summed for themselves first and added whole.
+// A serial sum of n random terms is off by about 0.4 sqrt(n / 2) 2^-24 of its size: outputs over 16,384 keys by 37 2^-24, 9 so (forward 101 -> 102 us, query
+// gradient 133 -> 133 for 16,384 keys of 64 channels; 128 channels 178 -> 183 and 274 -> 278).  16-bit results have no use for it.
+template <typename F, typename A> __device__ __forceinline__ A mma_whole(F a, F b, A c) { return mma(a, b, c); }
+__device__ __forceinline__ f32x4 mma_whole(f32x8 a, f32x8 b, f32x4 c) { return c + mma(a, b, f32x4{0.f, 0.f, 0.f, 0.f}); }
+template <typename F> __device__ __forceinline__ f32x4 mma4_whole(F a, F b, f32x4 c) { return mma4(a, b, c); }
+__device__ __forceinline__ f32x4 mma4_whole(f32x4 a, f32x4 b, f32x4 c) { return c + mma4(a, b, f32x4{0.f, 0.f, 0.f, 0.f}); }
+
 // The two shapes: S x S products of KS k-elements, AE results per lane.  Result e of a lane in quarter (half) q = lane / S is row
 // row(e) + 4 q of the tile.
 template <int S> struct Shape;
@@ -577,7 +585,7 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     }
     l += sum;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) o[i / PF] = mma(i < AH ? vf[i % AH] : v_frag(i), pf[i % PF], o[i / PF]);
+    for (int i = 0; i < NV; ++i) o[i / PF] = mma_whole(i < AH ? vf[i % AH] : v_frag(i), pf[i % PF], o[i / PF]);
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
     cur = nxt;
     nxt = keys.finish(raw);
@@ -715,7 +723,7 @@ __global__ __launch_bounds__(256, OCC) void attend_few_kernel(AttnArgs a) {
     l += (p[0] + p[1]) + (p[2] + p[3]);
     const frag4 pf = __builtin_convertvector(p, frag4);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] = mma4(vt[d], pf, o[d]);
+    for (int d = 0; d < DT; ++d) o[d] = mma4_whole(vt[d], pf, o[d]);
   }
   join_sets<T, DP, 16, 1, 4>(a, smem, o, m, l, row_of, a.splits > 1 ? a.part + ((int64_t)work * a.splits + split) * 16 * (a.D + 2) : nullptr, b, 0, wave);
 }
@@ -1036,7 +1044,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const frag k = i < AH ? ka[i % AH] : k_frag(i);
-      o[i / PF] = mma(k, gf[i % PF], o[i / PF]);
+      o[i / PF] = mma_whole(k, gf[i % PF], o[i / PF]);
       if constexpr (TWO) o[i / PF] = mma(k, gl[i % PF], o[i / PF]);
     }
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products

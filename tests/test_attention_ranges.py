@@ -139,3 +139,30 @@ def test_fp32_key_gradients_are_not_one_serial_sum(b, hk, nq, group, d, q_block)
             size = want.norm()
             err, floor = ((x.double() - want).norm().item() / size.item() / u for x in (got[i, seen, j], near))
             assert err <= 1.25 * (9.0 ** 2 + floor ** 2) ** 0.5, "%s: error %.1f u, that of the terms %.1f u" % (name, err, floor)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nk,d,q_block", [(32768, 16384, 64, 64), (512, 65536, 64, 1)])
+def test_fp32_sums_over_many_keys(nq, nk, d, q_block):
+    """Queries enough for the whole GPU (no split of the keys), thousands of keys each.  As above: a serial sum over 16,384 keys is off by 36 u of its size,
+    of sums of 32 (few rows: 16 of each 64) by 0.4 sqrt(n / 64) u (few rows: 0.4 sqrt(n / 128) u, the query gradient's two halves as before).  The gradient's
+    probabilities come from lse, 10 of 2^-20: roundings of 4.6 u, and of 3.2 u in log2 units, and those of the exponents, 3.2 u: 6.5 u."""
+    u = 2.0 ** -24
+    g = torch.Generator(device=DEV).manual_seed(nk)
+    q, k, v, do = (torch.randn(1, n, 1, d, device=DEV, generator=g) for n in (nq, nk, nk, nq))
+    top = nk // 64
+    blocks = torch.arange(top, device=DEV).int().expand(1, 1, nq // q_block, top).contiguous()
+    q.requires_grad_(True)
+    out = A.block_attention(q, k, v, blocks, q_block=q_block)
+    dq, = torch.autograd.grad(out, q, do)
+    n = min(nq, 1024)
+    sums = lambda w, y: sum(w[:, i:i + 512] @ y[i:i + 512] for i in range(0, nk, 512))   # noqa: E731
+    results = []
+    for cast in (torch.float64, torch.float32):
+        Q, K, V, G = (t[0, :m, 0].detach().to(cast) for t, m in ((q, n), (k, nk), (v, nk), (do, n)))
+        p, _, ds = dense(Q, K, V, G, d ** -0.5)
+        results.append((sums(p, V), sums(ds, K)))
+    for name, got, want, near in zip(("out", "dq"), (out, dq), *results):
+        err, floor = (((x.double() - want).norm() / want.norm()).item() / u for x in (got[0, :n, 0].detach(), near))
+        bound = 1.25 * (0.4 ** 2 * nk / 64 + 6.5 ** 2 + floor ** 2) ** 0.5
+        assert err <= bound, "%s: error %.1f u, that of the terms %.1f u, bound %.1f u" % (name, err, floor, bound)
