@@ -814,13 +814,15 @@ template <int S, typename V, int N, typename O, int DT> __device__ __forceinline
   }
 }
 
-// TWO: what rounding takes from a 16-bit operand (a score gradient; for dV a probability) is multiplied too.  Rounded once, it makes an error
-// of 1.4 times that of the result's own rounding; where the terms are few or lie along the sum (fewer than 64 channels) up to 1.6.  There
-// two parts are taken: in calls so small that it costs nothing (up to 2^20 scores: a few microseconds of a call of 150), and for heads of
-// fewer than 64 channels.
+// TWO: what rounding takes from a 16-bit operand (a score gradient; for dV a probability) is multiplied too.  Rounded once, it adds an error of the size of the
+// result's own rounding: together 1.46 times that.  Where a sum has few terms, or a tensor few sums, the roundings do not average out
+// (items of 8 queries up to 2.3, of 300 up to 1.58; 100 keys, one of them with most of the weight, up to 1.67), and below 64 channels they lie along the sum: there both
+// parts are taken (1.0 to 1.1, with one dominant key up to 1.4).  The rule looks at the sums of one item: whatever shares a call with it does not matter.
+// Two parts throughout would cost dq 248 -> 299 us, dk and dv 415 -> 487 (training step of 63,600 bf16 keys).
+constexpr int64_t kFewKeys = 512, kFewQueries = 2048;
 template <typename T> static bool two_parts(const AttnArgs &a) {
   const int64_t keys = (int64_t)a.cap << a.lb;
-  return sizeof(T) == 2 && (a.D < 64 || (int64_t)a.B * a.Nq * a.Hq * (keys < a.Nk ? keys : a.Nk) <= 1 << 20);
+  return sizeof(T) == 2 && (a.D < 64 || (keys < a.Nk ? keys : a.Nk) <= kFewKeys || (int64_t)a.Nq * a.G <= kFewQueries);
 }
 
 // delta of every row: 16 lanes per row, 8 channels each.  The output is taken as it was before its rounding (out + lo): delta is

@@ -166,3 +166,28 @@ def test_fp32_sums_over_many_keys(nq, nk, d, q_block):
         err, floor = (((x.double() - want).norm() / want.norm()).item() / u for x in (got[0, :n, 0].detach(), near))
         bound = 1.25 * (0.4 ** 2 * nk / 64 + 6.5 ** 2 + floor ** 2) ** 0.5
         assert err <= bound, "%s: error %.1f u, that of the terms %.1f u, bound %.1f u" % (name, err, floor, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,nq,nk,d", [(1, 300, 500, 64), (8, 300, 500, 64), (4, 4000, 100, 128), (64, 64, 3000, 96)])
+def test_gradients_with_few_terms_are_exact_alone_and_in_a_batch(b, nq, nk, d, dtype):
+    """Sums of few terms (queries or keys): the operands' roundings are no part of the error, whatever else is in the call.  What is left is the rounding of the
+    result and that of the forward's probabilities, through rowsum(dout o out)."""
+    g = torch.Generator().manual_seed(nk + d)
+    h = half(dtype)
+    q, k, v, do = (rnd(g, b, n, 1, d, dtype=dtype, scale=s) for n, s in ((nq, 1.5), (nk, 1), (nk, 1), (nq, 1)))
+    top = -(-nk // 64)
+    blocks = torch.arange(top, device=DEV).int().expand(b, 1, -(-nq // 64), top).contiguous()
+    leaves = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(A.block_attention(*leaves, blocks), leaves, do.to(DEV))
+    for i in {0, b // 2, b - 1}:
+        Q, K, V, G = (t[i, :, 0].to(DEV).double() for t in (q, k, v, do))
+        c = d ** -0.5
+        p, _, ds = dense(Q, K, V, G, c)
+        delta = (p * (G @ V.T)).square().sum(-1, keepdim=True) * c * c           # variance of rowsum(dout o out) over h^2 / 3
+        for name, x, want, var in (("dq", got[0], ds @ K, delta * (p @ K).square()), ("dk", got[1], ds.T @ Q, (p * p * delta).T @ Q.square()), ("dv", got[2], p.T @ G, None)):
+            own = own_rounding(want, dtype)
+            bound = 1.1 * (own ** 2 + (0 if var is None else h * h / 3 * var.sum().item())) ** 0.5
+            err = (x[i, :, 0].double() - want).norm().item()
+            assert err <= bound, "%s of item %d: %.3f times its own rounding, bound %.3f" % (name, i, err / own, bound / own)
