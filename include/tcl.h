@@ -292,7 +292,7 @@ int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, c
  *   lse = -inf.  visible as in tcl_block_means; blocks (B,Hkv,S,top_k) int32: an index outside [0, nb) is no block, a repeated one
  *   counts once, order does not matter.  lse (B,Hq,Nq) fp32, natural logarithm, nullable (the backward pass needs it).  out_lo (16-bit
  *   types, nullable): laid out like out, what its rounding took from it, for the backward pass.
- *   Limits: top_k <= 2048, nb <= 65,536, q_block * G <= 2^20 (q_block beyond Nq counts as Nq).
+ *   Limits: top_k <= 2048, nb <= 65,536, q_block * G <= 2^20 (q_block beyond Nq counts as Nq); scale finite, of any sign.
  *   Contents of invisible keys do not matter (NaN and infinities included).  A workspace of 0 bytes may be NULL. */
 size_t tcl_block_attention_fwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block,
                                                int64_t q_block);

@@ -6,6 +6,7 @@ stream of the tensor's device.  There is no CPU path: a CPU tensor raises.
 """
 import ctypes
 import functools
+import math
 
 import torch
 from torch.autograd import forward_ad
@@ -856,6 +857,8 @@ def block_attention(q, k, v, blocks, visible=None, block=64, q_block=64, scale=N
     bl = _side("blocks", blocks, dev, (torch.int32,), (b, hk, -(-nq // q_block), blocks.shape[3]))
     vis = _visible(visible, dev, b, nk)
     scale = float(d ** -0.5 if scale is None else scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite (got %r)" % scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = BlockAttentionFn.apply(q, k, v, bl, vis, block, q_block, scale)
     else:

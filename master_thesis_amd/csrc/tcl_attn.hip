@@ -21,6 +21,7 @@
 // term, the size of the rounding of the result itself; fp16, whose steps are absolute below 2^-14, after scaling: PScale, GradRange);
 // nothing else is rounded before the end.
 #include "tcl_common.h"
+#include <math.h>
 
 namespace tcl {
 
@@ -1473,6 +1474,7 @@ static int attn_setup(AttnArgs &a, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq
   TCL_REQUIRE(top_k <= kMaxTop, TCL_ERR_UNSUPPORTED, "block_attention: %ld blocks per group (at most %ld)", (long)top_k, (long)kMaxTop);
   TCL_REQUIRE(cdiv(Nk, block) <= kMaxKeyBlocks, TCL_ERR_UNSUPPORTED, "block_attention: %ld keys (at most %ld blocks)", (long)Nk, (long)kMaxKeyBlocks);
   TCL_REQUIRE(dtype == TCL_DT_F32 || dtype == TCL_DT_BF16 || dtype == TCL_DT_F16, TCL_ERR_UNSUPPORTED, "block_attention: unknown dtype %d", dtype);
+  TCL_REQUIRE(isfinite((float)(scale * 1.4426950408889634074)), TCL_ERR_ARG, "block_attention: scale %g", scale);
   if (q_block > Nq) q_block = Nq > 0 ? Nq : 1;
   TCL_REQUIRE(q_block * (Hq / Hkv) <= kMaxRows, TCL_ERR_UNSUPPORTED, "block_attention: groups of %ld query rows (at most %ld)", (long)(q_block * (Hq / Hkv)), (long)kMaxRows);
   a.B = (int)B; a.Nq = (int)Nq; a.Nk = (int)Nk; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.G = (int)(Hq / Hkv); a.D = (int)D;

@@ -771,3 +771,29 @@ def test_forward_mode_derivatives_are_refused_on_the_gpu():
                 call(forward_ad.make_dual(x, torch.ones_like(x)), x)
             plain = call(x, x)                                                    # in a level, without a tangent: as ever
         assert torch.equal(plain, call(x, x))
+
+
+# ------------------------------------------------------------------------------------------------ scales that are no numbers
+NO_SCALES = [float("nan"), float("inf"), -float("inf"), 3e38]
+
+
+def test_c_entries_refuse_scales_that_are_not_finite():
+    import ctypes
+    from master_thesis_amd import _lib
+    lib, one = _lib.lib(), ctypes.c_void_p(4096)
+    for scale in NO_SCALES:
+        assert lib.tcl_block_attention_fwd(one, 16, 8, 8, one, 512, 8, 8, one, 512, 8, 8, None, one, one, 16, 8, 8, None, None,
+                                           1, 2, 64, 2, 1, 8, 1, 64, 1, scale, 0, one, 0, None) == 2
+        assert lib.tcl_block_attention_bwd(one, 16, 8, 8, one, 16, 8, 8, one, 512, 8, 8, one, 512, 8, 8, None, one, one, 16, 8, 8, None, one,
+                                           None, 0, 0, 0, None, 0, 0, 0, None, 0, 0, 0, 1, 2, 64, 2, 1, 8, 1, 64, 1, scale, 0, one, 1 << 20, None) == 2
+        assert b"scale" in lib.tcl_last_error()
+
+
+@pytest.mark.gpu
+def test_scales_that_are_not_finite_are_refused():
+    """(A NaN gave finite outputs: those of equal scores.)"""
+    x, bl = torch.randn(1, 2, 1, 8, device=DEV, requires_grad=True), torch.zeros(1, 1, 1, 1, dtype=torch.int32, device=DEV)
+    for scale in NO_SCALES:
+        for t in (x, x.detach()):
+            with pytest.raises((ValueError, TclError), match="scale"):
+                A.block_attention(t, t, t, bl, scale=scale)
