@@ -189,6 +189,12 @@ template <int N> __device__ __forceinline__ void tile_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// Lanes of one wave exchange values through LDS: the hardware keeps a wave's LDS operations in order, and this tells the compiler to (it costs no instruction)
+__device__ __forceinline__ void wave_exchange() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // Where the pieces of this thread lie: piece u of an image of ROWS rows is row u * RPU + threadIdx.x / NCH, chunk `ch` of it (the
 // same for every u, or one of two in turn where a step is 8 rows)
@@ -709,12 +715,14 @@ __global__ __launch_bounds__(256, OCC) void attend_few_kernel(AttnArgs a) {
           *reinterpret_cast<f32x4 *>(row + (((c * 8 + g * 2 + 1) ^ I::swz(col)) << 4)) = __builtin_shufflevector(vf[c], vf[c], 4, 5, 6, 7);
         }
       }
+      wave_exchange();                                           // the rows are there
     }
     if (t + 1 < nt) load(__builtin_amdgcn_readfirstlane(next));
     if (part == 0) continue;
     frag4 vt[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) vt[d] = col_frag4<T, DP>(img, d * 16, lane);
+    wave_exchange();                                             // the rows have been read
     const float mx = column_max<16>(max2(max2(sc[0], sc[1]), max2(sc[2], sc[3])));
     raise_reference<16, T>(mx * sc2, m, l, o);
     const float ms = (m == kNegInf ? 0.f : m) - PScale<T>::fwd;
