@@ -282,7 +282,7 @@ int tcl_block_means(const void *k, int64_t k_sb, int64_t k_sn, int64_t k_sh, con
 /*   The blocks each group of queries attends to.  A group is q_block consecutive tokens with the G query heads of one key head; its
  *   score of block j is <sum of its queries, means[j]> in 64 bits.  blocks int32 (B,Hkv,S,top_k), S = ceil(N / q_block): the top_k
  *   best blocks with counts > 0 (ties to the lower index; a score of -inf or NaN is not chosen), in ascending order, -1 behind the
- *   last.  nb up to 16,384.  A workspace of 0 bytes may be NULL. */
+ *   last.  nb up to 16,384 (above 512: B * Hkv and S / 16 below 65,536).  A workspace of 0 bytes may be NULL. */
 size_t tcl_select_blocks_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t Hkv, int64_t D, int64_t nb, int64_t q_block);
 int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const float *means, const int32_t *counts, int32_t *blocks,
                       int64_t B, int64_t N, int64_t H, int64_t Hkv, int64_t D, int64_t nb, int64_t top_k, int64_t q_block, int dtype,

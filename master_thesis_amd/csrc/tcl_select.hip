@@ -499,7 +499,9 @@ extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int6
   const size_t size = dtype == TCL_DT_F32 ? 4 : 2;
   TCL_REQUIRE(aligned(q, 4 * size) && q_sb % 4 == 0 && q_sn % 4 == 0 && q_sh % 4 == 0 && aligned(means, 16), TCL_ERR_ARG,
               "select_blocks: query rows must start on 4 elements, means on 16 bytes");
-  TCL_REQUIRE(rows < (1LL << 31) && B * Hkv < 65536 && cdiv(S, 16) < 65536, TCL_ERR_SHAPE, "select_blocks: %ld groups are too many for one call", (long)rows);
+  const bool fused = select_is_fused(nb), direct = select_is_direct(N, H, Hkv, nb, q_block);
+  // the scores' kernel has a grid of three dimensions, which only a choice from many blocks needs
+  TCL_REQUIRE(rows < (1LL << 31) && (fused || nb == 0 || (B * Hkv < 65536 && cdiv(S, 16) < 65536)), TCL_ERR_SHAPE, "select_blocks: %ld groups are too many for one call", (long)rows);
   const size_t need = tcl_select_blocks_workspace_bytes(B, N, H, Hkv, D, nb, q_block);
   TCL_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), TCL_ERR_WORKSPACE, "select_blocks: workspace of %zu bytes needed", need);
   SelectArgs a{q, means, counts, blocks, (double *)workspace, nullptr, q_sb, q_sn, q_sh, (int)B, (int)N, (int)H, (int)Hkv, (int)(H / Hkv), (int)D, (int)nb,
@@ -509,7 +511,6 @@ extern "C" int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int6
   a.by_g = make_fastdiv((uint32_t)a.G);
   const int64_t per_group = (q_block < N ? q_block : N) * a.G;
   TCL_REQUIRE(per_group < (1LL << 31), TCL_ERR_SHAPE, "select_blocks: groups of %ld query rows", (long)per_group);
-  const bool fused = select_is_fused(nb), direct = select_is_direct(N, H, Hkv, nb, q_block);
   if (nb > 0 && !direct) {
     const dim3 pool((unsigned)cdiv(rows, 4));
     if (dtype == TCL_DT_F32) hipLaunchKernelGGL((select_pool_kernel<float>), pool, dim3(256), 0, s, a);

@@ -797,3 +797,22 @@ def test_scales_that_are_not_finite_are_refused():
         for t in (x, x.detach()):
             with pytest.raises((ValueError, TclError), match="scale"):
                 A.block_attention(t, t, t, bl, scale=scale)
+
+
+# ------------------------------------------------------------------------------------------------ many groups
+def test_c_entry_refuses_more_groups_than_the_grid_of_the_scores():
+    import ctypes
+    from master_thesis_amd import _lib
+    lib, one = _lib.lib(), ctypes.c_void_p(4096)
+    sel = lambda b, n, nb: lib.tcl_select_blocks(one, 16, 8, 8, one, one, one, b, n, 1, 1, 8, nb, 1, 1, 0, one, 1 << 60, None)   # noqa: E731
+    assert sel(65536, 1, 513) == 1 and sel(1, 1 << 20, 513) == 1 and b"too many" in lib.tcl_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,n", [(1, (1 << 20) + 17), (70000, 1)])
+def test_select_for_a_million_tokens_or_many_items(b, n):
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q, means = torch.randn(b, n, 1, 8, device=DEV, generator=g), torch.randn(b, 1, 3, 8, device=DEV, generator=g)
+    got = A.select_blocks(q, means, torch.ones(b, 3, dtype=torch.int32, device=DEV), 1, 1)
+    score = (q[:, :, 0, None].double() * means[:, 0, None].double()).sum(-1)
+    assert torch.equal(got[:, 0, :, 0], score.argmax(-1).int())
