@@ -816,3 +816,34 @@ def test_select_for_a_million_tokens_or_many_items(b, n):
     got = A.select_blocks(q, means, torch.ones(b, 3, dtype=torch.int32, device=DEV), 1, 1)
     score = (q[:, :, 0, None].double() * means[:, 0, None].double()).sum(-1)
     assert torch.equal(got[:, 0, :, 0], score.argmax(-1).int())
+
+
+# ------------------------------------------------------------------------------------------------ the documented sequence
+def documented():
+    """The python blocks of the documents at the root that use the operators"""
+    import pathlib
+    import re
+    texts = [p.read_text() for p in sorted(pathlib.Path(__file__).resolve().parent.parent.glob("*.md"))]
+    return [b for t in texts for b in re.findall(r"```python\n(.*?)```", t, re.S) if "utils import attention as A" in b]
+
+
+def test_documented_calls_fit_the_signatures():
+    import ast
+    import inspect
+    assert documented()
+    for block in documented():
+        for n in ast.walk(ast.parse(block)):
+            if isinstance(n, ast.Call) and isinstance(n.func, ast.Attribute) and isinstance(n.func.value, ast.Name) and n.func.value.id == "A":
+                inspect.signature(getattr(A, n.func.attr)).bind(*n.args, **{k.arg: k.value for k in n.keywords})
+
+
+@pytest.mark.gpu
+def test_documented_sequence_runs():
+    for block in documented():
+        g = torch.Generator(device=DEV).manual_seed(1)
+        maps = torch.randn(2, 128, 10, 30, 53, device=DEV, generator=g, dtype=torch.bfloat16)
+        space = {"maps": maps, "heads": 2, "q": torch.randn(2, 1590, 2, 64, device=DEV, dtype=torch.bfloat16), "v": torch.randn(2, 15900, 2, 64, device=DEV, dtype=torch.bfloat16),
+                 "visible": (torch.rand(2, 15900, device=DEV) < 0.8).float()}
+        exec(block, space)
+        assert space["out"].shape == (2, 1590, 2, 64) and torch.isfinite(space["out"]).all()
+        assert torch.equal(space["maps"].view(2, 15900, 2, 64)[:, 1590 + 53 + 2, 1], maps[:, 64:, 1, 1, 2])      # frame 1, row 1, column 2
