@@ -65,7 +65,7 @@ SIGNATURES = {
 
 PREC_F32, PREC_BF16, PREC_BF16X3 = 0, 1, 2
 CTX_DEFAULT, CTX_COMPLETE, CTX_CM_MODULE = 0, 1, 2
-DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+DT_F32, DT_BF16, DT_F16, DT_STATISTICS = 0, 1, 2, 16
 VMODE_NONE, VMODE_NEAREST, VMODE_BILINEAR_THRESHOLD = 0, 1, 2
 
 _lib = None

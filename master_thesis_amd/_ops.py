@@ -785,21 +785,22 @@ def _attend_bytes(*sizes):
     return _lib.lib().tcl_block_attention_fwd_workspace_bytes(*sizes)
 
 
-def _attend(q, k, v, blocks, visible, block, q_block, scale, want_lse, want_lo=False):
-    """-> out (B,Nq,Hq,D), lse (B,Hq,Nq) | None, what out's rounding took | None; q, k, v as _rows16 left them."""
+def _attend(q, k, v, blocks, visible, block, q_block, scale, want_lse, training=False):
+    """-> out (B,Nq,Hq,D), lse (B,Hq,Nq) | None, what out's rounding took | None; training: lse (3,B,Hq,Nq) with the softmax's statistics behind it.
+    q, k, v as _rows16 left them."""
     dev = q.device
     b, nq, hq, d = q.shape
     nk, hk = k.shape[1], k.shape[2]
     top = blocks.shape[3]
     out = torch.empty((b, nq, hq, d), dtype=q.dtype, device=dev)
-    lse = torch.empty((b, hq, nq), dtype=torch.float32, device=dev) if want_lse else None
-    lo = torch.empty_like(out) if want_lo and q.dtype != torch.float32 else None
+    lse = torch.empty((3, b, hq, nq) if training else (b, hq, nq), dtype=torch.float32, device=dev) if want_lse else None
+    lo = torch.empty_like(out) if training and q.dtype != torch.float32 else None
     nbytes = _attend_bytes(b, nq, nk, hq, hk, d, top, block, q_block)
     ws = _workspace(nbytes, dev) if nbytes else None      # only for few tokens, whose keys are split
     with _on(dev):
         _lib.call("tcl_block_attention_fwd", q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), _p(visible),
-                  blocks.data_ptr(), out.data_ptr(), *_strides(out), _p(lo), _p(lse), b, nq, nk, hq, hk, d, top, block, q_block, scale, _DT[q.dtype],
-                  _p(ws), nbytes, _stream(dev))
+                  blocks.data_ptr(), out.data_ptr(), *_strides(out), _p(lo), _p(lse), b, nq, nk, hq, hk, d, top, block, q_block, scale,
+                  _DT[q.dtype] | (_lib.DT_STATISTICS if training else 0), _p(ws), nbytes, _stream(dev))
     return out, lse, lo
 
 
@@ -810,8 +811,9 @@ class BlockAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, blocks, visible, block, q_block, scale):
         qc, kc, vc = _rows16(q), _rows16(k), _rows16(v)
-        out, lse, lo = _attend(qc, kc, vc, blocks, visible, block, q_block, scale, True, True)
-        ctx.save_for_backward(qc, kc, vc, blocks, visible, out, lse, lo)
+        out, statistics, lo = _attend(qc, kc, vc, blocks, visible, block, q_block, scale, True, True)
+        lse = statistics[0]
+        ctx.save_for_backward(qc, kc, vc, blocks, visible, out, statistics, lo)
         ctx.meta = (block, q_block, scale)
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -819,7 +821,7 @@ class BlockAttentionFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_out, _g_lse):
-        q, k, v, blocks, visible, out, lse, lo = ctx.saved_tensors
+        q, k, v, blocks, visible, out, statistics, lo = ctx.saved_tensors
         block, q_block, scale = ctx.meta
         b, nq, hq, d = q.shape
         nk, hk = k.shape[1], k.shape[2]
@@ -831,10 +833,10 @@ class BlockAttentionFn(torch.autograd.Function):
         ws = _workspace(_lib.lib().tcl_block_attention_bwd_workspace_bytes(b, nq, nk, hq, hk, d, top, block, q_block), dev)
         with _on(dev):
             _lib.call("tcl_block_attention_bwd", _p(go), *_strides(go), _p(q), *_strides(q), _p(k), *_strides(k), _p(v), *_strides(v),
-                      _p(visible), _p(blocks), _p(out), *_strides(out), _p(lo), _p(lse),
+                      _p(visible), _p(blocks), _p(out), *_strides(out), _p(lo), _p(statistics),
                       _p(g_q), *(none if g_q is None else _strides(g_q)), _p(g_k), *(none if g_k is None else _strides(g_k)),
                       _p(g_v), *(none if g_v is None else _strides(g_v)),
-                      b, nq, nk, hq, hk, d, top, block, q_block, scale, _DT[q.dtype], _p(ws), ws.numel(), _stream(dev))
+                      b, nq, nk, hq, hk, d, top, block, q_block, scale, _DT[q.dtype] | _lib.DT_STATISTICS, _p(ws), ws.numel(), _stream(dev))
         return g_q, g_k, g_v, None, None, None, None, None
 
 

@@ -104,6 +104,7 @@ struct AttnArgs {
   const int32_t *blocks;
   void *out, *lo, *dq, *dk, *dv;   // lo: what rounding took from out, laid out like it
   float *lse;                      // (B, Hq, Nq), natural logarithm
+  float *ref, *weight;             // (B, Hq, Nq): what the backward pass takes the probabilities from, or null: from lse (row_statistics)
   float *delta;                    // (B, Hq, Nq)
   uint32_t *inv;                   // (B, Hkv, nb, words): which groups chose the block
   uint32_t *chosen;                // (B, Hkv, nb): by how many entries, directly behind inv
@@ -383,6 +384,28 @@ struct KeySource {
   }
 };
 
+// The statistics of a row, from its reference (log2 units; +inf for a row that sees nothing), the sum under it and one over that.  lse holds the
+// probabilities of the backward pass only to |lse| 2^-24 each (scores of 10^4: value gradients off by 8 10^-4; of 10^8: 10^8 times too large), so P is taken as
+// the forward has it: exp2(score - ref) weight, the one exact where the other is not small (a factor more per score of dk and dv: training step of 63,600
+// keys 398 -> 403 us, fp32 186 -> 189; dq has it once a row).
+template <typename T> __device__ __forceinline__ void put_statistics(const AttnArgs &a, int64_t at, float mx, float sum, float inv) {
+  a.lse[at] = sum == 0.f ? kNegInf : (mx - PScale<T>::fwd + __builtin_log2f(sum)) * kLn2;
+  if (a.ref) {
+    a.ref[at] = sum == 0.f ? kPosInf : mx - PScale<T>::fwd;
+    a.weight[at] = inv;
+  }
+}
+__device__ __forceinline__ void row_statistics(const AttnArgs &a, int64_t at, float &ref, float &weight) {
+  if (a.ref) {
+    ref = a.ref[at];
+    weight = a.weight[at];
+  } else {
+    const float x = a.lse[at];
+    ref = x == kNegInf ? kPosInf : x * kLog2e;
+    weight = 1.f;
+  }
+}
+
 // Joins the WN key sets of a workgroup's M = S WM rows and writes them: every wave leaves its output, maximum and sum, and a thread adds
 // them up under the common maximum.  `o`, `m`, `l` as the forward's loops leave them; `part`: where a split's partial rows go, or null.
 template <typename T, int DP, int S, int WM, int WN, typename Rows>
@@ -441,7 +464,7 @@ __device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const t
     }
     *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.out) + at) = y;
     if (sizeof(T) == 2 && a.lo) *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.lo) + at) = lo;
-    if (ch == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx - PScale<T>::fwd + __builtin_log2f(sum)) * kLn2;
+    if (ch == 0 && a.lse) put_statistics<T>(a, ((int64_t)b * a.Hq + head) * a.Nq + token, mx, sum, inv);
   }
 }
 
@@ -789,11 +812,11 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
       lo[1] = (T)(o.y * inv - (float)y1);
     }
   }
-  if (lane == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head) * a.Nq + token] = sum == 0.f ? kNegInf : (mx - PScale<T>::fwd + __builtin_log2f(sum)) * kLn2;
+  if (lane == 0 && a.lse) put_statistics<T>(a, ((int64_t)b * a.Hq + head) * a.Nq + token, mx, sum, inv);
 }
 
 // ------------------------------------------------------------------------------------------ backward
-// With P = exp(scale S - lse) and dP = dout V^T:  dV = P^T dout,  dS = scale P o (dP - delta),  delta = rowsum(dout o out),
+// With P = exp(scale S - lse) (row_statistics) and dP = dout V^T:  dV = P^T dout,  dS = scale P o (dP - delta),  delta = rowsum(dout o out),
 // dQ = dS K,  dK = dS^T Q.  dQ is summed per query tile (like the forward), dK and dV per key tile: two kernels that both recompute
 // S and dP, and no atomics, so a gradient does not depend on the order of the workgroups.
 
@@ -943,7 +966,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     return r < a.rows && token < a.Nq;
   };
   frag qf[KC], df[KC];
-  float lse2 = kPosInf, delta = 0.f;                             // exp2(x - inf) = 0: no row, or a row that sees nothing
+  float ref = kPosInf, weight = 0.f, delta = 0.f;                // exp2(x - inf) = 0: no row, or a row that sees nothing
   {
     int token, head;
     const bool ok = row_of(wm * S + col, token, head);
@@ -951,8 +974,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
     const T *d = reinterpret_cast<const T *>(a.dout) + (int64_t)b * a.sdo.b + (int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h;
     if (ok) {
       const int64_t at = ((int64_t)b * a.Hq + head) * a.Nq + token;
-      const float x = a.lse[at];
-      if (x != kNegInf) lse2 = x * kLog2e;
+      row_statistics(a, at, ref, weight);
       delta = a.delta[at];
     }
 #pragma unroll
@@ -1041,7 +1063,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < KU * H::AE; ++e) {
       const int u = e / H::AE, x = e % H::AE;
-      const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][x], c2, -lse2));
+      const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][x], c2, -ref));
       sc[u][x] = p * (dp[u][x] - delta);
       if constexpr (GradRange<T>::on) sc[u][x] *= range;
     }
@@ -1066,7 +1088,7 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
   __syncthreads();
 #pragma unroll
   for (int d = 0; d < DT; ++d) {
-    if constexpr (GradRange<T>::on) o[d] *= 1.f / range;         // every key set has one of its own
+    o[d] *= GradRange<T>::on ? weight / range : weight;          // every key set has a range of its own
 #pragma unroll
     for (int e = 0; e < H::AE; e += 4)
       *reinterpret_cast<f32x4 *>(jo + (wn * M + wm * S + col) * F::LO + d * S + H::row(e) + g * 4) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
@@ -1105,8 +1127,8 @@ template <typename T, int DP> struct DkvTile {
   static constexpr int M = 64, TR = 32, NB = sizeof(T) == 4 && DP > 64 ? 2 : 4;
   static constexpr size_t img = (size_t)TR * Img<T, DP>::RB, tiles = NB * 2 * img;     // Q and dout
   static constexpr size_t body = tiles;
-  // behind the tiles: where a row lies in q and dout (in 16 bytes), lse and delta, the list of groups
-  static constexpr size_t bytes = body + kBatch * 16 + 32 * kWindow * 4;
+  // behind the tiles: where a row lies in q and dout (in 16 bytes), statistics and delta, the list of groups
+  static constexpr size_t bytes = body + kBatch * 20 + 32 * kWindow * 4;
 };
 template <typename T, int DP, bool TWO>
 __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
@@ -1116,7 +1138,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
   typedef typename Vec8<T>::type frag;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   u32x2 *tab = reinterpret_cast<u32x2 *>(smem + F::body);                              // [kBatch], x = ~0: no row
-  float *lse2 = reinterpret_cast<float *>(tab + kBatch), *delta = lse2 + kBatch;       // [kBatch] each
+  float *refs = reinterpret_cast<float *>(tab + kBatch), *weights = refs + kBatch, *delta = weights + kBatch;   // [kBatch] each
   int *list = reinterpret_cast<int *>(delta + kBatch);                                 // [32 kWindow]
   __shared__ int n_list;
 
@@ -1228,7 +1250,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
       for (int u = 0; u < kBatch / 256; ++u) {
         const int r = u * 256 + tid;
         u32x2 where = {~0u, ~0u};
-        float ls = kPosInf, de = 0.f;                            // exp2(x - inf) = 0
+        float ref = kPosInf, weight = 0.f, de = 0.f;             // exp2(x - inf) = 0
         if (r < in_batch) {
           const unsigned e = a.by_rows.div(r0 + r), rr = r0 + r - e * (unsigned)a.rows;
           const unsigned tk = a.by_g.div(rr);
@@ -1239,13 +1261,13 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
             where.x = (unsigned)(((int64_t)token * a.sq.n + (int64_t)head * a.sq.h) / u16);
             where.y = (unsigned)(((int64_t)token * a.sdo.n + (int64_t)head * a.sdo.h) / u16);
             const int64_t at = ((int64_t)b * a.Hq + head) * a.Nq + token;
-            const float x = a.lse[at];
-            if (x != kNegInf) ls = x * kLog2e - PScale<T>::bits;
+            row_statistics(a, at, ref, weight);
             de = a.delta[at];
           }
         }
         tab[r] = where;
-        lse2[r] = ls;
+        refs[r] = ref - PScale<T>::bits;
+        weights[r] = weight;
         delta[r] = de;
       }
       __syncthreads();
@@ -1304,10 +1326,11 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
               df[u][c] = row_frag<T, DP>(drows, u * 16 + col, c * 32 + g * 8);
             }
         }
-        f32x4 ls[2], de[2];
+        f32x4 ref[2], we[2], de[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          ls[u] = *reinterpret_cast<const f32x4 *>(lse2 + t * TR + u * 16 + g * 4);
+          ref[u] = *reinterpret_cast<const f32x4 *>(refs + t * TR + u * 16 + g * 4);
+          we[u] = *reinterpret_cast<const f32x4 *>(weights + t * TR + u * 16 + g * 4);
           de[u] = *reinterpret_cast<const f32x4 *>(delta + t * TR + u * 16 + g * 4);
         }
         if constexpr (ahead) __builtin_amdgcn_sched_barrier(0);
@@ -1334,7 +1357,7 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][e], a.c, -ls[u][e]));
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][e], a.c, -ref[u][e])) * we[u][e];
             dp[u][e] = p * (dp[u][e] - de[u][e]);
             if constexpr (GradRange<T>::on) dp[u][e] *= range;
             pf[u * 4 + e] = (T)p;
@@ -1518,6 +1541,11 @@ static bool rows16(const void *p, const Str &s, int dtype) {
   const int64_t ve = dtype == TCL_DT_F32 ? 4 : 8;
   return aligned(p, 16) && s.b % ve == 0 && s.n % ve == 0 && s.h % ve == 0;
 }
+static void statistics_behind(AttnArgs &a) {
+  const int64_t rows = (int64_t)a.B * a.Hq * a.Nq;
+  a.ref = a.lse + rows;
+  a.weight = a.ref + rows;
+}
 // the rows of a block are addressed by 32-bit byte offsets from its first
 static bool near_rows(const Str &s) { return s.n >= 0 && s.n < (1LL << 22); }
 // the query rows of a batch item by 32-bit counts of 16 bytes
@@ -1544,11 +1572,14 @@ extern "C" int tcl_block_attention_fwd(const void *q, int64_t q_sb, int64_t q_sn
                                        int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block, int64_t q_block,
                                        double scale, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   AttnArgs a{};
+  const bool statistics = dtype & TCL_DT_STATISTICS;
+  dtype &= ~TCL_DT_STATISTICS;
   const int rc = attn_setup(a, B, Nq, Nk, Hq, Hkv, D, top_k, block, q_block, scale, dtype);
   if (rc != TCL_OK) return rc;
   if (B == 0 || Nq == 0) return TCL_OK;
   TCL_REQUIRE(q && out && blocks && (Nk == 0 || (k && v)), TCL_ERR_ARG, "block_attention: null pointer");
   a.q = q; a.k = k; a.v = v; a.vis = visible; a.blocks = blocks; a.out = out; a.lo = out_lo; a.lse = lse;
+  if (statistics && lse) statistics_behind(a);
   a.sq = Str{q_sb, q_sn, q_sh}; a.sk = Str{k_sb, k_sn, k_sh}; a.sv = Str{v_sb, v_sn, v_sh}; a.so = Str{o_sb, o_sn, o_sh};
   TCL_REQUIRE(rows16(q, a.sq, dtype) && (Nk == 0 || (rows16(k, a.sk, dtype) && rows16(v, a.sv, dtype))) && rows16(out, a.so, dtype) && aligned(out_lo, 16), TCL_ERR_ARG,
               "block_attention: rows must start on 16 bytes");
@@ -1589,11 +1620,14 @@ extern "C" int tcl_block_attention_bwd(const void *grad_out, int64_t g_sb, int64
                                        int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block, int64_t q_block,
                                        double scale, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   AttnArgs a{};
+  const bool statistics = dtype & TCL_DT_STATISTICS;
+  dtype &= ~TCL_DT_STATISTICS;
   const int rc = attn_setup(a, B, Nq, Nk, Hq, Hkv, D, top_k, block, q_block, scale, dtype);
   if (rc != TCL_OK) return rc;
   if (B == 0 || Nq == 0 || Nk == 0) return TCL_OK;             // the caller zeroes gradients of an empty attention
   TCL_REQUIRE(grad_out && q && k && v && out && blocks && lse, TCL_ERR_ARG, "block_attention backward: null pointer");
   a.q = q; a.k = k; a.v = v; a.dout = grad_out; a.vis = visible; a.blocks = blocks; a.out = const_cast<void *>(out); a.lo = const_cast<void *>(out_lo); a.lse = const_cast<float *>(lse);
+  if (statistics) statistics_behind(a);
   a.dq = g_q; a.dk = g_k; a.dv = g_v;
   a.sq = Str{q_sb, q_sn, q_sh}; a.sk = Str{k_sb, k_sn, k_sh}; a.sv = Str{v_sb, v_sn, v_sh}; a.so = Str{o_sb, o_sn, o_sh}; a.sdo = Str{g_sb, g_sn, g_sh};
   a.sdq = Str{gq_sb, gq_sn, gq_sh}; a.sdk = Str{gk_sb, gk_sn, gk_sh}; a.sdv = Str{gv_sb, gv_sn, gv_sh};

@@ -191,3 +191,53 @@ def test_gradients_with_few_terms_are_exact_alone_and_in_a_batch(b, nq, nk, d, d
             bound = 1.1 * (own ** 2 + (0 if var is None else h * h / 3 * var.sum().item())) ** 0.5
             err = (x[i, :, 0].double() - want).norm().item()
             assert err <= bound, "%s of item %d: %.3f times its own rounding, bound %.3f" % (name, i, err / own, bound / own)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size,dtype", [(s, t) for s in (20.0, 100.0, 1e3, 1e4, 1e6, 1e8) for t in (torch.float32, torch.bfloat16, torch.float16)
+                                        if s <= 1e4 or t != torch.float16])      # larger queries are no fp16 numbers
+def test_gradients_under_large_scores(size, dtype):
+    """Scores up to many times 10^8: the softmax is one key in the end, and its value gets the whole cotangent.  As exact as the same formulas in plain fp32
+    products (scores of either side are rounded alike), and a few roundings: of P, its weight and the product."""
+    g = torch.Generator().manual_seed(11)
+    n, d = 1024, 64
+    q, k, v, do = (rnd(g, n, d, dtype=dtype, scale=s) for s in (size ** 0.5, size ** 0.5, 1, 1))
+    grads = gradients(q, k, v, do)
+    results = []
+    for cast in (torch.float64, torch.float32):
+        Q, K, V, G = (t.to(DEV).to(cast) for t in (q, k, v, do))
+        p, _, ds = dense(Q, K, V, G, d ** -0.5)
+        results.append([t.double() for t in (ds @ K, ds.T @ Q, p.T @ G)])
+    for name, got, want, near in zip(("dq", "dk", "dv"), grads, *results):
+        if name != "dv" and (dtype != torch.float32 or size > 100):           # what the score's own rounding leaves of the differences
+            continue
+        err, floor = ((x - want).norm().item() / want.norm().item() for x in (got, near.to(dtype).double()))
+        assert err <= 1.5 * floor + 4 * 2.0 ** -24, "%s: error %.3g, plain %.3g" % (name, err, floor)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_c_entries_with_lse_alone(dtype):
+    """A caller that keeps nothing but lse: the gradients of the Python call, to the rounding of lse (6 at most: 2^-22, twice, of every probability)."""
+    from master_thesis_amd import _lib, _ops
+    g = torch.Generator().manual_seed(12)
+    nq, nk, h, d = 70, 200, 2, 32
+    q, do = (rnd(g, 1, nq, h, d, dtype=dtype).to(DEV) for _ in range(2))
+    k, v = (rnd(g, 1, nk, h, d, dtype=dtype).to(DEV) for _ in range(2))
+    blocks = torch.arange(4, device=DEV).int().expand(1, h, 2, 4).contiguous()
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out, lse = A.block_attention(*leaves, blocks, return_lse=True)
+    want = torch.autograd.grad(out, leaves, do)
+    got_out, got_lse, lo = torch.empty_like(q), torch.full((h, nq), float("nan"), device=DEV), torch.empty_like(q)
+    strides = [t for x in (q, k, v) for t in (x.data_ptr(), *_ops._strides(x))]
+    sizes = (1, nq, nk, h, h, d, 4, 64, 64, d ** -0.5, _ops._DT[dtype])
+    low = None if dtype == torch.float32 else lo.data_ptr()
+    ws = torch.empty(_lib.lib().tcl_block_attention_bwd_workspace_bytes(*sizes[:9]) + (1 << 20), dtype=torch.uint8, device=DEV)
+    tail = (ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+    _lib.call("tcl_block_attention_fwd", *strides, None, blocks.data_ptr(), got_out.data_ptr(), *_ops._strides(q), low, got_lse.data_ptr(), *sizes, *tail)
+    assert torch.equal(got_out, out) and torch.equal(got_lse, lse[0])
+    got = [torch.full_like(t, float("nan")) for t in (q, k, v)]
+    _lib.call("tcl_block_attention_bwd", do.data_ptr(), *_ops._strides(do), *strides, None, blocks.data_ptr(), got_out.data_ptr(), *_ops._strides(q), low, got_lse.data_ptr(),
+              *[t for x in got for t in (x.data_ptr(), *_ops._strides(x))], *sizes, *tail)
+    for a, b in zip(got, want):
+        assert (a.double() - b.double()).norm() <= (2.0 ** -20 + (0 if dtype == torch.float32 else half(dtype))) * b.double().norm()
