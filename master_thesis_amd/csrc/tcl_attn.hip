@@ -406,6 +406,13 @@ __device__ __forceinline__ void row_statistics(const AttnArgs &a, int64_t at, fl
   }
 }
 
+// x, as a number that the compiler knows nothing about: where one value's rounding to 16 bits is used twice (the output, and what is missing from it), it has rounded
+// the product once for one use and twice for the other, and the two were a step apart
+__device__ __forceinline__ float settled(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 // Joins the WN key sets of a workgroup's M = S WM rows and writes them: every wave leaves its output, maximum and sum, and a thread adds
 // them up under the common maximum.  `o`, `m`, `l` as the forward's loops leave them; `part`: where a split's partial rows go, or null.
 template <typename T, int DP, int S, int WM, int WN, typename Rows>
@@ -459,8 +466,9 @@ __device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const t
     typename Vec4<T>::type y, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      y[e] = (T)(x4[e] * inv);
-      lo[e] = (T)(x4[e] * inv - (float)y[e]);
+      const float z = settled(x4[e] * inv);
+      y[e] = (T)z;
+      lo[e] = (T)(z - (float)y[e]);
     }
     *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.out) + at) = y;
     if (sizeof(T) == 2 && a.lo) *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.lo) + at) = lo;
@@ -804,12 +812,13 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
   if (lane * 2 < a.D) {
     const int64_t at = (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch;
     T *y = reinterpret_cast<T *>(a.out) + at, *lo = reinterpret_cast<T *>(a.lo) + at;
-    const T y0 = (T)(o.x * inv), y1 = (T)(o.y * inv);
+    const float z0 = settled(o.x * inv), z1 = settled(o.y * inv);
+    const T y0 = (T)z0, y1 = (T)z1;
     y[0] = y0;
     y[1] = y1;
     if (sizeof(T) == 2 && a.lo) {
-      lo[0] = (T)(o.x * inv - (float)y0);
-      lo[1] = (T)(o.y * inv - (float)y1);
+      lo[0] = (T)(z0 - (float)y0);
+      lo[1] = (T)(z1 - (float)y1);
     }
   }
   if (lane == 0 && a.lse) put_statistics<T>(a, ((int64_t)b * a.Hq + head) * a.Nq + token, mx, sum, inv);

@@ -241,3 +241,25 @@ def test_c_entries_with_lse_alone(dtype):
               *[t for x in got for t in (x.data_ptr(), *_ops._strides(x))], *sizes, *tail)
     for a, b in zip(got, want):
         assert (a.double() - b.double()).norm() <= (2.0 ** -20 + (0 if dtype == torch.float32 else half(dtype))) * b.double().norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nq,nk,q_block", [(64, 3, 64), (64, 3, 1), (1, 4096, 1)])
+def test_output_and_what_its_rounding_took(nq, nk, q_block, dtype):
+    """Three equal keys are seen: probabilities of a third each, whose operands are exact.  What training keeps of the output next to it has to add up to the mean of
+    the three values, also where that lies halfway between two numbers of the type."""
+    from master_thesis_amd import _ops
+    g = torch.Generator().manual_seed(nk)
+    d, h = 128, half(dtype)
+    v = rnd(g, 16, nk, 1, d, dtype=dtype).to(DEV)
+    visible = torch.zeros(16, nk, device=DEV)
+    at = [0, nk // 2, nk - 1]
+    visible[:, at] = 1
+    top = -(-nk // 64)
+    blocks = torch.arange(top, device=DEV).int().expand(16, 1, -(-nq // q_block), top).contiguous()
+    out, _, lo = _ops._attend(torch.zeros(16, nq, 1, d, dtype=dtype, device=DEV), torch.ones_like(v), v, blocks, visible, 64, q_block, 1.0, True, True)
+    want = v[:, at].double().mean(1, keepdim=True)
+    # the remainder's own rounding (h of at most h of the output), 1 / 3, the product and the three-term sum in fp32 (of terms up to the largest value)
+    tol = h * h * want.abs() + 4 * 2.0 ** -24 * v[:, at].double().abs().amax(1, keepdim=True)
+    assert ((out.double() + lo.double() - want).abs() <= tol).all()
