@@ -173,14 +173,36 @@ template <> struct PScale<_Float16> { static constexpr float room = 4.f, fwd = 1
 // (fp16: 16, scaled 2^14) far from every type's limits, and it costs no accuracy, since all sums are of floating-point numbers.  So the sums and outputs so
 // far are scaled only where a score passes the reference by more (64 tiles of random scores, 32 rows a wave: in 1 or 2 tiles instead of about 45).
 // A NaN becomes the reference, and with it the whole row.
-template <int S, typename T, typename O> __device__ __forceinline__ void raise_reference(float mx, float &m, float &l, O &o) {
+template <int S, typename T, typename O> __device__ __forceinline__ void raise_reference(float mx, float &m, float &l, float &lr, O &o) {
   if (__any(!(mx <= m + PScale<T>::room))) {
     const float mn = max2(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.f : mn));
     m = mn;
     l *= f;
+    lr *= f;
 #pragma unroll
     for (int d = 0; d < (int)(sizeof(O) / sizeof(o[0])); ++d) o[d] *= f;
   }
+}
+// c + the sum of rounded probabilities (a training step divides by it what it keeps of the output for rowsum(dout o out): the roundings' errors are then those of
+// the values' differences from the output, where over the unrounded sum they are those of the values, which may have a large common part: with values of
+// mean 5 and deviation 1 dq was off by twice its own rounding, of mean 50 by 17 times, now by 1.05).  Forward of the training step of 63,600 keys 215 -> 222 us.
+__device__ __forceinline__ float add_rounded(float c, bf16x4 p) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  const pair one = {(__bf16)1.f, (__bf16)1.f};
+  c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 0, 1), one, c, false);
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 2, 3), one, c, false);
+}
+__device__ __forceinline__ float add_rounded(float c, f16x4 p) {
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+  const pair one = {(_Float16)1.f, (_Float16)1.f};
+  c = __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 0, 1), one, c, false);
+  return __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 2, 3), one, c, false);
+}
+__device__ __forceinline__ float add_rounded(float c, bf16x8 p) {
+  return add_rounded(add_rounded(c, __builtin_shufflevector(p, p, 0, 1, 2, 3)), __builtin_shufflevector(p, p, 4, 5, 6, 7));
+}
+__device__ __forceinline__ float add_rounded(float c, f16x8 p) {
+  return add_rounded(add_rounded(c, __builtin_shufflevector(p, p, 0, 1, 2, 3)), __builtin_shufflevector(p, p, 4, 5, 6, 7));
 }
 // all but the last N LDS-DMAs of this wave have landed and every LDS read of it has been served; then the workgroup meets
 // (by the builtin: a wait in inline assembly is unknown to the compiler, which then waits again, for the tile that is on its way)
@@ -384,6 +406,9 @@ struct KeySource {
   }
 };
 
+// of a sum: nothing seen gives zero; NaN stays NaN
+__device__ __forceinline__ float inverse(float sum) { return sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); }
+
 // The statistics of a row, from its reference (log2 units; +inf for a row that sees nothing), the sum under it and one over that.  lse holds the
 // probabilities of the backward pass only to |lse| 2^-24 each (scores of 10^4: value gradients off by 8 10^-4; of 10^8: 10^8 times too large), so P is taken as
 // the forward has it: exp2(score - ref) weight, the one exact where the other is not small (a factor more per score of dk and dv: training step of 63,600
@@ -413,23 +438,28 @@ __device__ __forceinline__ float settled(float x) {
   return x;
 }
 
-// Joins the WN key sets of a workgroup's M = S WM rows and writes them: every wave leaves its output, maximum and sum, and a thread adds
-// them up under the common maximum.  `o`, `m`, `l` as the forward's loops leave them; `part`: where a split's partial rows go, or null.
+// Joins the WN key sets of a workgroup's M = S WM rows and writes them: every wave leaves its output, maximum and sums, and a thread adds
+// them up under the common maximum.  `o`, `m`, `l`, `lr` as the forward's loops leave them; `part`: where a split's partial rows go, or null.
 template <typename T, int DP, int S, int WM, int WN, typename Rows>
-__device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const typename Shape<S>::acc (&o)[DP / S], float m, float l, const Rows &row_of, float *pm, int b, int wm, int wn) {
+__device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const typename Shape<S>::acc (&o)[DP / S], float m, float l, float lr, const Rows &row_of, float *pm, int b, int wm, int wn) {
   typedef Shape<S> H;
   constexpr int M = S * WM, LO = DP + 4, DT = DP / S;
   const int tid = threadIdx.x, lane = tid % 64, col = lane % S, g = lane / S;
   float *jo = reinterpret_cast<float *>(smem);                   // [WN][M][LO]
-  float *jm = jo + WN * M * LO, *jl = jm + WN * M;            // [WN][M] each
+  float *jm = jo + WN * M * LO, *jl = jm + WN * M, *jr = jl + WN * M;   // [WN][M] each
   __syncthreads();
   {
     const int r = wn * M + wm * S + col;
-    if (S == 16) l += __shfl_xor(l, 16, 64);
+    if (S == 16) {
+      l += __shfl_xor(l, 16, 64);
+      lr += __shfl_xor(lr, 16, 64);
+    }
     l += __shfl_xor(l, 32, 64);
+    lr += __shfl_xor(lr, 32, 64);
     if (g == 0) {
       jm[r] = m;
       jl[r] = l;
+      jr[r] = lr;
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -443,7 +473,7 @@ __device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const t
     const int r = (int)a.by_d4.div((unsigned)id), ch = (id - r * (a.D / 4)) * 4;
     int token, head;
     if (!row_of(r, token, head)) continue;
-    float mx = kNegInf, sum = 0.f;
+    float mx = kNegInf, sum = 0.f, rounded = 0.f;
 #pragma unroll
     for (int x = 0; x < WN; ++x) mx = max2(mx, jm[x * M + r]);
     f32x4 x4 = {0.f, 0.f, 0.f, 0.f};
@@ -451,6 +481,7 @@ __device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const t
     for (int x = 0; x < WN; ++x) {
       const float f = mx == kNegInf ? 0.f : __builtin_amdgcn_exp2f(jm[x * M + r] - mx);
       sum += mx == kNegInf ? 0.f : jl[x * M + r] * f;
+      rounded += mx == kNegInf ? 0.f : jr[x * M + r] * f;
       x4 += *reinterpret_cast<const f32x4 *>(jo + (x * M + r) * LO + ch) * f;
     }
     if (pm) {
@@ -458,17 +489,18 @@ __device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const t
       if (ch == 0) {
         pm[(int64_t)M * a.D + r] = mx;
         pm[(int64_t)M * a.D + M + r] = sum;
+        pm[(int64_t)M * a.D + 2 * M + r] = rounded;
       }
       continue;
     }
-    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // nothing seen: zero; NaN stays NaN
+    const float inv = inverse(sum), inv_rounded = inverse(rounded);
     const int64_t at = (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch;
     typename Vec4<T>::type y, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float z = settled(x4[e] * inv);
       y[e] = (T)z;
-      lo[e] = (T)(z - (float)y[e]);
+      lo[e] = (T)(x4[e] * inv_rounded - (float)y[e]);
     }
     *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.out) + at) = y;
     if (sizeof(T) == 2 && a.lo) *reinterpret_cast<typename Vec4<T>::type *>(reinterpret_cast<T *>(a.lo) + at) = lo;
@@ -488,10 +520,11 @@ __device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const t
 template <typename T, int DP, int S, int WM, int WN, int KU> struct FwdTile {
   static constexpr int M = S * WM, TK = S * KU * WN, LO = DP + 4;
   static constexpr size_t img = (size_t)TK * Img<T, DP>::RB, tiles = 4 * img;          // K and V, twice
-  static constexpr size_t join = (size_t)WN * M * (LO + 2) * 4;                        // outputs, maxima and sums of the key sets
+  static constexpr size_t join = (size_t)WN * M * (LO + 3) * 4;                        // outputs, maxima and sums of the key sets
   static constexpr size_t body = tiles > join ? tiles : join;
 };
-template <typename T, int DP, int S, int WM, int WN, int KU>
+// LO: for a training step of 16-bit types (add_rounded).
+template <typename T, int DP, int S, int WM, int WN, int KU, bool LO>
 __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
   typedef FwdTile<T, DP, S, WM, WN, KU> F;
   typedef Shape<S> H;
@@ -567,7 +600,7 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     for (int c = 0; c < KC; ++c) qf[c] = -qf[c];
   }
   acc o[DT];
-  float m = kNegInf, l = 0.f;                                    // reference in log2 units, sum of exp2(score - reference), scaled as P is
+  float m = kNegInf, l = 0.f, lr = 0.f;                          // reference in log2 units, sums of exp2(score - reference), scaled as P is, and rounded as P is
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = acc(0.f);
   if (nt > 0) nxt = keys.finish(raw);
@@ -611,7 +644,7 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 2; e < E; ++e) mx = max2(mx, sc[e / H::AE][e % H::AE]);
     mx = column_max<S>(mx);
-    raise_reference<S, T>(mx * sc2, m, l, o);
+    raise_reference<S, T>(mx * sc2, m, l, lr, o);
     const float ms = (m == kNegInf ? 0.f : m) - PScale<T>::fwd;  // nothing seen yet: exp2(-inf - 0) = 0
     float sum = 0.f;
     frag pf[PF];
@@ -622,6 +655,10 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
       pf[e / 8][e % 8] = (T)p;
     }
     l += sum;
+    if constexpr (LO) {
+#pragma unroll
+      for (int i = 0; i < PF; ++i) lr = add_rounded(lr, pf[i]);
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) o[i / PF] = mma_whole(i < AH ? vf[i % AH] : v_frag(i), pf[i % PF], o[i / PF]);
     __builtin_amdgcn_sched_barrier(0);                           // the mask of the tile after next is not waited for before the products
@@ -629,7 +666,7 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
     nxt = keys.finish(raw);
   }
 
-  join_sets<T, DP, S, WM, WN>(a, smem, o, m, l, row_of, a.splits > 1 ? a.part + ((int64_t)work * a.splits + split) * M * (a.D + 2) : nullptr, b, wm, wn);
+  join_sets<T, DP, S, WM, WN>(a, smem, o, m, l, lr, row_of, a.splits > 1 ? a.part + ((int64_t)work * a.splits + split) * M * (a.D + 3) : nullptr, b, wm, wn);
 }
 
 // Few rows (a group of up to 16: one token of some heads): one workgroup holds all of them, and no element of a key is used twice.  The four
@@ -641,10 +678,10 @@ __global__ __launch_bounds__(256, 2) void attend_fwd_kernel(AttnArgs a) {
 // vector instructions of the softmax take about half the time.  A single token of 4 items against 64 blocks of 128 (34 MB): 14 us, 5 of them
 // the launch and the list, and 4 for the join.
 template <typename T, int DP> struct FewTile {
-  static constexpr size_t img = (size_t)16 * Img<T, DP>::RB, tiles = 4 * img, join = (size_t)4 * 16 * (DP + 6) * 4;
+  static constexpr size_t img = (size_t)16 * Img<T, DP>::RB, tiles = 4 * img, join = (size_t)4 * 16 * (DP + 7) * 4;
   static constexpr size_t body = tiles > join ? tiles : join;
 };
-template <typename T, int DP, int OCC>
+template <typename T, int DP, int OCC, bool LO>
 __global__ __launch_bounds__(256, OCC) void attend_few_kernel(AttnArgs a) {
   typedef FewTile<T, DP> F;
   typedef Img<T, DP> I;
@@ -712,7 +749,7 @@ __global__ __launch_bounds__(256, OCC) void attend_few_kernel(AttnArgs a) {
   };
   const float sc2 = fmaxf(fabsf(a.c), 1e-30f);                   // not 0: -inf times it has to stay -inf
   f32x4 o[DT];
-  float m = kNegInf, l = 0.f;
+  float m = kNegInf, l = 0.f, lr = 0.f;
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (nt > 0) load(__builtin_amdgcn_readfirstlane(key_of(0)));
@@ -755,17 +792,18 @@ __global__ __launch_bounds__(256, OCC) void attend_few_kernel(AttnArgs a) {
     for (int d = 0; d < DT; ++d) vt[d] = col_frag4<T, DP>(img, d * 16, lane);
     wave_exchange();                                             // the rows have been read
     const float mx = column_max<16>(max2(max2(sc[0], sc[1]), max2(sc[2], sc[3])));
-    raise_reference<16, T>(mx * sc2, m, l, o);
+    raise_reference<16, T>(mx * sc2, m, l, lr, o);
     const float ms = (m == kNegInf ? 0.f : m) - PScale<T>::fwd;
     f32x4 p;
 #pragma unroll
     for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], sc2, -ms));
     l += (p[0] + p[1]) + (p[2] + p[3]);
     const frag4 pf = __builtin_convertvector(p, frag4);
+    if constexpr (LO) lr = add_rounded(lr, pf);
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = mma4_whole(vt[d], pf, o[d]);
   }
-  join_sets<T, DP, 16, 1, 4>(a, smem, o, m, l, row_of, a.splits > 1 ? a.part + ((int64_t)work * a.splits + split) * 16 * (a.D + 2) : nullptr, b, 0, wave);
+  join_sets<T, DP, 16, 1, 4>(a, smem, o, m, l, lr, row_of, a.splits > 1 ? a.part + ((int64_t)work * a.splits + split) * 16 * (a.D + 3) : nullptr, b, 0, wave);
 }
 // Joins the splits (at most kMaxSplits) of a row: one workgroup per row.  Lane x of every wave holds split x's factor; the waves take
 // the splits in turn, a lane two channels of them, and are added up in wave order.  Everything is asked for at once: the time is that
@@ -781,18 +819,18 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
   const int bh = (int)(work / a.chunks / a.S), hk = bh % a.Hkv, b = bh / a.Hkv;
   const int row = chunk * M + r, t = (int)a.by_g.div((unsigned)row), token = s * a.q_block + t, head = hk * a.G + (row - t * a.G);
   if (row >= a.rows || token >= a.Nq) return;
-  const int64_t step = (int64_t)M * (a.D + 2);
+  const int64_t step = (int64_t)M * (a.D + 3);
   const float *p = a.part + work * a.splits * step;
   const int x = min(lane, a.splits - 1);
   const float m = lane < a.splits ? p[x * step + (int64_t)M * a.D + r] : kNegInf;
-  const float l = p[x * step + (int64_t)M * a.D + M + r];
+  const float l = p[x * step + (int64_t)M * a.D + M + r], lr = p[x * step + (int64_t)M * a.D + 2 * M + r];
   const int ch = min(lane * 2, a.D - 2);
   float2 v[kMaxSplits / 4];
 #pragma unroll
   for (int i = 0; i < kMaxSplits / 4; ++i) v[i] = *reinterpret_cast<const float2 *>(p + min(i * 4 + wave, a.splits - 1) * step + (int64_t)r * a.D + ch);
   const float mx = wave_max(m);
   const float w = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mx);
-  const float sum = wave_sum(m == kNegInf ? 0.f : l * w);
+  const float sum = wave_sum(m == kNegInf ? 0.f : l * w), rounded = wave_sum(m == kNegInf ? 0.f : lr * w);
   float2 o = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < kMaxSplits / 4; ++i) {                     // a split that is not there has a factor of 0
@@ -808,7 +846,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
     o.x += sums[i][lane].x;
     o.y += sums[i][lane].y;
   }
-  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  const float inv = inverse(sum), inv_rounded = inverse(rounded);
   if (lane * 2 < a.D) {
     const int64_t at = (int64_t)b * a.so.b + (int64_t)token * a.so.n + (int64_t)head * a.so.h + ch;
     T *y = reinterpret_cast<T *>(a.out) + at, *lo = reinterpret_cast<T *>(a.lo) + at;
@@ -817,8 +855,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int M) {
     y[0] = y0;
     y[1] = y1;
     if (sizeof(T) == 2 && a.lo) {
-      lo[0] = (T)(z0 - (float)y0);
-      lo[1] = (T)(z1 - (float)y1);
+      lo[0] = (T)(o.x * inv_rounded - (float)y0);
+      lo[1] = (T)(o.y * inv_rounded - (float)y1);
     }
   }
   if (lane == 0 && a.lse) put_statistics<T>(a, ((int64_t)b * a.Hq + head) * a.Nq + token, mx, sum, inv);
@@ -1440,11 +1478,11 @@ template <typename K> static int launch(K kernel, size_t lds, int64_t blocks, co
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, s, a);
   return check_launch(what);
 }
-template <typename T, int DP> static int launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t s) {
+template <typename T, int DP, bool LO> static int launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t s) {
   const char *what = "block_attention";
-  if (a.rows <= kFewRows) return launch(attend_few_kernel<T, DP, (sizeof(T) == 4 && DP > 64 ? 2 : 4)>, FewTile<T, DP>::body + list_bytes(a), blocks, a, s, what);
-  if constexpr (sizeof(T) == 4) return launch(attend_fwd_kernel<T, DP, 16, 4, 1, 2>, FwdTile<T, DP, 16, 4, 1, 2>::body + list_bytes(a), blocks, a, s, what);
-  else return launch(attend_fwd_kernel<T, DP, 32, 2, 2, 1>, FwdTile<T, DP, 32, 2, 2, 1>::body + list_bytes(a), blocks, a, s, what);
+  if (a.rows <= kFewRows) return launch(attend_few_kernel<T, DP, (sizeof(T) == 4 && DP > 64 ? 2 : 4), LO>, FewTile<T, DP>::body + list_bytes(a), blocks, a, s, what);
+  if constexpr (sizeof(T) == 4) return launch(attend_fwd_kernel<T, DP, 16, 4, 1, 2, LO>, FwdTile<T, DP, 16, 4, 1, 2>::body + list_bytes(a), blocks, a, s, what);
+  else return launch(attend_fwd_kernel<T, DP, 32, 2, 2, 1, LO>, FwdTile<T, DP, 32, 2, 2, 1>::body + list_bytes(a), blocks, a, s, what);
 }
 template <typename T, int DP, bool TWO> static int launch_dq(AttnArgs a, hipStream_t s) {
   const char *what = "block_attention backward (queries)";
@@ -1488,7 +1526,7 @@ template <typename T, int DP, bool TWO> static int launch_dkv(const AttnArgs &a,
     default: return CALL(T, 128);                                 \
   }
 template <typename T> static int fwd_by_dim(const AttnArgs &a, int64_t blocks, hipStream_t s) {
-#define CALL(T, DP) (launch_fwd<T, DP>(a, blocks, s))
+#define CALL(T, DP) (sizeof(T) == 2 && a.lo ? launch_fwd<T, DP, sizeof(T) == 2>(a, blocks, s) : launch_fwd<T, DP, false>(a, blocks, s))
   TCL_BY_DIM(T, CALL)
 #undef CALL
 }
@@ -1543,7 +1581,7 @@ static FwdPlan fwd_plan(const AttnArgs &a, bool f32) {
   int64_t n = cdiv(2 * kNumCU, p.works > 0 ? p.works : 1);
   if (n > tiles / 2) n = tiles / 2;
   p.splits = (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
-  p.part = p.splits > 1 ? round_up((size_t)p.works * p.splits * fwd_rows(a) * (a.D + 2) * 4, 256) : 0;
+  p.part = p.splits > 1 ? round_up((size_t)p.works * p.splits * fwd_rows(a) * (a.D + 3) * 4, 256) : 0;
   return p;
 }
 static bool rows16(const void *p, const Str &s, int dtype) {

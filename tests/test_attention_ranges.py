@@ -263,3 +263,32 @@ def test_output_and_what_its_rounding_took(nq, nk, q_block, dtype):
     # the remainder's own rounding (h of at most h of the output), 1 / 3, the product and the three-term sum in fp32 (of terms up to the largest value)
     tol = h * h * want.abs() + 4 * 2.0 ** -24 * v[:, at].double().abs().amax(1, keepdim=True)
     assert ((out.double() + lo.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nk,d,q_block", [(16, 64, 64), (100, 128, 64), (1000, 64, 64), (700, 64, 1)])
+@pytest.mark.parametrize("kind", ["mean 5", "mean 50", "no negative ones", "large scores"])
+def test_gradients_of_values_with_a_common_part(kind, nk, d, q_block, dtype):
+    """Values (and cotangents) of one sign or with a mean, and rows with one key of nearly all weight: rowsum(dout o out) and dout v^T are large and nearly the same.  The
+    forward's roundings of the probabilities come into their difference by the values' distances from the output alone, that of what is kept of
+    the output by h^2 of it."""
+    g = torch.Generator().manual_seed(nk + d)
+    nq, h = 256, half(dtype)
+    size = 30.0 if kind == "large scores" else 1.5
+    q, k, v, do = rnd(g, nq, d, scale=size), rnd(g, nk, d), rnd(g, nk, d), rnd(g, nq, d)
+    if kind.startswith("mean"):
+        v = v + float(kind[5:])
+    if kind == "no negative ones":
+        v, do = v.relu(), do.abs()
+    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
+    dq, dk, _ = gradients(q, k, v, do, q_block)
+    Q, K, V, G = (t.to(DEV).double() for t in (q, k, v, do))
+    c = d ** -0.5
+    p, t, ds = dense(Q, K, V, G, c)
+    delta = (p * t).square().sum(-1, keepdim=True) + h * h * (G * (p @ V)).square().sum(-1, keepdim=True)     # variance over h^2 / 3
+    delta = delta * c * c
+    for name, got, want, var in (("dq", dq, ds @ K, delta * (p @ K).square()), ("dk", dk, ds.T @ Q, (p * p * delta).T @ Q.square())):
+        own = own_rounding(want, dtype)
+        bound, err = 1.1 * (own ** 2 + h * h / 3 * var.sum().item()) ** 0.5, (got - want).norm().item()
+        assert err <= bound, "%s: %.2f times its own rounding, bound %.2f" % (name, err / own, bound / own)
