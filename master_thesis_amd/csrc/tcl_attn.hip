@@ -166,8 +166,8 @@ template <int S> __device__ __forceinline__ bool key_seen(unsigned part, int row
 // fp16 steps are absolute below 2^-14, so a probability is scaled up as an operand: in the forward, where those of a row are exp2(score - reference), by
 // 2^10 (unscaled, the tail of a long row is lost: 131,068 keys with 2^-25.2 of the largest each are 0.4 % of its weight and came out as zeros; scaled,
 // each loses 2^-35 of the largest at most), in the backward, where P <= 1, by 2^14.
-template <typename T> struct PScale { static constexpr float room = 8.f, fwd = 0.f, bits = 0.f, inv = 1.f; };
-template <> struct PScale<_Float16> { static constexpr float room = 4.f, fwd = 10.f, bits = 14.f, inv = 0x1p-14f; };
+template <typename T> struct PScale { static constexpr float room = 8.f, fwd = 0.f, up = 1.f, inv = 1.f; };
+template <> struct PScale<_Float16> { static constexpr float room = 4.f, fwd = 10.f, up = 0x1p14f, inv = 0x1p-14f; };
 
 // The running maximum need not be the maximum: any reference r with the scores at most `room` above it (in log2 units) keeps exp2(score - r) <= 256
 // (fp16: 16, scaled 2^14) far from every type's limits, and it costs no accuracy, since all sums are of floating-point numbers.  So the sums and outputs so
@@ -1313,8 +1313,8 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(AttnArgs a) {
           }
         }
         tab[r] = where;
-        refs[r] = ref - PScale<T>::bits;
-        weights[r] = weight;
+        refs[r] = ref;
+        weights[r] = weight * PScale<T>::up;                     // not into ref, which may be too large to take it
         delta[r] = de;
       }
       __syncthreads();

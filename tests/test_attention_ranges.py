@@ -195,7 +195,7 @@ def test_gradients_with_few_terms_are_exact_alone_and_in_a_batch(b, nq, nk, d, d
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("size,dtype", [(s, t) for s in (20.0, 100.0, 1e3, 1e4, 1e6, 1e8) for t in (torch.float32, torch.bfloat16, torch.float16)
-                                        if s <= 1e4 or t != torch.float16])      # larger queries are no fp16 numbers
+                                        if s <= 1e6 or t != torch.float16])      # fp16: scores of up to 2 10^7
 def test_gradients_under_large_scores(size, dtype):
     """Scores up to many times 10^8: the softmax is one key in the end, and its value gets the whole cotangent.  As exact as the same formulas in plain fp32
     products (scores of either side are rounded alike), and a few roundings: of P, its weight and the product."""
@@ -213,6 +213,31 @@ def test_gradients_under_large_scores(size, dtype):
             continue
         err, floor = ((x - want).norm().item() / want.norm().item() for x in (got, near.to(dtype).double()))
         assert err <= 1.5 * floor + 4 * 2.0 ** -24, "%s: error %.3g, plain %.3g" % (name, err, floor)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_block", [1, 64])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 1.6e7), (torch.float16, 4e7), (torch.bfloat16, 1e9), (torch.float32, 1e9)])
+def test_the_largest_scores(dtype, size, q_block):
+    """All scores near `size`, one far above the rest: its value is the output, and its value's gradient the sum of the cotangents."""
+    g = torch.Generator().manual_seed(13)
+    n, d = 512, 64
+    q, k = (torch.full((n, d), (8 * size / d) ** 0.5).to(dtype) for _ in range(2))
+    k[77] *= 1.0625
+    v, do = rnd(g, n, d, dtype=dtype), rnd(g, n, d, dtype=dtype)
+    blocks = torch.arange(8, device=DEV).int().expand(1, 1, n // q_block, 8).contiguous()
+    leaves = [t.to(DEV)[None, :, None].requires_grad_(True) for t in (q, k, v)]
+    out = A.block_attention(*leaves, blocks, q_block=q_block)
+    dv, = torch.autograd.grad(out, leaves[2], do.to(DEV)[None, :, None])
+    h = half(dtype)
+    want = v[77].to(DEV).double()
+    assert ((out[0, :, 0].double() - want).abs() <= 2 * h * want.abs() + 2.0 ** -22).all()
+    total = do.to(DEV).double().sum(0)
+    near = (2 * h * do.to(DEV).double().square().sum(0).sqrt() * 6 + 2 * h * total.abs() + 2.0 ** -24 * n * do.to(DEV).double().abs().sum(0))
+    assert ((dv[0, 77, 0].double() - total).abs() <= near).all()
+    rest = dv[0, :, 0].clone()
+    rest[77] = 0
+    assert rest.abs().max() == 0
 
 
 @pytest.mark.gpu
