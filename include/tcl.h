@@ -292,9 +292,10 @@ int tcl_select_blocks(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, c
 /*   out = softmax(scale q k^T) v over the visible keys of the blocks chosen for the query's group; a query that sees no key gets 0 and
  *   lse = -inf.  visible as in tcl_block_means; blocks (B,Hkv,S,top_k) int32: an index outside [0, nb) is no block, a repeated one
  *   counts once, order does not matter.  lse (B,Hq,Nq) fp32, natural logarithm, nullable (the backward pass needs it).  out_lo (16-bit
- *   types, nullable): laid out like out, what its rounding took from it, for the backward pass.  With TCL_DT_STATISTICS two more tensors
+ *   types, nullable): laid out like out, what the backward pass adds to it (its rounding, and what that of the probabilities did).  With TCL_DT_STATISTICS two more tensors
  *   (B,Hq,Nq) fp32 lie behind lse, for the backward pass, which else takes the probabilities from lse (exact to |lse| 2^-24): a reference in log2 units
  *   (+inf where nothing is seen) and one over the sum of exp2(score log2(e) - reference).
+ *   Scores (scale q k) below 10^9, fp16 2 10^7: beyond, exp2 of a rounded difference may overflow to NaN.
  *   Limits: top_k <= 2048, nb <= 65,536, q_block * G <= 2^20 (q_block beyond Nq counts as Nq); scale finite, of any sign.
  *   Contents of invisible keys do not matter (NaN and infinities included).  A workspace of 0 bytes may be NULL. */
 size_t tcl_block_attention_fwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int64_t top_k, int64_t block,

@@ -513,8 +513,8 @@ __device__ __forceinline__ void join_sets(const AttnArgs &a, char *smem, const t
 // running maximum, sum and output for its S KU keys of each tile, joined at the end, so the only meeting of the waves in the loop is
 // the hand-over of the tile.
 // Measured: 32 x 1,590 tokens x 2 heads against 2,048 of 15,900 keys of 64 bf16 channels 115 us (464 TFLOP/s; a large product reaches
-// 1,261), 4 x 6,360 x 2 against 4,096 of 63,600 of 128 channels 221 us (483), 2 x 4,096 x 4 against 1,024 of 16,384 of 64 fp32 channels 101
-// us (85 of 154).  By counters (128 channels) the vector unit is busy 40 % of the time, the matrix pipe 21 %, with 1.34 of the 2 waves that a
+// 1,261), 4 x 6,360 x 2 against 4,096 of 63,600 of 128 channels 222 us (481, a training step's), 2 x 4,096 x 4 against 1,024 of 16,384 of 64 fp32 channels 101
+// us (85 of 154).  By counters (128 channels) the vector unit is busy 32 % of the time, the matrix pipe 21 %, with 1.35 of the 2 waves that a
 // SIMD has room for: equal pieces of work do not fill the last round of the GPU (800 workgroups on 512 places).  Idle lanes for hidden
 // rows, in place of a choice of addresses, save a tenth of the vector instructions and lose 3 %.
 template <typename T, int DP, int S, int WM, int WN, int KU> struct FwdTile {
@@ -895,8 +895,7 @@ template <int S, typename V, int N, typename O, int DT> __device__ __forceinline
 
 // TWO: what rounding takes from a 16-bit operand (a score gradient; for dV a probability) is multiplied too.  Rounded once, it adds an error of the size of the
 // result's own rounding: together 1.46 times that.  Where a sum has few terms, or a tensor few sums, the roundings do not average out
-// (items of 8 queries up to 2.3, of 300 up to 1.58; 100 keys, one of them with most of the weight, up to 1.67), and below 64 channels they lie along the sum: there both
-// parts are taken (1.0 to 1.1, with one dominant key up to 1.4).  The rule looks at the sums of one item: whatever shares a call with it does not matter.
+// (items of 8 queries up to 2.3, of 300 up to 1.58), and below 64 channels they lie along the sum: there both parts are taken (1.00 to 1.06).  The rule looks at the sums of one item: whatever shares a call with it does not matter.
 // Two parts throughout would cost dq 248 -> 299 us, dk and dv 415 -> 487 (training step of 63,600 bf16 keys).
 constexpr int64_t kFewKeys = 512, kFewQueries = 2048;
 template <typename T> static bool two_parts(const AttnArgs &a) {
@@ -978,7 +977,7 @@ __global__ __launch_bounds__(1024) void attend_order_kernel(AttnArgs a) {
   for (int j = threadIdx.x; j < a.nb; j += 1024) order[atomicAdd(&start[cls(cnt[j])], 1u)] = j;
 }
 
-// The forward's tiles with two products for one: 247 us (648 TFLOP/s) for the training step of 63,600 keys, fp32 134 us (96).
+// The forward's tiles with two products for one: 244 us (656 TFLOP/s) for the training step of 63,600 keys, fp32 133 us (97).
 template <typename T, int DP, int S, int WM, int WN> struct DqTile {
   static constexpr int KU = 32 / S, M = S * WM, TK = 32 * WN, LO = DP + 4;             // 32 keys a wave
   static constexpr size_t img = (size_t)TK * Img<T, DP>::RB, tiles = 4 * img;          // K and V, twice
@@ -1160,8 +1159,8 @@ __global__ __launch_bounds__(256, OCC) void attend_dq_kernel(AttnArgs a) {
 // as a stream (group after group, in ascending order) in tiles of 32; rows and keys have changed places with the forward:
 // S = Q K^T leaves a lane the probabilities of ITS key, the operand of dV^T = dout^T P and, as dS, of dK^T = Q^T dS.
 // 16 keys a wave: with 32 (half the LDS reads per product) the two accumulators take 350 registers, one wave per SIMD, and
-// every wait shows (802 against 594 us then for the training step of 63,600 keys, 412 now: 518 TFLOP/s; fp32 as in the forward 188 us, 92).
-// LDS is busy 40 % of the time, the vector unit 32 %, the matrix pipe 24 %.  Rows lie scattered, so their tiles come from a ring
+// every wait shows (802 against 594 us then for the training step of 63,600 keys, 416 now: 513 TFLOP/s; fp32 as in the forward 189 us, 91).
+// LDS is busy 41 % of the time, the vector unit 32 %, the matrix pipe 23 %.  Rows lie scattered, so their tiles come from a ring
 // of four, three tiles ahead; where the rows lie is worked out for 512 of them at a time, not in the loop.
 constexpr int kWindow = 32;    // words of group bits taken at a time: up to 1024 groups in the list
 constexpr int kBatch = 512;    // rows located at a time
